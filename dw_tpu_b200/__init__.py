@@ -10,6 +10,12 @@ names:
 * ``e8m0_encode`` / ``e8m0_decode``
 * ``route_topk``, ``MoELayer`` / ``fused_moe_func``
 
+and the operators of a transformer block around that layer:
+
+* ``route_grouped_topk``  routing limited to the best groups of experts
+* ``dense_matmul``        a product with bias, activation and residual (router, shared expert)
+* ``pre_norm`` / ``post_norm``  the norms around the block, with its gate and residual
+
 Importing the package checks that the library has been built and raises if
 it is missing; the library itself is mapped on the first op call. There is no
 CPU or library fallback.
@@ -19,6 +25,8 @@ from . import _lib
 
 _lib.require_built()
 
+from .block_norm import post_norm, pre_norm  # noqa: E402
+from .dense import dense_matmul  # noqa: E402
 from .e8m0_scale import e8m0_decode, e8m0_encode  # noqa: E402
 from .fused_moe import FP4MoEWeights, MoELayer, fused_moe_func  # noqa: E402
 from .gmm_v2 import (b200_to_e2m1, codes_to_e2m1, decode_codes, e2m1_to_codes,  # noqa: E402
@@ -27,7 +35,7 @@ from .moe_fast_combine import (combine_pallas, combine_shared, combine_xla,  # n
                                fast_combine)
 from .moe_fast_dispatch import (dispatch_gather, dispatch_gather_pallas,  # noqa: E402
                                 fast_dispatch_gather, moe_permute, sorted_token_indices)
-from .routing import dedupe_topk, route_hash, route_topk  # noqa: E402
+from .routing import dedupe_topk, route_grouped_topk, route_hash, route_topk  # noqa: E402
 
 __all__ = [
     "gmm_v2", "gmm", "gmm_wrapper", "e2m1_to_codes", "codes_to_e2m1", "decode_codes",
@@ -35,4 +43,5 @@ __all__ = [
     "sorted_token_indices", "moe_permute", "dispatch_gather", "dispatch_gather_pallas",
     "fast_combine", "combine_xla", "combine_pallas", "combine_shared", "e8m0_encode", "e8m0_decode",
     "route_topk", "route_hash", "dedupe_topk", "MoELayer", "FP4MoEWeights", "fused_moe_func",
+    "route_grouped_topk", "dense_matmul", "pre_norm", "post_norm",
 ]

@@ -32,6 +32,9 @@ U8 = 2
 ACT_NONE = 0
 ACT_SWIGLU = 1
 ACT_SWIGLU_CLAMP = 2
+ACT_SILU = 3
+ACT_GELU = 4
+ACT_GELU_TANH = 5
 FP4_E2M1 = 0
 FP4_TOKAMAX = 1
 FP4_B200 = 2
@@ -39,6 +42,14 @@ LAYOUTS = {"e2m1": FP4_E2M1, "b200": FP4_B200}
 SCORE_SOFTMAX = 0
 SCORE_SIGMOID = 1
 SCORE_SQRTSOFTPLUS = 2
+GROUP_MAX = 0
+GROUP_TOP2 = 1
+NORM_RMS = 0
+NORM_LAYER = 1
+GATE_NONE = 0
+GATE_TOKEN = 1
+GATE_CHANNEL = 2
+GATE_FULL = 3
 LAYER_SCRATCH_BYTES = 33554432  # DWM_LAYER_SCRATCH_BYTES
 EP_HANDLE_BYTES = 64
 EP_COUNTS = 1
@@ -77,6 +88,12 @@ SIGNATURES = {
     "dwm_e8m0_decode": ([_P, _SZ, _P, _P], _I),
     "dwm_route_topk": ([_P, _I, _I, _I, _I, _I, _I, _P, _I, _P, _P, _P, _P], _I),
     "dwm_route_hash": ([_P, _I, _I, _I, _I, _I, _I, _P, _I, _P, _P, _P, _P], _I),
+    "dwm_route_grouped_topk": ([_P, _I, _I64, _I, _I, _I, _I, _I, _I, _I, _I, _F, _P, _I, _P, _P,
+                                _P, _P], _I),
+    "dwm_dense_matmul": ([_P, _I64, _P, _I64, _I, _I, _I, _P, _I, _I, _F, _P, _I, _I64, _F, _P,
+                          _I, _I64, _P], _I),
+    "dwm_block_norm": ([_P, _I, _I64, _P, _I, _I64, _I, _I, _I, _F, _I, _P, _P, _P, _I, _I, _I64,
+                        _F, _F, _P, _P, _I, _P, _I64, _P, _I, _I64, _P], _I),
     "dwm_dedupe_topk": ([_P, _P, _I, _I, _I, _P, _P], _I),
     "dwm_sorted_token_indices": ([_P, _I64, _I, _P, _P], _I),
     "dwm_permute": ([_P, _I, _I, _I, _P, _P, _P, _P, _P], _I),

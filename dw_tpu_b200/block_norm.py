@@ -1,0 +1,53 @@
+"""The norms before and after a block on B200, fused with the block's gate, its
+scale and the residual's scale."""
+
+from __future__ import annotations
+
+import torch
+
+from . import ops
+
+
+def pre_norm(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *,
+             eps: float = 1e-6, kind: str = "rms", out_dtype: torch.dtype = torch.bfloat16,
+             out: torch.Tensor | None = None) -> torch.Tensor:
+    """The norm before a block: ``norm(x) * weight (+ bias)`` of x [t, h] (bf16
+    or f32), ``kind`` "rms" or "layer"; statistics in f32. ``out`` (which may
+    be ``x``) is written and returned if given. Inference only: no gradient."""
+    ops.no_grad_needed(x, weight, bias)
+    if out is None:
+        out = torch.empty(x.shape, dtype=out_dtype, device=x.device)
+    ops.block_norm_out(x, out, weight=weight, bias=bias, eps=eps, kind=kind)
+    return out
+
+
+def post_norm(y: torch.Tensor, residual: torch.Tensor, *,
+              norm_weight: torch.Tensor | None = None, norm_bias: torch.Tensor | None = None,
+              gate: torch.Tensor | None = None, scale: float = 1.0, residual_scale: float = 1.0,
+              next_weight: torch.Tensor | None = None, next_bias: torch.Tensor | None = None,
+              eps: float = 1e-6, kind: str = "rms", out_dtype: torch.dtype = torch.bfloat16,
+              residual_out: torch.Tensor | None = None, out: torch.Tensor | None = None):
+    """After a block with output y [t, h], in one pass:
+
+        r = residual_scale * residual + scale * gate * norm(y)
+        h = norm(r)
+
+    Returns (r in residual's dtype, h in ``out_dtype``). norm(y) has
+    ``norm_weight`` / ``norm_bias`` and is y itself without a weight; h has
+    ``next_weight`` / ``next_bias`` (the next block's ``pre_norm``) and is None
+    without a weight. gate: one value a token [t, 1], a channel [h], or an
+    element [t, h]. h is formed from the f32 r. ``residual_out`` may be
+    ``residual`` (the stream updated in place) and ``out`` may be ``y``.
+    Inference only: no gradient."""
+    ops.no_grad_needed(y, residual, norm_weight, norm_bias, gate, next_weight, next_bias)
+    if residual_out is None:
+        residual_out = torch.empty(residual.shape, dtype=residual.dtype, device=residual.device)
+    if next_weight is None:
+        if out is not None or next_bias is not None:
+            raise ValueError("out and next_bias need next_weight")
+    elif out is None:
+        out = torch.empty(residual.shape, dtype=out_dtype, device=residual.device)
+    ops.block_norm_out(residual, out, weight=next_weight, bias=next_bias, y=y,
+                       r_out=residual_out, norm_weight=norm_weight, norm_bias=norm_bias,
+                       gate=gate, scale=scale, residual_scale=residual_scale, eps=eps, kind=kind)
+    return residual_out, out

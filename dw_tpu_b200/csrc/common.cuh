@@ -35,6 +35,30 @@ int set_smem_limit(const void* kernel, int bytes, const char* what);
 // must not outlive a context.
 int current_context(void** ctx);
 
+// The memory of `rows` rows of `width` bytes, `ld` bytes apart.
+struct RowSpan {
+  uintptr_t at;
+  int64_t rows, width, ld;
+};
+inline RowSpan row_span(const void* p, int64_t rows, int64_t cols, int64_t ld, int element_size) {
+  return {reinterpret_cast<uintptr_t>(p), p ? rows : 0, cols * element_size, ld * element_size};
+}
+// Whether two of them share a byte. Columns of one wider tensor (rows equally
+// far apart) are told apart; rows of unlike distances count as overlapping
+// where their extents do.
+inline bool rows_overlap(const RowSpan& p, const RowSpan& q) {
+  if (p.rows <= 0 || q.rows <= 0) return false;
+  const uintptr_t p_end = p.at + (uintptr_t)((p.rows - 1) * p.ld + p.width);
+  const uintptr_t q_end = q.at + (uintptr_t)((q.rows - 1) * q.ld + q.width);
+  if (p_end <= q.at || q_end <= p.at) return false;
+  if (p.rows == 1 && q.rows == 1) return true;
+  const int64_t ld = p.rows > 1 ? p.ld : q.ld;
+  if ((p.rows > 1 && q.rows > 1 && p.ld != q.ld) || p.width > ld || q.width > ld) return true;
+  int64_t d = (int64_t)(q.at - p.at) % ld;  // q's first byte within p's rows
+  if (d < 0) d += ld;
+  return d < p.width || d + q.width > ld;
+}
+
 #define DWM_CHECK_ARG(cond, ...)                                   \
   do {                                                             \
     if (!(cond)) return ::dwm::set_error(DWM_ERR_INVALID, __VA_ARGS__); \

@@ -1,0 +1,48 @@
+"""Dense products of the MoE block on B200: the router's logits and the shared
+expert's projections, with bias, activation and residual in the epilogue."""
+
+from __future__ import annotations
+
+import torch
+
+from . import _lib as L
+from . import ops
+
+_ACTS = {None: L.ACT_NONE, "silu": L.ACT_SILU, "gelu": L.ACT_GELU,
+         "gelu_tanh": L.ACT_GELU_TANH, "swiglu": L.ACT_SWIGLU,
+         "swiglu_clamp": L.ACT_SWIGLU_CLAMP}
+
+
+def dense_matmul(x: torch.Tensor, w: torch.Tensor, *, bias: torch.Tensor | None = None,
+                 act: str | None = None, act_limit: float | None = None,
+                 residual: torch.Tensor | None = None, residual_scale: float = 1.0,
+                 out_dtype: torch.dtype | None = None,
+                 out: torch.Tensor | None = None) -> torch.Tensor:
+    """``residual_scale * residual + act(x @ w.T + bias)``, rounded once.
+
+    x bf16 [m, k]; w bf16 [n, k] (a Linear layer's layout); k a multiple of 8,
+    rows of both on 16 bytes. ``act``: None, "silu", "gelu" (erf), "gelu_tanh",
+    each element by itself, or "swiglu" / "swiglu_clamp" on the [gate | up]
+    halves of n (then the result has n / 2 columns; the clamp is gate <=
+    ``act_limit``, |up| <= ``act_limit``). Note that ``gmm_v2``'s ``fuse_act``
+    calls SwiGLU "silu". bias [n], residual and the result [m, n or n / 2] are
+    bf16 or f32; ``out_dtype`` is bf16 by default. ``out`` (which may be
+    ``residual``) is written and returned if given. Inference only: no
+    gradient."""
+    if act not in _ACTS:
+        raise ValueError(f"act {act!r} not supported (one of {sorted(k for k in _ACTS if k)})")
+    code = _ACTS[act]
+    if code == L.ACT_SWIGLU_CLAMP and act_limit is None:
+        raise ValueError("swiglu_clamp needs act_limit")
+    ops.no_grad_needed(x, w, bias, residual)
+    if out is None:
+        if x.dim() != 2 or w.dim() != 2:
+            raise ValueError("x and w must be 2-D")
+        n = w.shape[0]
+        if code in (L.ACT_SWIGLU, L.ACT_SWIGLU_CLAMP):
+            n //= 2
+        out = torch.empty((x.shape[0], n), dtype=out_dtype or torch.bfloat16, device=x.device)
+    elif out_dtype is not None and out.dtype != out_dtype:
+        raise ValueError(f"out is {out.dtype}, out_dtype {out_dtype}")
+    return ops.dense_matmul_out(x, w, out, bias=bias, act=code, act_limit=act_limit or 0.0,
+                                residual=residual, residual_scale=residual_scale)

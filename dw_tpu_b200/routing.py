@@ -32,6 +32,39 @@ def route_topk(gating_output: torch.Tensor, top_k: int, renormalize: bool = True
     return w32.to(dtype), ids
 
 
+def route_grouped_topk(gating_output: torch.Tensor, top_k: int, num_groups: int,
+                       topk_groups: int, renormalize: bool = True, scoring_fn: str = "sigmoid",
+                       group_score: str = "top2", routed_scale: float = 1.0,
+                       dtype: torch.dtype = torch.bfloat16, bias: torch.Tensor | None = None,
+                       num_valid_tokens: int | None = None):
+    """Group-limited ``route_topk``: (topk_weights in ``dtype``, topk_ids int32).
+
+    The experts are ``num_groups`` (at most 32) groups of consecutive ones; the
+    ``topk_groups`` best groups stay open and the ``top_k`` best experts are
+    chosen in them, best first, ties to the lower index. An expert's choice
+    value is its score plus ``bias`` (the balance bias: selection only), a
+    group's the best choice in it (``group_score="max"``) or the sum of its two
+    best ("top2"). The weights are the scores, divided by their sum if
+    ``renormalize``, times ``routed_scale``. Selection is that of 64-bit scores
+    whatever the logits' dtype. Inference only: no gradient."""
+    logits = gating_output
+    if logits.dtype not in (torch.bfloat16, torch.float32):
+        logits = logits.float()
+    ops.no_grad_needed(logits, bias)
+    t = logits.shape[0]
+    ids = torch.empty((t, top_k), dtype=torch.int32, device=logits.device)
+    narrow = dtype == torch.bfloat16
+    w = torch.empty((t, top_k), dtype=torch.bfloat16 if narrow else torch.float32,
+                    device=logits.device)
+    ops.route_grouped_topk_out(logits, top_k, num_groups, topk_groups, ids,
+                               None if narrow else w, w if narrow else None,
+                               scoring_fn=scoring_fn, group_score=group_score,
+                               renormalize=renormalize, routed_scale=routed_scale,
+                               bias=None if bias is None else bias.float().contiguous(),
+                               num_valid_tokens=num_valid_tokens)
+    return w.to(dtype), ids
+
+
 def route_hash(gating_output: torch.Tensor, hash_ids: torch.Tensor, renormalize: bool = True,
                scoring_fn: str = "sigmoid", dtype: torch.dtype = torch.bfloat16,
                num_valid_tokens: int | None = None):

@@ -50,6 +50,10 @@ extern "C" {
 #define DWM_ACT_SWIGLU 1       /* silu(gate) * up on [gate | up] halves */
 #define DWM_ACT_SWIGLU_CLAMP 2 /* gate = min(gate, L), up = clip(up, -L, L) */
 
+#define DWM_ACT_SILU 3         /* dense product only, element by element: v * sigmoid(v) */
+#define DWM_ACT_GELU 4         /* v * Phi(v), by erf */
+#define DWM_ACT_GELU_TANH 5    /* its tanh form */
+
 #define DWM_FP4_E2M1 0    /* OCP e2m1 nibbles (sign | e1 e0 | m) */
 #define DWM_FP4_TOKAMAX 1 /* tokamax codes q = sign*(2e+m), int4 two's compl. */
 #define DWM_FP4_B200 2    /* the B200 load-time layout (dwm_fp4_to_b200):
@@ -62,6 +66,17 @@ extern "C" {
 #define DWM_SCORE_SOFTMAX 0
 #define DWM_SCORE_SIGMOID 1
 #define DWM_SCORE_SQRTSOFTPLUS 2
+
+#define DWM_GROUP_MAX 0  /* a group's value: its best expert's choice */
+#define DWM_GROUP_TOP2 1 /* the sum of its two best experts' choices */
+
+#define DWM_NORM_RMS 0
+#define DWM_NORM_LAYER 1
+
+#define DWM_GATE_NONE 0
+#define DWM_GATE_TOKEN 1   /* gate [t] (row stride ldg) */
+#define DWM_GATE_CHANNEL 2 /* gate [h] */
+#define DWM_GATE_FULL 3    /* gate [t, h] (row stride ldg) */
 
 /* ---- library ------------------------------------------------------------ */
 const char* dwm_version(void);
@@ -198,6 +213,27 @@ int dwm_route_hash(const void* logits, int logits_dtype, int t, int e, int top_k
 int dwm_dedupe_topk(float* topk_weights_f32, int32_t* topk_ids, int t, int top_k,
                     int num_experts, void* topk_weights_bf16, void* stream);
 
+/* Group-limited top-k routing. The e experts are num_groups (at most 32)
+ * groups of e / num_groups consecutive ones. With s = the scores of
+ * dwm_route_topk and c = s + bias (the choice), a group's value is its largest
+ * c (DWM_GROUP_MAX) or the sum of its two largest (DWM_GROUP_TOP2); the
+ * topk_groups groups of largest value stay open, and the top_k experts of
+ * largest c within them are chosen, in descending order. Ties, of groups and
+ * of experts, go to the lower index. The weights are s at the chosen experts,
+ * divided by their sum if renormalize (0 where that is 0), times
+ * routed_scale. The order is that of c in 64 bits (without bias, that of the
+ * logits, which is the same in exact arithmetic), so it does not depend on
+ * how f32 rounds nearly equal scores. A NaN choice ranks below every number;
+ * -inf logits have score 0. Rows >= num_valid_tokens (if >= 0) get expert 0
+ * with weight 0. e <= 1024, top_k <= min(32, topk_groups * e / num_groups).
+ * logits rows are ld_logits elements apart. The outputs are contiguous as in
+ * dwm_route_topk and must not overlap the inputs. */
+int dwm_route_grouped_topk(const void* logits, int logits_dtype, int64_t ld_logits, int t, int e,
+                           int top_k, int num_groups, int topk_groups, int scoring,
+                           int group_score, int renormalize, float routed_scale,
+                           const float* bias, int num_valid_tokens, int32_t* topk_ids,
+                           float* topk_weights_f32, void* topk_weights_bf16, void* stream);
+
 /* ---- permute / dispatch (KD, X0405:70-98) -------------------------------- */
 /* KD:41-44: out[j] = argsort[j] / topk. */
 int dwm_sorted_token_indices(const int32_t* topk_argsort, int64_t n, int topk, int32_t* out,
@@ -235,6 +271,46 @@ int dwm_combine_shared(const void* x, int x_dtype, int64_t x_rows, const int32_t
                        const void* w, int w_dtype, int t, int h, int topk, const void* shared,
                        int shared_dtype, float routed_scale, int mid_dtype, void* out,
                        int out_dtype, void* stream);
+
+/* ---- dense product with its epilogue --------------------------------------
+ *   out = residual_scale * residual + act(x w^T + bias)
+ * x bf16 [m, k] and w bf16 [n, k] (rows ldx and ldw elements apart; every row
+ * starts on 16 bytes: k, ldx and ldw are multiples of 8), products accumulated
+ * in f32, bias [n] (bf16 or f32, may be NULL), act one of DWM_ACT_* (SwiGLU on
+ * the [gate | up] halves of w's rows: n_out = n / 2, else n), residual
+ * [m, n_out] (bf16 or f32, rows ldr apart, may be NULL), out [m, n_out] (bf16
+ * or f32, rows ldo apart), everything after the products in f32, rounded once.
+ * out may be the residual itself; it must not overlap anything else. m, n and
+ * the strides of residual and out are free (rows that start on 16 bytes are
+ * stored faster). The result of a call depends on its shapes and values alone
+ * (no atomics). Router logits and shared expert of the MoE block; no
+ * counterpart in the reference, where both are outside this path. */
+int dwm_dense_matmul(const void* x, int64_t ldx, const void* w, int64_t ldw, int m, int n, int k,
+                     const void* bias, int bias_dtype, int act, float act_limit,
+                     const void* residual, int residual_dtype, int64_t ldr, float residual_scale,
+                     void* out, int out_dtype, int64_t ldo, void* stream);
+
+/* ---- the norms around a block ---------------------------------------------
+ * After the block and before the next, in one pass over the rows:
+ *   r = residual_scale * residual + scale * gate * n2(y)
+ *   h = n1(r)
+ * n(v) = (v - m) / sqrt(mean((v - m)^2) + eps) * w + b with m = 0
+ * (DWM_NORM_RMS) or m = mean(v) (DWM_NORM_LAYER); statistics, products and
+ * sums in f32, h from the f32 r, each output rounded once. y [t, h] (bf16 or
+ * f32) is the block's output, residual [t, h] and r_out share one dtype, h_out
+ * is bf16 or f32, w1 / b1 / w2 / b2 [h] share one; b1 and b2 may be NULL.
+ * inner = 0: n2 is the identity. h_out = NULL: no n1 (w1 unused). y = NULL:
+ * only h = n1(residual) (r_out NULL, no gate, inner = 0). ld*: row strides in
+ * elements, any; 16-byte loads are used where every row of every tensor starts
+ * on 16 bytes. An output may be one of y, residual and a full gate itself (same
+ * pointer, stride and element size); any other overlap is refused.
+ * 1 <= h <= 16384, eps > 0. No counterpart in the reference. */
+int dwm_block_norm(const void* y, int y_dtype, int64_t ldy, const void* residual,
+                   int residual_dtype, int64_t ldres, int t, int h, int kind, float eps,
+                   int inner, const void* w2, const void* b2, const void* gate, int gate_dtype,
+                   int gate_mode, int64_t ldg, float scale, float residual_scale,
+                   const void* w1, const void* b1, int w_dtype, void* r_out, int64_t ldr,
+                   void* h_out, int h_dtype, int64_t ldh, void* stream);
 
 /* ---- the single-device layer in one call ---------------------------------
  * fused_moe_func's GMM path (X0104:88-98, X0405, X0404 on one device):
