@@ -92,7 +92,7 @@ SIGNATURES = {
                                 _P, _P], _I),
     "dwm_dense_matmul": ([_P, _I64, _P, _I64, _I, _I, _I, _P, _I, _I, _F, _P, _I, _I64, _F, _P,
                           _I, _I64, _P], _I),
-    "dwm_block_norm": ([_P, _I, _I64, _P, _I, _I64, _I, _I, _I, _F, _I, _P, _P, _P, _I, _I, _I64,
+    "dwm_block_norm": ([_P, _I, _I64, _P, _I, _I64, _I, _I, _I, _F, _I, _P, _P, _P, _I, _I64,
                         _F, _F, _P, _P, _I, _P, _I64, _P, _I, _I64, _P], _I),
     "dwm_dedupe_topk": ([_P, _P, _I, _I, _I, _P, _P], _I),
     "dwm_sorted_token_indices": ([_P, _I64, _I, _P, _P], _I),

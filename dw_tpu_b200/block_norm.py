@@ -35,8 +35,8 @@ def post_norm(y: torch.Tensor, residual: torch.Tensor, *,
     Returns (r in residual's dtype, h in ``out_dtype``). norm(y) has
     ``norm_weight`` / ``norm_bias`` and is y itself without a weight; h has
     ``next_weight`` / ``next_bias`` (the next block's ``pre_norm``) and is None
-    without a weight. gate: one value a token [t, 1], a channel [h], or an
-    element [t, h]. h is formed from the f32 r. ``residual_out`` may be
+    without a weight. gate (y's dtype): one value a token [t, 1], a channel
+    [h], or an element [t, h]. h is formed from the f32 r. ``residual_out`` may be
     ``residual`` (the stream updated in place) and ``out`` may be ``y``.
     Inference only: no gradient."""
     ops.no_grad_needed(y, residual, norm_weight, norm_bias, gate, next_weight, next_bias)

@@ -13,6 +13,8 @@
 // Bound: memory. A row of each tensor is read once and written once, and
 // stays in registers between the two norms. One CTA takes one row (a warp,
 // rows of up to 1024 elements), each thread up to 32 of its elements.
+#include <algorithm>
+
 #include "common.cuh"
 
 namespace dwm {
@@ -21,11 +23,8 @@ namespace norm {
 struct Args {
   const void* y;      // NULL: no block output, h = n1(residual)
   const void* res;
-  const void* w2;     // n2's weight and bias; inner = 0: n2 is the identity
-  const void* b2;
-  const void* w1;     // n1's
-  const void* b1;
-  const void* gate;
+  const void* vec[4]; // weight and bias of n2 (inner = 0: n2 is the identity) and of n1
+  const void* gate;   // of y's type
   void* r_out;        // NULL without y
   void* h_out;        // NULL: no n1
   int64_t ldy, ldres, ldg, ldr, ldh;  // row strides in elements
@@ -33,216 +32,580 @@ struct Args {
   int inner;          // apply n2
   int layer;          // layer norm, else RMS norm
   int gate_mode;      // DWM_GATE_*
-  int w_f32, gate_f32, h_f32;
+  int y_f32, res_f32, w_f32, h_f32;
   float eps, scale, res_scale;
+  // Streaming kernel: a group's ring of stages, and where the residual's and
+  // the full gate's rows start in a stage.
+  int stages, stage_bytes, off_res, off_gate;
+  // Where the vectors lie in its shared memory, a channel's gate the fifth;
+  // 0 bytes apart: left in global memory.
+  int vec_bytes;
+  int* status;
 };
+constexpr int W2 = 0, B2 = 1, W1 = 2, B1 = 3, CHANNEL_GATE = 4;
 
-__device__ __forceinline__ float ld1(const void* p, int64_t i, bool f32) {
-  return f32 ? static_cast<const float*>(p)[i]
-             : bf16_bits_to_f32(static_cast<const uint16_t*>(p)[i]);
+// Element types known when the kernel is compiled, or when it runs.
+constexpr int BF = 0, FP = 1, ANY = 2;
+template <int D>
+__device__ __forceinline__ bool is_f32(int runtime) {
+  return D == ANY ? runtime != 0 : D == FP;
+}
+template <int D>
+__device__ __forceinline__ int bytes_of(int runtime) {
+  return is_f32<D>(runtime) ? 4 : 2;
 }
 
-// N consecutive elements as f32. N = 8: 16-byte loads (the caller has checked
-// the alignment); N = 1: one element.
-template <int N>
-__device__ __forceinline__ void ld(const void* p, int64_t i, bool f32, float (&v)[N]) {
-  if constexpr (N == 8) {
-    if (f32) {
-      const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
-      const float4 a = q[0], b = q[1];
-      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-      v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-    } else {
-      const uint4 q = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + i);
-      const uint32_t u[4] = {q.x, q.y, q.z, q.w};
+// A thread works on pairs of its elements (VEC = 1: on one element a pair).
+__host__ __device__ constexpr int pairs(int vec) { return vec == 1 ? 1 : vec / 2; }
+
+// A thread's CPT x VEC elements of a row as they were loaded. VEC = 8: one or
+// two 16-byte loads (the host has checked the alignment); VEC = 1: one element.
+// Element j of load c sits at column (i + c * threads) * VEC + j.
+template <int VEC, int CPT, int D>
+struct Raw {
+  static constexpr int W = VEC == 1 ? 1 : D == BF ? 4 : 8;  // words per load
+  uint32_t u[CPT][W];
+
+  // From global memory. One branch on the type for all loads, so that they
+  // are issued together.
+  __device__ __forceinline__ void load(const void* p, const int (&col)[CPT], int f32) {
+    if (is_f32<D>(f32)) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        v[2 * j] = __uint_as_float(u[j] << 16);
-        v[2 * j + 1] = __uint_as_float(u[j] & 0xFFFF0000u);
+      for (int c = 0; c < CPT; ++c) {
+        const uint8_t* q = static_cast<const uint8_t*>(p) + col[c] * 4;
+        if constexpr (VEC == 1) {
+          u[c][0] = *reinterpret_cast<const uint32_t*>(q);
+        } else {
+          put(c, 0, *reinterpret_cast<const uint4*>(q));
+          put(c, 4, *reinterpret_cast<const uint4*>(q + 16));
+        }
+      }
+    } else {
+#pragma unroll
+      for (int c = 0; c < CPT; ++c) {
+        const uint8_t* q = static_cast<const uint8_t*>(p) + col[c] * 2;
+        if constexpr (VEC == 1)
+          u[c][0] = *reinterpret_cast<const uint16_t*>(q);
+        else
+          put(c, 0, *reinterpret_cast<const uint4*>(q));
       }
     }
-  } else {
-    v[0] = ld1(p, i, f32);
   }
-}
-
-template <int N>
-__device__ __forceinline__ void st(void* p, int64_t i, bool f32, const float (&v)[N]) {
-  if constexpr (N == 8) {
-    if (f32) {
-      float4* q = reinterpret_cast<float4*>(static_cast<float*>(p) + i);
-      q[0] = make_float4(v[0], v[1], v[2], v[3]);
-      q[1] = make_float4(v[4], v[5], v[6], v[7]);
+  // From shared memory.
+  __device__ __forceinline__ void load_s(uint32_t p, const int (&col)[CPT], int f32) {
+    if (is_f32<D>(f32)) {
+#pragma unroll
+      for (int c = 0; c < CPT; ++c) {
+        const uint32_t q = p + (uint32_t)col[c] * 4;
+        if constexpr (VEC == 1) {
+          u[c][0] = lds_u32(q);
+        } else {
+          put(c, 0, lds_u128(q));
+          put(c, 4, lds_u128(q + 16));
+        }
+      }
     } else {
-      uint4 q;
-      q.x = f32_to_bf16_bits(v[0]) | (f32_to_bf16_bits(v[1]) << 16);
-      q.y = f32_to_bf16_bits(v[2]) | (f32_to_bf16_bits(v[3]) << 16);
-      q.z = f32_to_bf16_bits(v[4]) | (f32_to_bf16_bits(v[5]) << 16);
-      q.w = f32_to_bf16_bits(v[6]) | (f32_to_bf16_bits(v[7]) << 16);
-      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + i) = q;
+#pragma unroll
+      for (int c = 0; c < CPT; ++c) {
+        const uint32_t q = p + (uint32_t)col[c] * 2;
+        if constexpr (VEC == 1)
+          u[c][0] = lds_u16(q);
+        else
+          put(c, 0, lds_u128(q));
+      }
     }
-  } else {
-    if (f32)
-      static_cast<float*>(p)[i] = v[0];
+  }
+  __device__ __forceinline__ void put(int c, int w, const uint4& x) {
+    u[c][w % W] = x.x; u[c][(w + 1) % W] = x.y; u[c][(w + 2) % W] = x.z; u[c][(w + 3) % W] = x.w;
+  }
+  // Elements 2 j and 2 j + 1 of load c (VEC = 1: the one element, and 0).
+  template <bool F>
+  __device__ __forceinline__ F2 at(int c, int j) const {
+    if constexpr (VEC == 1)
+      return f2(__uint_as_float(F ? u[c][0] : u[c][0] << 16), 0.0f);
+    else if (F)
+      return f2(__uint_as_float(u[c][(2 * j) % W]), __uint_as_float(u[c][(2 * j + 1) % W]));
     else
-      static_cast<uint16_t*>(p)[i] = (uint16_t)f32_to_bf16_bits(v[0]);
+      return f2(__uint_as_float(u[c][j] << 16), __uint_as_float(u[c][j] & 0xFFFF0000u));
   }
-}
-
-// Sum over the threads of one row: a warp (warps == 1), or the whole CTA by
-// way of `part` (one slot a warp; summed in warp order by every thread, so
-// all threads hold the same bits). Each sum of a row has a `part` of its own,
-// so one barrier a sum is enough.
-__device__ __forceinline__ float row_sum(float v, int warps, float* part) {
-#pragma unroll
-  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  if (warps == 1) return v;
-  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
-  __syncthreads();
-  float s = 0.0f;
-  for (int w = 0; w < warps; ++w) s += part[w];
-  return s;
-}
-
-// VEC elements a load (8, or 1 for rows that are not 16-byte aligned), CPT
-// loads a thread: thread i of the row's TPR threads holds elements
-// (i + c * TPR) * VEC + [0, VEC). YF / RF: y and the residual are f32.
-template <int VEC, int CPT, bool YF, bool RF>
-__global__ void __launch_bounds__(512) block_norm_kernel(const Args a) {
-  __shared__ float part[4][32];
-  const int tpr = blockDim.x, warps = tpr >> 5;
-  const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
-  if (row >= a.t) return;  // whole warps of a one-warp-per-row CTA
-  const bool layer = a.layer != 0;
-  const float inv_h = 1.0f / (float)a.h;
-  bool in[CPT];
-  int col[CPT];
-  float v[CPT][VEC], res[CPT][VEC];
-#pragma unroll
-  for (int c = 0; c < CPT; ++c) {
-    col[c] = ((int)threadIdx.x + c * tpr) * VEC;
-    in[c] = col[c] < a.h;  // h is a multiple of VEC
-#pragma unroll
-    for (int q = 0; q < VEC; ++q) v[c][q] = res[c][q] = 0.0f;
-    if (in[c]) {
-      if (a.y) ld<VEC>(a.y, row * a.ldy + col[c], YF, v[c]);
-      ld<VEC>(a.res, row * a.ldres + col[c], RF, res[c]);
-    }
-  }
-
-  // mean and reciprocal root of the mean square of u over the row.
-  auto stats = [&](float (&u)[CPT][VEC], float* p0, float* p1, float& mean, float& rstd) {
-    mean = 0.0f;
-    if (layer) {
-      float s = 0.0f;
+  // v <- f(v, elements) for all pairs; again one branch on the type.
+  template <class F>
+  __device__ __forceinline__ void into(F2 (&v)[CPT][pairs(VEC)], int f32, const F& f) const {
+    if (is_f32<D>(f32)) {
 #pragma unroll
       for (int c = 0; c < CPT; ++c)
 #pragma unroll
-        for (int q = 0; q < VEC; ++q) s += u[c][q];
-      mean = row_sum(s, warps, p0) * inv_h;
+        for (int q = 0; q < pairs(VEC); ++q) v[c][q] = f(v[c][q], at<true>(c, q));
+    } else {
+#pragma unroll
+      for (int c = 0; c < CPT; ++c)
+#pragma unroll
+        for (int q = 0; q < pairs(VEC); ++q) v[c][q] = f(v[c][q], at<false>(c, q));
     }
-    float s2 = 0.0f;
+  }
+};
+
+template <int VEC>
+__device__ __forceinline__ void st(uint8_t* p, bool f32, const F2 (&v)[pairs(VEC)]) {
+  float e[2 * pairs(VEC)];
+#pragma unroll
+  for (int q = 0; q < pairs(VEC); ++q) f2_split(v[q], e[2 * q], e[2 * q + 1]);
+  if constexpr (VEC == 8) {
+    if (f32) {
+      float4* q = reinterpret_cast<float4*>(p);
+      q[0] = make_float4(e[0], e[1], e[2], e[3]);
+      q[1] = make_float4(e[4], e[5], e[6], e[7]);
+    } else {
+      *reinterpret_cast<uint4*>(p) =
+          make_uint4(f32x2_to_bf16x2(e[0], e[1]), f32x2_to_bf16x2(e[2], e[3]),
+                     f32x2_to_bf16x2(e[4], e[5]), f32x2_to_bf16x2(e[6], e[7]));
+    }
+  } else {
+    if (f32)
+      *reinterpret_cast<float*>(p) = e[0];
+    else
+      *reinterpret_cast<uint16_t*>(p) = (uint16_t)f32_to_bf16_bits(e[0]);
+  }
+}
+
+// The threads that share a row: `threads` of them (whole warps), this one the
+// `i`-th, barrier `bar` theirs alone. part: one slot a warp for each of a
+// row's (at most four) sums, so one barrier a sum is enough; 16-byte aligned,
+// the slots of absent warps zero.
+struct Group {
+  int i, threads, bar;
+  float (*part)[32];
+
+  __device__ __forceinline__ void sync() const {
+    if (threads == 32)
+      __syncwarp();
+    else
+      asm volatile("bar.sync %0, %1;" ::"r"(bar), "r"(threads) : "memory");
+  }
+  __device__ __forceinline__ void clear_parts() const {
+    for (int j = i; j < 128; j += threads) part[j / 32][j % 32] = 0.0f;
+  }
+  // Sum over the row's threads, in a fixed order: the same bits in all of
+  // them. between() runs after the barrier (with one warp a row: none).
+  template <class F>
+  __device__ __forceinline__ float sum(float v, int slot, const F& between) const {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if (threads == 32) {
+      between();
+      return v;
+    }
+    if ((i & 31) == 0) part[slot][i >> 5] = v;
+    sync();
+    between();
+    float s = 0.0f;
+    for (int w = 0; w < threads; w += 128) {
+      const float4 p = *reinterpret_cast<const float4*>(&part[slot][w / 32]);
+      s += (p.x + p.y) + (p.z + p.w);
+    }
+    return s;
+  }
+};
+
+// u <- norm(u) * w + b over a row. read_done() runs once every thread of the
+// row has all of its elements of u.
+template <int VEC, int CPT, int WD, class Vec, class Done>
+__device__ __forceinline__ void normalise(F2 (&u)[CPT][pairs(VEC)], const bool (&in)[CPT],
+                                          const Args& a, const Group& g, int slot, float inv_h,
+                                          const Vec& vec, int weight, int bias,
+                                          const Done& read_done) {
+  auto total = [](F2 x) {
+    float lo, hi;
+    f2_split(x, lo, hi);
+    return lo + hi;
+  };
+  if (a.layer) {
+    F2 s = f2(0.0f, 0.0f);
 #pragma unroll
     for (int c = 0; c < CPT; ++c)
       if (in[c]) {
 #pragma unroll
-        for (int q = 0; q < VEC; ++q) {
-          const float d = u[c][q] - mean;
-          s2 = fmaf(d, d, s2);
-        }
+        for (int q = 0; q < pairs(VEC); ++q) s = f2_add(s, u[c][q]);
       }
-    rstd = rsqrtf(row_sum(s2, warps, p1) * inv_h + a.eps);
-  };
-
-  if (a.y) {
-    float mean = 0.0f, rstd = 1.0f;
-    if (a.inner) stats(v, part[0], part[1], mean, rstd);
-    const float tok = a.gate_mode == DWM_GATE_TOKEN ? ld1(a.gate, row * a.ldg, a.gate_f32) : 1.0f;
+    const float mean = g.sum(total(s), slot, [] {}) * inv_h;
+    // The second half of a VEC = 1 pair stays 0.
+    const F2 minus = f2(-mean, VEC == 1 ? 0.0f : -mean);
 #pragma unroll
-    for (int c = 0; c < CPT; ++c) {
-      if (!in[c]) continue;
-      if (a.inner) {
-        float w[VEC];
-        ld<VEC>(a.w2, col[c], a.w_f32, w);
+    for (int c = 0; c < CPT; ++c)
 #pragma unroll
-        for (int q = 0; q < VEC; ++q) v[c][q] = (v[c][q] - mean) * rstd * w[q];
-        if (a.b2) {
-          ld<VEC>(a.b2, col[c], a.w_f32, w);
+      for (int q = 0; q < pairs(VEC); ++q) u[c][q] = f2_add(u[c][q], minus);
+  }
+  F2 s2 = f2(0.0f, 0.0f);
 #pragma unroll
-          for (int q = 0; q < VEC; ++q) v[c][q] += w[q];
-        }
-      }
-      if (a.gate_mode == DWM_GATE_TOKEN) {
+  for (int c = 0; c < CPT; ++c)
+    if (in[c]) {
 #pragma unroll
-        for (int q = 0; q < VEC; ++q) v[c][q] *= tok;
-      } else if (a.gate_mode != DWM_GATE_NONE) {
-        float g[VEC];
-        ld<VEC>(a.gate, (a.gate_mode == DWM_GATE_FULL ? row * a.ldg : 0) + col[c], a.gate_f32, g);
-#pragma unroll
-        for (int q = 0; q < VEC; ++q) v[c][q] *= g[q];
-      }
-#pragma unroll
-      for (int q = 0; q < VEC; ++q) res[c][q] = fmaf(a.scale, v[c][q], a.res_scale * res[c][q]);
-      st<VEC>(a.r_out, row * a.ldr + col[c], RF, res[c]);
+      for (int q = 0; q < pairs(VEC); ++q) s2 = f2_fma(u[c][q], u[c][q], s2);
     }
+  const float rstd = rsqrtf(g.sum(total(s2), slot + 1, read_done) * inv_h + a.eps);
+  const F2 rstd2 = f2(rstd, rstd);
+  vec(weight, [&](const Raw<VEC, CPT, WD>& w) {
+    w.into(u, a.w_f32, [&](F2 v, F2 x) { return f2_mul(f2_mul(v, rstd2), x); });
+  });
+  if (a.vec[bias])
+    vec(bias, [&](const Raw<VEC, CPT, WD>& b) {
+      b.into(u, a.w_f32, [](F2 v, F2 x) { return f2_add(v, x); });
+    });
+}
+
+// One row: both norms, gate, residual, stores. y, res, gate and vec (a weight
+// or bias) are functions that hand their loaded elements on: from registers
+// where the caller has loaded them ahead, or from where they lie. r_out and
+// h_out point to the row. read_done() runs once every thread has the row's
+// elements.
+template <int VEC, int CPT, int YD, int RD, int WD, class Y, class Res, class Gate, class Vec,
+          class Done>
+__device__ __forceinline__ void do_row(const Args& a, const Group& g, uint8_t* r_out,
+                                       uint8_t* h_out, float inv_h, const int (&col)[CPT],
+                                       const bool (&in)[CPT], float gate_tok, const Y& y,
+                                       const Res& res, const Gate& gate, const Vec& vec,
+                                       const Done& read_done) {
+  F2 v[CPT][pairs(VEC)];
+  if (a.y) {
+    y([&](const Raw<VEC, CPT, YD>& x) {
+      x.into(v, a.y_f32, [](F2, F2 e) { return e; });
+    });
+    if (a.inner) normalise<VEC, CPT, WD>(v, in, a, g, 0, inv_h, vec, W2, B2, [] {});
+    if (a.gate_mode >= DWM_GATE_CHANNEL)
+      gate([&](const Raw<VEC, CPT, YD>& x) {
+        x.into(v, a.y_f32, [](F2 u, F2 e) { return f2_mul(u, e); });
+      });
+    const F2 scale = f2(a.scale * gate_tok, a.scale * gate_tok);
+    const F2 res_scale = f2(a.res_scale, a.res_scale);
+    res([&](const Raw<VEC, CPT, RD>& x) {
+      x.into(v, a.res_f32, [&](F2 u, F2 e) { return f2_fma(scale, u, f2_mul(res_scale, e)); });
+    });
+    const int es = bytes_of<RD>(a.res_f32);
+#pragma unroll
+    for (int c = 0; c < CPT; ++c)
+      if (in[c]) st<VEC>(r_out + col[c] * es, es == 4, v[c]);
+  } else {
+    res([&](const Raw<VEC, CPT, RD>& x) {
+      x.into(v, a.res_f32, [](F2, F2 e) { return e; });
+    });
   }
   if (a.h_out) {
-    float mean, rstd;
-    stats(res, part[2], part[3], mean, rstd);
+    normalise<VEC, CPT, WD>(v, in, a, g, 2, inv_h, vec, W1, B1, read_done);
+    if (a.h_f32) {
 #pragma unroll
-    for (int c = 0; c < CPT; ++c) {
-      if (!in[c]) continue;
-      float w[VEC];
-      ld<VEC>(a.w1, col[c], a.w_f32, w);
+      for (int c = 0; c < CPT; ++c)
+        if (in[c]) st<VEC>(h_out + col[c] * 4, true, v[c]);
+    } else {
 #pragma unroll
-      for (int q = 0; q < VEC; ++q) res[c][q] = (res[c][q] - mean) * rstd * w[q];
-      if (a.b1) {
-        ld<VEC>(a.b1, col[c], a.w_f32, w);
-#pragma unroll
-        for (int q = 0; q < VEC; ++q) res[c][q] += w[q];
-      }
-      st<VEC>(a.h_out, row * a.ldh + col[c], a.h_f32, res[c]);
+      for (int c = 0; c < CPT; ++c)
+        if (in[c]) st<VEC>(h_out + col[c] * 2, false, v[c]);
     }
+  } else {
+    g.sync();
+    read_done();
   }
 }
 
+template <int YD>
+__device__ __forceinline__ float token_gate(const Args& a, int64_t row) {
+  if (a.gate_mode != DWM_GATE_TOKEN) return 1.0f;
+  return is_f32<YD>(a.y_f32)
+             ? static_cast<const float*>(a.gate)[row * a.ldg]
+             : bf16_bits_to_f32(static_cast<const uint16_t*>(a.gate)[row * a.ldg]);
+}
+
+// Loads past the row's end read its first elements, which nothing uses.
 template <int VEC, int CPT>
-int launch(const Args& a, bool yf, bool rf, int tpr, int rows, cudaStream_t s) {
-  const dim3 block((unsigned)tpr, (unsigned)rows);
-  const unsigned grid = (unsigned)((a.t + rows - 1) / rows);
-  if (yf)
-    rf ? block_norm_kernel<VEC, CPT, true, true><<<grid, block, 0, s>>>(a)
-       : block_norm_kernel<VEC, CPT, true, false><<<grid, block, 0, s>>>(a);
-  else
-    rf ? block_norm_kernel<VEC, CPT, false, true><<<grid, block, 0, s>>>(a)
-       : block_norm_kernel<VEC, CPT, false, false><<<grid, block, 0, s>>>(a);
+__device__ __forceinline__ void columns(const Args& a, const Group& g, int (&col)[CPT],
+                                        bool (&in)[CPT]) {
+#pragma unroll
+  for (int c = 0; c < CPT; ++c) {
+    col[c] = (g.i + c * g.threads) * VEC;
+    in[c] = col[c] < a.h;  // h is a multiple of VEC
+    if (!in[c]) col[c] = 0;
+  }
+}
+
+__device__ __forceinline__ const uint8_t* row_ptr(const void* p, int64_t row, int64_t ld, int es) {
+  return static_cast<const uint8_t*>(p) + row * ld * es;
+}
+__device__ __forceinline__ uint8_t* row_ptr(void* p, int64_t row, int64_t ld, int es) {
+  return static_cast<uint8_t*>(p) + row * ld * es;
+}
+
+// The most threads of a CTA: those that a row of MAX_H needs, and in the
+// streaming kernel 1024 (64 registers each) unless a thread has 32 elements.
+template <int VEC, int CPT>
+constexpr int max_threads(bool stream) {
+  return VEC * CPT > 16 || (VEC == 8 && !stream) ? 512 : 1024;
+}
+
+// A few rows: one group a row, every load of a row issued before its first
+// sum, so that a row costs one memory latency. threadIdx.y: the CTA's groups.
+template <int VEC, int CPT, int YD, int RD, int WD>
+__global__ void __launch_bounds__(max_threads<VEC, CPT>(false)) block_norm_kernel(const Args a) {
+  __shared__ __align__(16) float part[4][32];
+  const Group g{(int)threadIdx.x, (int)blockDim.x, 0, part};
+  const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+  if (row >= a.t) return;  // a whole warp of a CTA with a warp a row
+  int col[CPT];
+  bool in[CPT];
+  columns<VEC, CPT>(a, g, col, in);
+  const int ye = bytes_of<YD>(a.y_f32), re = bytes_of<RD>(a.res_f32);
+  const uint8_t* pg = row_ptr(a.gate, a.gate_mode == DWM_GATE_FULL ? row : 0, a.ldg, ye);
+  // Up to 16 elements a thread everything is loaded ahead; the gate and the
+  // weights of more would not fit the registers.
+  constexpr bool AHEAD = VEC == 8 && CPT <= 2;
+  Raw<VEC, CPT, YD> y, gate;
+  Raw<VEC, CPT, RD> res;
+  Raw<VEC, CPT, WD> w2, w1;
+  if (a.y) y.load(row_ptr(a.y, row, a.ldy, ye), col, a.y_f32);
+  res.load(row_ptr(a.res, row, a.ldres, re), col, a.res_f32);
+  if (AHEAD) {
+    if (a.inner) w2.load(a.vec[W2], col, a.w_f32);
+    if (a.gate_mode >= DWM_GATE_CHANNEL) gate.load(pg, col, a.y_f32);
+    if (a.h_out) w1.load(a.vec[W1], col, a.w_f32);
+  }
+  const float tok = token_gate<YD>(a, row);
+  if (g.threads > 32) {
+    g.clear_parts();
+    g.sync();
+  }
+  do_row<VEC, CPT, YD, RD, WD>(
+      a, g, row_ptr(a.r_out, row, a.ldr, re), row_ptr(a.h_out, row, a.ldh, a.h_f32 ? 4 : 2),
+      1.0f / (float)a.h, col, in, tok, [&](auto f) { f(y); }, [&](auto f) { f(res); },
+      [&](auto f) {
+        if (!AHEAD) gate.load(pg, col, a.y_f32);
+        f(gate);
+      },
+      [&](int which, auto f) {
+        if (AHEAD && which == W2) {
+          f(w2);
+        } else if (AHEAD && which == W1) {
+          f(w1);
+        } else {
+          Raw<VEC, CPT, WD> x;
+          x.load(a.vec[which], col, a.w_f32);
+          f(x);
+        }
+      },
+      [] {});
+}
+
+// Many rows: one CTA an SM, its groups taking rows in turn. A group's first
+// thread keeps a ring of bulk copies (cp.async.bulk) of its next rows of y,
+// residual and full gate in flight, so that the memory is busy while the group
+// sums and stores. The vectors that all rows share lie in shared memory (the
+// ring leaves the L1 cache too small for them). A row whose bytes do not start on 16 is copied from
+// the 16-byte granule it starts in to the one it ends in.
+__device__ __forceinline__ uint32_t bulk_bytes(const uint8_t* p, int bytes) {
+  const uint64_t at = reinterpret_cast<uint64_t>(p);
+  return (uint32_t)(((at + bytes + 15) & ~15ull) - (at & ~15ull));
+}
+__device__ __forceinline__ void bulk_row(uint32_t dst, const uint8_t* p, int bytes, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+          dst),
+      "l"(reinterpret_cast<uint64_t>(p) & ~15ull), "r"(bulk_bytes(p, bytes)), "r"(smem_u32(bar))
+      : "memory");
+}
+
+constexpr int MAX_STAGES = 8;
+constexpr int MAX_GROUPS = 16;
+
+template <int VEC, int CPT, int YD, int RD, int WD>
+__global__ void __launch_bounds__(max_threads<VEC, CPT>(true), 1)
+    block_norm_stream_kernel(const Args a) {
+  __shared__ __align__(16) float part[MAX_GROUPS][4][32];
+  __shared__ uint64_t full[MAX_GROUPS][MAX_STAGES];
+  __shared__ int abort_word;
+  extern __shared__ __align__(16) uint8_t ring[];
+  volatile int* abort_flag = &abort_word;
+  const int gi = threadIdx.y, groups = blockDim.y;
+  const Group g{(int)threadIdx.x, (int)blockDim.x, gi, part[gi]};
+  const uint32_t vectors = smem_u32(ring);
+  const uint32_t stages =
+      vectors + (uint32_t)(5 * a.vec_bytes + gi * a.stages * a.stage_bytes);
+  if (g.i == 0) {
+    for (int s = 0; s < a.stages; ++s) mbar_init(&full[gi][s], 1);
+    fence_mbar_init();
+    *abort_flag = 0;
+  }
+  g.clear_parts();
+  __syncthreads();
+  int col[CPT];
+  bool in[CPT];
+  columns<VEC, CPT>(a, g, col, in);
+  const float inv_h = 1.0f / (float)a.h;
+  const int64_t first = (int64_t)blockIdx.x * groups + gi, step = (int64_t)gridDim.x * groups;
+  const bool full_gate = a.gate_mode == DWM_GATE_FULL;
+  const int ye = bytes_of<YD>(a.y_f32), re = bytes_of<RD>(a.res_f32), he = a.h_f32 ? 4 : 2;
+  auto fetch = [&](int64_t row, int s) {
+    const uint8_t* py = row_ptr(a.y, row, a.ldy, ye);
+    const uint8_t* pr = row_ptr(a.res, row, a.ldres, re);
+    const uint8_t* pg = row_ptr(a.gate, row, a.ldg, ye);
+    uint32_t bytes = bulk_bytes(pr, a.h * re);
+    if (a.y) bytes += bulk_bytes(py, a.h * ye);
+    if (full_gate) bytes += bulk_bytes(pg, a.h * ye);
+    uint64_t* bar = &full[gi][s];
+    const uint32_t dst = stages + (uint32_t)(s * a.stage_bytes);
+    mbar_arrive_expect_tx(bar, bytes);
+    if (a.y) bulk_row(dst, py, a.h * ye, bar);
+    bulk_row(dst + a.off_res, pr, a.h * re, bar);
+    if (full_gate) bulk_row(dst + a.off_gate, pg, a.h * ye, bar);
+  };
+  if (g.i == 0)
+    for (int s = 0; s < a.stages; ++s)
+      if (first + s * step < a.t) fetch(first + s * step, s);
+  if (a.vec_bytes) {
+    // 16 bytes a load, or an element a load where they are not aligned.
+#pragma unroll
+    for (int j = 0; j < 5; ++j) {
+      const void* p = j < 4 ? a.vec[j] : a.gate_mode == DWM_GATE_CHANNEL ? a.gate : nullptr;
+      const int es = j < 4 ? bytes_of<WD>(a.w_f32) : ye;
+      if (!p) continue;
+      uint8_t* dst = ring + j * a.vec_bytes;
+      const int tid = gi * g.threads + g.i, threads = groups * g.threads;
+      if (VEC == 8) {
+        for (int i = tid; i < a.h * es / 16; i += threads)
+          reinterpret_cast<uint4*>(dst)[i] = static_cast<const uint4*>(p)[i];
+      } else if (es == 4) {
+        for (int i = tid; i < a.h; i += threads)
+          reinterpret_cast<uint32_t*>(dst)[i] = static_cast<const uint32_t*>(p)[i];
+      } else {
+        for (int i = tid; i < a.h; i += threads)
+          reinterpret_cast<uint16_t*>(dst)[i] = static_cast<const uint16_t*>(p)[i];
+      }
+    }
+    __syncthreads();
+  }
+  int s = 0;
+  uint32_t ph = 0;
+  uint8_t* r_out = row_ptr(a.r_out, first, a.ldr, re);
+  uint8_t* h_out = row_ptr(a.h_out, first, a.ldh, he);
+  for (int64_t row = first; row < a.t; row += step) {
+    const float tok = token_gate<YD>(a, row);
+    // After a wait that ran out (reported in the status word) the rows are not
+    // what they should be, but the group stays together.
+    mbar_wait(&full[gi][s], ph, abort_flag, a.status);
+    const uint32_t at = stages + (uint32_t)(s * a.stage_bytes);
+    // Where the row's first byte sits in its first granule.
+    auto lead = [&](const void* p, int64_t ld, int es) {
+      return VEC == 8 ? 0u : (uint32_t)reinterpret_cast<uint64_t>(row_ptr(p, row, ld, es)) & 15u;
+    };
+    do_row<VEC, CPT, YD, RD, WD>(
+        a, g, r_out, h_out, inv_h, col, in, tok,
+        [&](auto f) {
+          Raw<VEC, CPT, YD> x;
+          x.load_s(at + lead(a.y, a.ldy, ye), col, a.y_f32);
+          f(x);
+        },
+        [&](auto f) {
+          Raw<VEC, CPT, RD> x;
+          x.load_s(at + a.off_res + lead(a.res, a.ldres, re), col, a.res_f32);
+          f(x);
+        },
+        [&](auto f) {
+          if (full_gate) {
+            Raw<VEC, CPT, YD> x;
+            x.load_s(at + a.off_gate + lead(a.gate, a.ldg, ye), col, a.y_f32);
+            f(x);
+          } else {
+            Raw<VEC, CPT, YD> x;
+            if (a.vec_bytes)
+              x.load_s(vectors + CHANNEL_GATE * a.vec_bytes, col, a.y_f32);
+            else
+              x.load(a.gate, col, a.y_f32);
+            f(x);
+          }
+        },
+        [&](int which, auto f) {
+          Raw<VEC, CPT, WD> x;
+          if (a.vec_bytes)
+            x.load_s(vectors + which * a.vec_bytes, col, a.w_f32);
+          else
+            x.load(a.vec[which], col, a.w_f32);
+          f(x);
+        },
+        [&] {
+          if (g.i == 0 && row + a.stages * step < a.t) fetch(row + a.stages * step, s);
+        });
+    r_out += step * a.ldr * re;
+    h_out += step * a.ldh * he;
+    if (++s == a.stages) { s = 0; ph ^= 1; }
+  }
+  // A copy that a wait gave up on lands before the exit.
+  if (g.i == 0 && *abort_flag)
+    for (int i = 0; i < a.stages; ++i) mbar_wait(&full[gi][i], ph ^ (i >= s), nullptr, a.status);
+}
+
+template <int VEC, int CPT, int YD, int RD, int WD>
+int launch(Args a, cudaStream_t s) {
+  const int n = (a.h + VEC - 1) / VEC;  // loads a row
+  // A group: as many warps as the row takes with CPT loads a thread.
+  const int threads = ((n + CPT - 1) / CPT + 31) / 32 * 32;
+  const int groups = std::min(MAX_GROUPS, max_threads<VEC, CPT>(true) / threads);
+  if ((int64_t)a.t > 2 * (int64_t)num_sms() * groups) {
+    auto room = [&](int f32) { return (a.h * (f32 ? 4 : 2) + 15) / 16 * 16 + (VEC == 1 ? 16 : 0); };
+    a.off_res = a.y ? room(a.y_f32) : 0;
+    a.off_gate = a.off_res + room(a.res_f32);
+    a.stage_bytes = a.off_gate + (a.gate_mode == DWM_GATE_FULL ? room(a.y_f32) : 0);
+    const int budget = 208 * 1024;
+    a.vec_bytes = (a.h * std::max(a.w_f32 ? 4 : 2, a.y_f32 ? 4 : 2) + 15) / 16 * 16;
+    if (5 * a.vec_bytes + 2 * groups * a.stage_bytes > budget) a.vec_bytes = 0;
+    const int left = budget - 5 * a.vec_bytes;
+    a.stages = std::min(MAX_STAGES, left / (groups * a.stage_bytes));
+    if (a.stages >= 2) {
+      auto fn = block_norm_stream_kernel<VEC, CPT, YD, RD, WD>;
+      const int rc = set_smem_limit(reinterpret_cast<const void*>(fn), budget, "norm smem attribute");
+      if (rc) return rc;
+      a.status = status_ptr();
+      fn<<<(unsigned)num_sms(), dim3((unsigned)threads, (unsigned)groups),
+           (size_t)5 * a.vec_bytes + (size_t)groups * a.stages * a.stage_bytes, s>>>(a);
+      return check_cuda(cudaGetLastError(), "block_norm launch");
+    }
+  }
+  // A warp a row, four a CTA, or a CTA a row.
+  const int rows = threads == 32 ? 4 : 1;
+  block_norm_kernel<VEC, CPT, YD, RD, WD>
+      <<<(unsigned)((a.t + rows - 1) / rows), dim3((unsigned)threads, (unsigned)rows), 0, s>>>(a);
   return check_cuda(cudaGetLastError(), "block_norm launch");
 }
 
-// Rows of at most 32 elements a thread and 512 threads (a thread's two rows
-// of f32 are 64 registers, which 1024 threads would not have).
+template <int VEC, int YD, int RD, int WD>
+int by_width(const Args& a, cudaStream_t s) {
+  const int n = (a.h + VEC - 1) / VEC;
+  const bool many = a.t > 2 * num_sms();
+  if constexpr (VEC == 8) {
+    // Few rows: a load a thread.
+    if (n <= 32 || (!many && n <= 512)) return launch<8, 1, YD, RD, WD>(a, s);
+    if (n <= 1024) return launch<8, 2, YD, RD, WD>(a, s);
+    return launch<8, 4, YD, RD, WD>(a, s);
+  } else {
+    if (n <= 8192) return launch<1, 8, YD, RD, WD>(a, s);
+    return launch<1, 16, YD, RD, WD>(a, s);
+  }
+}
+
+// Rows of at most 32 elements a thread of 512 (VEC = 1: 16 a thread of 1024).
 constexpr int MAX_H = 16384;
 
-int run(const Args& a, bool yf, bool rf, bool vec, cudaStream_t s) {
-  const int n = vec ? a.h / 8 : a.h;  // loads a row
-  const int max_cpt = vec ? 4 : 32;
-  int tpr = 32;
-  while (tpr < 512 && tpr * max_cpt < n) tpr *= 2;
-  if (tpr > 32 || n > 128) {
-    // A CTA a row: more threads with fewer loads each, down to two.
-    while (tpr < 512 && (n + tpr - 1) / tpr > (vec ? 2 : 8)) tpr *= 2;
-  }
-  const int rows = tpr == 32 ? 4 : 1;
-  const int cpt = (n + tpr - 1) / tpr;
-  if (vec) {
-    if (cpt <= 1) return launch<8, 1>(a, yf, rf, tpr, rows, s);
-    if (cpt <= 2) return launch<8, 2>(a, yf, rf, tpr, rows, s);
-    return launch<8, 4>(a, yf, rf, tpr, rows, s);
-  }
-  if (cpt <= 4) return launch<1, 4>(a, yf, rf, tpr, rows, s);
-  if (cpt <= 8) return launch<1, 8>(a, yf, rf, tpr, rows, s);
-  if (cpt <= 16) return launch<1, 16>(a, yf, rf, tpr, rows, s);
-  return launch<1, 32>(a, yf, rf, tpr, rows, s);
+int run(const Args& a, bool vec, cudaStream_t s) {
+  if (!vec) return by_width<1, ANY, ANY, ANY>(a, s);
+#define DWM_NORM(YD, RD, WD)                                                               \
+  if ((a.y_f32 != 0) == (YD == FP) && (a.res_f32 != 0) == (RD == FP) &&                    \
+      (a.w_f32 != 0) == (WD == FP))                                                        \
+    return by_width<8, YD, RD, WD>(a, s);
+  DWM_NORM(BF, BF, BF)
+  DWM_NORM(BF, BF, FP)
+  DWM_NORM(BF, FP, BF)
+  DWM_NORM(BF, FP, FP)
+  DWM_NORM(FP, BF, BF)
+  DWM_NORM(FP, BF, FP)
+  DWM_NORM(FP, FP, BF)
+  DWM_NORM(FP, FP, FP)
+#undef DWM_NORM
+  return set_error(DWM_ERR_UNSUPPORTED, "norm dtype combination");
 }
 
 }  // namespace norm
@@ -253,7 +616,7 @@ using namespace dwm;
 extern "C" int dwm_block_norm(const void* y, int y_dtype, int64_t ldy, const void* residual,
                               int residual_dtype, int64_t ldres, int t, int h, int kind,
                               float eps, int inner, const void* w2, const void* b2,
-                              const void* gate, int gate_dtype, int gate_mode, int64_t ldg,
+                              const void* gate, int gate_mode, int64_t ldg,
                               float scale, float residual_scale, const void* w1, const void* b1,
                               int w_dtype, void* r_out, int64_t ldr, void* h_out, int h_dtype,
                               int64_t ldh, void* stream) {
@@ -264,7 +627,7 @@ extern "C" int dwm_block_norm(const void* y, int y_dtype, int64_t ldy, const voi
   DWM_CHECK_ARG(kind == DWM_NORM_RMS || kind == DWM_NORM_LAYER, "unknown norm kind %d", kind);
   DWM_CHECK_ARG(eps > 0.0f, "eps must be positive");
   DWM_CHECK_ARG(is_float(residual_dtype) && is_float(w_dtype) && is_float(h_dtype) &&
-                    (!y || is_float(y_dtype)) && (!gate || is_float(gate_dtype)),
+                    (!y || is_float(y_dtype)),
                 "dtypes must be bf16 or f32");
   DWM_CHECK_ARG(gate_mode >= DWM_GATE_NONE && gate_mode <= DWM_GATE_FULL &&
                     (gate_mode == DWM_GATE_NONE) == (gate == nullptr),
@@ -297,7 +660,7 @@ extern "C" int dwm_block_norm(const void* y, int y_dtype, int64_t ldy, const voi
     };
     const In ins[3] = {{y, ldy, es(y_dtype)},
                        {residual, ldres, es(residual_dtype)},
-                       {gate_mode == DWM_GATE_FULL ? gate : nullptr, ldg, es(gate_dtype)}};
+                       {gate_mode == DWM_GATE_FULL ? gate : nullptr, ldg, es(y_dtype)}};
     DWM_CHECK_ARG(!rows_overlap(r, ho), "the two outputs overlap");
     for (const In& i : ins) {
       const RowSpan in = row_span(i.p, t, h, i.ld, i.es);
@@ -311,9 +674,9 @@ extern "C" int dwm_block_norm(const void* y, int y_dtype, int64_t ldy, const voi
     const RowSpan vecs[5] = {
         row_span(w2, 1, h, h, es(w_dtype)), row_span(b2, 1, h, h, es(w_dtype)),
         row_span(w1, 1, h, h, es(w_dtype)), row_span(b1, 1, h, h, es(w_dtype)),
-        gate_mode == DWM_GATE_CHANNEL ? row_span(gate, 1, h, h, es(gate_dtype))
+        gate_mode == DWM_GATE_CHANNEL ? row_span(gate, 1, h, h, es(y_dtype))
                                       : row_span(gate_mode == DWM_GATE_TOKEN ? gate : nullptr, t,
-                                                 1, ldg, es(gate_dtype))};
+                                                 1, ldg, es(y_dtype))};
     for (const RowSpan& v : vecs)
       DWM_CHECK_ARG(!rows_overlap(v, r) && !rows_overlap(v, ho),
                     "an output overlaps a weight or the gate");
@@ -327,14 +690,14 @@ extern "C" int dwm_block_norm(const void* y, int y_dtype, int64_t ldy, const voi
                    rows16(w1, 0, w_dtype) && rows16(b1, 0, w_dtype) && rows16(w2, 0, w_dtype) &&
                    rows16(b2, 0, w_dtype) &&
                    (gate_mode < DWM_GATE_CHANNEL ||
-                    rows16(gate, gate_mode == DWM_GATE_FULL ? ldg : 0, gate_dtype));
+                    rows16(gate, gate_mode == DWM_GATE_FULL ? ldg : 0, y_dtype));
   norm::Args a;
   a.y = y;
   a.res = residual;
-  a.w2 = w2;
-  a.b2 = b2;
-  a.w1 = w1;
-  a.b1 = b1;
+  a.vec[norm::W2] = w2;
+  a.vec[norm::B2] = b2;
+  a.vec[norm::W1] = w1;
+  a.vec[norm::B1] = b1;
   a.gate = gate;
   a.r_out = r_out;
   a.h_out = h_out;
@@ -348,12 +711,14 @@ extern "C" int dwm_block_norm(const void* y, int y_dtype, int64_t ldy, const voi
   a.inner = inner != 0;
   a.layer = kind == DWM_NORM_LAYER;
   a.gate_mode = gate_mode;
+  a.y_f32 = y && y_dtype == DWM_F32;
+  a.res_f32 = residual_dtype == DWM_F32;
   a.w_f32 = w_dtype == DWM_F32;
-  a.gate_f32 = gate_dtype == DWM_F32;
   a.h_f32 = h_dtype == DWM_F32;
   a.eps = eps;
   a.scale = scale;
   a.res_scale = residual_scale;
-  return norm::run(a, y && y_dtype == DWM_F32, residual_dtype == DWM_F32, vec,
-                   static_cast<cudaStream_t>(stream));
+  a.stages = a.stage_bytes = a.off_res = a.off_gate = a.vec_bytes = 0;
+  a.status = nullptr;
+  return norm::run(a, vec, static_cast<cudaStream_t>(stream));
 }

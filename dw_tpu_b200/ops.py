@@ -532,8 +532,8 @@ def block_norm_out(residual, h_out=None, *, weight=None, bias=None, y=None, r_ou
     """r_out <- residual_scale * residual + scale * gate * n2(y) and
     h_out <- n1(r) (dwm_block_norm); without ``y`` only h_out <- n1(residual).
     n1 has ``weight`` / ``bias``, n2 ``norm_weight`` / ``norm_bias`` (without a
-    weight it is the identity). gate [t, 1], [h] or [t, h]; r_out has
-    residual's dtype. Rows may be strided; an output may be one of the row
+    weight it is the identity). gate [t, 1], [h] or [t, h] in y's dtype; r_out
+    has residual's dtype. Rows may be strided; an output may be one of the row
     inputs in place."""
     dev = _same_device(residual, h_out, weight, bias, y, r_out, norm_weight, norm_bias, gate)
     if dev != torch.cuda.current_device():
@@ -569,6 +569,8 @@ def block_norm_out(residual, h_out=None, *, weight=None, bias=None, y=None, r_ou
         raise ValueError("h_out, weight and bias belong together: h_out = norm(r) * weight + bias")
     mode = L.GATE_NONE
     if gate is not None:
+        if y is None or gate.dtype != y.dtype:
+            raise ValueError("gate goes with y and has its dtype")
         if gate.dim() == 1:
             _vector(gate, "gate", h)
             mode = L.GATE_CHANNEL
@@ -578,9 +580,8 @@ def block_norm_out(residual, h_out=None, *, weight=None, bias=None, y=None, r_ou
     rc = L.lib().dwm_block_norm(
         L.ptr(y), L.BF16 if y is None else L.dtype_code(y.dtype), ldy, residual.data_ptr(),
         L.dtype_code(residual.dtype), ldres, t, h, _NORMS[kind], float(eps),
-        int(norm_weight is not None), L.ptr(norm_weight), L.ptr(norm_bias), L.ptr(gate),
-        L.BF16 if gate is None else L.dtype_code(gate.dtype), mode, ldg, float(scale),
-        float(residual_scale), L.ptr(weight), L.ptr(bias),
+        int(norm_weight is not None), L.ptr(norm_weight), L.ptr(norm_bias), L.ptr(gate), mode, ldg,
+        float(scale), float(residual_scale), L.ptr(weight), L.ptr(bias),
         L.BF16 if wdt is None else L.dtype_code(wdt), L.ptr(r_out), ldr, L.ptr(h_out),
         L.BF16 if h_out is None else L.dtype_code(h_out.dtype), ldh,
         L.stream_ptr() if stream is None else stream)

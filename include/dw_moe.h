@@ -297,8 +297,8 @@ int dwm_dense_matmul(const void* x, int64_t ldx, const void* w, int64_t ldw, int
  * n(v) = (v - m) / sqrt(mean((v - m)^2) + eps) * w + b with m = 0
  * (DWM_NORM_RMS) or m = mean(v) (DWM_NORM_LAYER); statistics, products and
  * sums in f32, h from the f32 r, each output rounded once. y [t, h] (bf16 or
- * f32) is the block's output, residual [t, h] and r_out share one dtype, h_out
- * is bf16 or f32, w1 / b1 / w2 / b2 [h] share one; b1 and b2 may be NULL.
+ * f32) is the block's output, gate (DWM_GATE_*) has its dtype, residual [t, h]
+ * and r_out share one dtype, h_out is bf16 or f32, w1 / b1 / w2 / b2 [h] share one; b1 and b2 may be NULL.
  * inner = 0: n2 is the identity. h_out = NULL: no n1 (w1 unused). y = NULL:
  * only h = n1(residual) (r_out NULL, no gate, inner = 0). ld*: row strides in
  * elements, any; 16-byte loads are used where every row of every tensor starts
@@ -307,8 +307,8 @@ int dwm_dense_matmul(const void* x, int64_t ldx, const void* w, int64_t ldw, int
  * 1 <= h <= 16384, eps > 0. No counterpart in the reference. */
 int dwm_block_norm(const void* y, int y_dtype, int64_t ldy, const void* residual,
                    int residual_dtype, int64_t ldres, int t, int h, int kind, float eps,
-                   int inner, const void* w2, const void* b2, const void* gate, int gate_dtype,
-                   int gate_mode, int64_t ldg, float scale, float residual_scale,
+                   int inner, const void* w2, const void* b2, const void* gate, int gate_mode,
+                   int64_t ldg, float scale, float residual_scale,
                    const void* w1, const void* b1, int w_dtype, void* r_out, int64_t ldr,
                    void* h_out, int h_dtype, int64_t ldh, void* stream);
 

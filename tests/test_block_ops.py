@@ -92,7 +92,7 @@ def test_route_refusals(lib, kw, message):
 
 def _norm(lib, **kw):
     a = dict(y=MB, ydt=0, ldy=64, res=2 * MB, rdt=0, ldres=64, t=4, h=64, kind=0, eps=1e-6,
-             inner=1, w2=3 * MB, b2=None, gate=None, gdt=0, gmode=0, ldg=0, scale=1.0, rs=1.0,
+             inner=1, w2=3 * MB, b2=None, gate=None, gmode=0, ldg=0, scale=1.0, rs=1.0,
              w1=4 * MB, b1=None, wdt=0, r=5 * MB, ldr=64, ho=6 * MB, hdt=0, ldh=64, stream=None)
     assert set(kw) <= set(a)
     a.update(kw)
