@@ -7,10 +7,9 @@
 // operand A, up to 128 rows of x are operand B, so a decode batch pays for its
 // own tokens (N = 16 and up) and not for 128. The k axis is split over a
 // cluster of 1, 2, 4 or 8 CTAs, which fills the GPU when w has few rows. Each
-// CTA puts its f32 partial tile in its shared memory; the cluster's CTAs then
-// share the tile's outputs out among them, and each adds the partials of its
-// share in CTA order (over distributed shared memory), so the result depends
-// on the shapes alone: no atomics, no workspace.
+// CTA owns some of the tile's rows of x; all send it their f32 partials of those
+// rows (bulk copies between the CTAs' shared memories), and it adds them in CTA
+// order, so the result depends on the shapes alone: no atomics, no workspace.
 //
 // With SwiGLU a tile is 64 gate rows and the 64 up rows of the same features,
 // which meet in the partial tile.
@@ -19,6 +18,7 @@
 // flight), for small shapes the launch and one memory latency, from ~100 rows
 // of x the tensor cores.
 #include <algorithm>
+#include <atomic>
 
 #include "common.cuh"
 
@@ -39,7 +39,9 @@ struct Args {
   int m, n_out, k;
   int act;
   int bias_f32, res_f32, out_f32;
-  int res_vec, out_vec;  // 8 elements at a column that is a multiple of 8 are 16-byte aligned
+  // 8 elements at a column that is a multiple of 8 are 16-byte aligned
+  int bias_vec, res_vec, out_vec;
+  int out_wide;  // 32 bytes of a row are 32-byte aligned
   float limit, res_scale;
   int* status;
 };
@@ -48,14 +50,15 @@ template <int BT>
 struct Layout {
   static constexpr int B_STAGE = BT * BK * 2;
   static constexpr int STG = A_STAGE + B_STAGE;
-  static constexpr int S = 98304 / STG;  // two CTAs per SM
-  static constexpr int PARTIAL = BT * TILE_W * 4;  // f32 [BT][TILE_W] over the stages
-  static constexpr int OFF_BAR = S * STG > PARTIAL ? S * STG : PARTIAL;
-  static constexpr int OFF_MISC = OFF_BAR + (2 * S + 1) * 8;
+  static constexpr int S = 204800 / STG;  // 6 (BT = 128) to 11 stages
+  static constexpr int PARTIAL = BT * TILE_W * 4;  // f32 [BT][TILE_W], over the stages
+  static constexpr int OFF_RECV = PARTIAL;         // the other CTAs' partials of the own rows
+  static constexpr int OFF_BAR = S * STG;
+  static constexpr int OFF_MISC = OFF_BAR + (2 * S + 2) * 8;
   static constexpr int ALLOC = OFF_MISC + 16 + 1024;  // slack for 1 KiB alignment
   static constexpr int TMEM_COLS = BT < 32 ? 32 : BT;
   static_assert(STG % 1024 == 0, "swizzled tiles need 1 KiB alignment");
-  static_assert(S >= 2 && 2 * (ALLOC + 1024) <= 233472, "two CTAs per SM");
+  static_assert(2 * PARTIAL <= S * STG && ALLOC <= 232448, "shared memory");
 };
 
 __device__ __forceinline__ float ld1(const void* p, int64_t i, int f32) {
@@ -63,89 +66,171 @@ __device__ __forceinline__ float ld1(const void* p, int64_t i, int f32) {
              : bf16_bits_to_f32(static_cast<const uint16_t*>(p)[i]);
 }
 
-__device__ __forceinline__ float sigmoid_full(float v) { return 1.0f / (1.0f + expf(-v)); }
-
-// The activation of one value. An f32 output takes full-precision functions,
-// a bf16 one (half a step: 2^-9 of the value) the MUFU forms (~1e-6).
-__device__ __forceinline__ float act1(float v, int act, int f32) {
-  if (act == DWM_ACT_SILU) return v * (f32 ? sigmoid_full(v) : sigmoid_fast(v));
-  if (act == DWM_ACT_GELU) return 0.5f * v * (1.0f + erff(v * 0.70710678118654752f));
-  if (act == DWM_ACT_GELU_TANH) {
-    // 0.5 (1 + tanh(u)) = sigmoid(2 u)
-    const float u = 1.5957691216057308f * fmaf(0.044715f * v * v, v, v);
-    return v * (f32 ? sigmoid_full(u) : sigmoid_fast(u));
+// N (8 or 16) neighbouring elements, 16-byte aligned.
+template <int N>
+__device__ __forceinline__ void load_n(const void* p, int64_t i, int f32, float (&v)[N]) {
+  if (f32) {
+    const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
+#pragma unroll
+    for (int j = 0; j < N / 4; ++j) {
+      const float4 x = q[j];
+      v[4 * j] = x.x; v[4 * j + 1] = x.y; v[4 * j + 2] = x.z; v[4 * j + 3] = x.w;
+    }
+  } else {
+    const uint4* q = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + i);
+#pragma unroll
+    for (int j = 0; j < N / 8; ++j) {
+      const uint4 x = q[j];
+      const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        v[8 * j + 2 * e] = __uint_as_float(w[e] << 16);
+        v[8 * j + 2 * e + 1] = __uint_as_float(w[e] & 0xFFFF0000u);
+      }
+    }
   }
-  return v;
 }
 
-// Outputs [col, col + 8) of row `row` from the products z (and, with SwiGLU,
-// the up products u): bias, activation, residual, one rounding.
-__device__ __forceinline__ void epilogue8(const Args& a, int64_t row, int col, float (&z)[8],
-                                          const float (&u)[8]) {
-  const bool glu = a.act == DWM_ACT_SWIGLU || a.act == DWM_ACT_SWIGLU_CLAMP;
-  const bool whole = col + 8 <= a.n_out;
+// 32 bytes, 32-byte aligned: one whole sector.
+__device__ __forceinline__ void stg_256(void* p, const uint32_t (&w)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]),
+               "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
+}
+
+// N values to `p` (bf16 or f32), 16-byte aligned; wide: 32-byte aligned.
+template <int N>
+__device__ __forceinline__ void store_n(void* p, int64_t i, int f32, bool wide,
+                                        const float (&v)[N]) {
+  uint32_t w[N];
+  int words;
+  uint8_t* at;
+  if (f32) {
 #pragma unroll
-  for (int q = 0; q < 8; ++q) {
-    float v = z[q], up = u[q];
-    if (a.bias && (whole || col + q < a.n_out)) {
-      v += ld1(a.bias, col + q, a.bias_f32);
-      if (glu) up += ld1(a.bias, a.n_out + col + q, a.bias_f32);
-    }
-    if (glu) {
-      if (a.act == DWM_ACT_SWIGLU_CLAMP) {
-        v = fminf(v, a.limit);
-        up = fminf(fmaxf(up, -a.limit), a.limit);
-      }
-      v = v * (a.out_f32 ? sigmoid_full(v) : sigmoid_fast(v)) * up;
-    } else {
-      v = act1(v, a.act, a.out_f32);
-    }
-    z[q] = v;
+    for (int q = 0; q < N; ++q) w[q] = __float_as_uint(v[q]);
+    words = N;
+    at = static_cast<uint8_t*>(p) + i * 4;
+  } else {
+#pragma unroll
+    for (int q = 0; q < N / 2; ++q) w[q] = f32x2_to_bf16x2(v[2 * q], v[2 * q + 1]);
+    words = N / 2;
+    at = static_cast<uint8_t*>(p) + i * 2;
   }
+#pragma unroll
+  for (int j = 0; j < N; j += 8) {
+    if (j >= words) break;
+    if (wide && j + 8 <= words) {
+      const uint32_t x[8] = {w[j], w[(j + 1) % N], w[(j + 2) % N], w[(j + 3) % N],
+                             w[(j + 4) % N], w[(j + 5) % N], w[(j + 6) % N], w[(j + 7) % N]};
+      stg_256(at + j * 4, x);
+    } else {
+      *reinterpret_cast<uint4*>(at + j * 4) = make_uint4(w[j], w[j + 1], w[j + 2], w[j + 3]);
+      if (j + 8 <= words)
+        *reinterpret_cast<uint4*>(at + j * 4 + 16) =
+            make_uint4(w[(j + 4) % N], w[(j + 5) % N], w[(j + 6) % N], w[(j + 7) % N]);
+    }
+  }
+}
+
+__device__ __forceinline__ float sigmoid_full(float v) { return 1.0f / (1.0f + expf(-v)); }
+
+// What a kernel's epilogue applies: nothing, a function of each element, or
+// SwiGLU of two (kernels of their own: the branches of the others would cost
+// the plain product its instruction cache).
+constexpr int PLAIN = 0, POINT = 1, GLU = 2;
+
+// The functions of one element. An f32 output takes full-precision functions,
+// a bf16 one (half a step: 2^-8 of the value) the MUFU forms (~1e-6).
+template <int ACT>
+__device__ __forceinline__ float act_of(float z, int f32) {
+  if (ACT == DWM_ACT_SILU) return z * (f32 ? sigmoid_full(z) : sigmoid_fast(z));
+  if (ACT == DWM_ACT_GELU) return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
+  // 0.5 (1 + tanh(u)) = sigmoid(2 u)
+  const float u = 1.5957691216057308f * fmaf(0.044715f * z * z, z, z);
+  return z * (f32 ? sigmoid_full(u) : sigmoid_fast(u));
+}
+template <int ACT, int N>
+__device__ __forceinline__ void act_of_n(float (&z)[N], int f32) {
+#pragma unroll
+  for (int q = 0; q < N; ++q) z[q] = act_of<ACT>(z[q], f32);
+}
+template <int N>
+__device__ __forceinline__ void point_act(float (&z)[N], int act, int f32) {
+  if (act == DWM_ACT_SILU)
+    act_of_n<DWM_ACT_SILU>(z, f32);
+  else if (act == DWM_ACT_GELU)
+    act_of_n<DWM_ACT_GELU>(z, f32);
+  else
+    act_of_n<DWM_ACT_GELU_TANH>(z, f32);
+}
+template <int EPI, int N>
+__device__ __forceinline__ void activate(const Args& a, float (&z)[N], float (&u)[N]) {
+  if (EPI == GLU) {
+    if (a.act == DWM_ACT_SWIGLU_CLAMP) {
+#pragma unroll
+      for (int q = 0; q < N; ++q) {
+        z[q] = fminf(z[q], a.limit);
+        u[q] = fminf(fmaxf(u[q], -a.limit), a.limit);
+      }
+    }
+    if (a.out_f32) {
+#pragma unroll
+      for (int q = 0; q < N; ++q) z[q] = z[q] * sigmoid_full(z[q]) * u[q];
+    } else {
+#pragma unroll
+      for (int q = 0; q < N; ++q) z[q] = z[q] * sigmoid_fast(z[q]) * u[q];
+    }
+  } else if (EPI == POINT) {
+    point_act(z, a.act, a.out_f32);
+  }
+}
+
+// Outputs [col, col + N) of row `row`, N = 8 or 16, from the products z (and,
+// with SwiGLU, the up products u): bias, activation, residual, one rounding.
+// Rows of out start on 16 bytes (Args::out_vec).
+template <int EPI, int N>
+__device__ __forceinline__ void epilogue(const Args& a, int64_t row, int col, float (&z)[N],
+                                         float (&u)[N]) {
+  const bool whole = col + N <= a.n_out;
+  if (a.bias) {
+    float b[N];
+    auto bias = [&](int off) {
+      if (whole && a.bias_vec) {
+        load_n(a.bias, off + col, a.bias_f32, b);
+      } else {
+#pragma unroll
+        for (int q = 0; q < N; ++q) b[q] = ld1(a.bias, off + min(col + q, a.n_out - 1), a.bias_f32);
+      }
+    };
+    bias(0);
+#pragma unroll
+    for (int q = 0; q < N; ++q) z[q] += b[q];
+    if (EPI == GLU) {
+      bias(a.n_out);
+#pragma unroll
+      for (int q = 0; q < N; ++q) u[q] += b[q];
+    }
+  }
+  activate<EPI>(a, z, u);
   if (a.residual) {
     const int64_t at = row * a.ldr + col;
     if (whole && a.res_vec) {
-      float r[8];
-      if (a.res_f32) {
-        const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(a.residual) + at);
-        const float4 x = p[0], y = p[1];
-        r[0] = x.x; r[1] = x.y; r[2] = x.z; r[3] = x.w;
-        r[4] = y.x; r[5] = y.y; r[6] = y.z; r[7] = y.w;
-      } else {
-        const uint4 x =
-            *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.residual) + at);
-        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+      float r[N];
+      load_n(a.residual, at, a.res_f32, r);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          r[2 * q] = __uint_as_float(w[q] << 16);
-          r[2 * q + 1] = __uint_as_float(w[q] & 0xFFFF0000u);
-        }
-      }
-#pragma unroll
-      for (int q = 0; q < 8; ++q) z[q] = fmaf(a.res_scale, r[q], z[q]);
+      for (int q = 0; q < N; ++q) z[q] = fmaf(a.res_scale, r[q], z[q]);
     } else {
 #pragma unroll
-      for (int q = 0; q < 8; ++q)
+      for (int q = 0; q < N; ++q)
         if (col + q < a.n_out) z[q] = fmaf(a.res_scale, ld1(a.residual, at + q, a.res_f32), z[q]);
     }
   }
   const int64_t at = row * a.ldo + col;
-  if (whole && a.out_vec) {
-    if (a.out_f32) {
-      float4* p = reinterpret_cast<float4*>(static_cast<float*>(a.out) + at);
-      p[0] = make_float4(z[0], z[1], z[2], z[3]);
-      p[1] = make_float4(z[4], z[5], z[6], z[7]);
-    } else {
-      uint4 o;
-      o.x = f32_to_bf16_bits(z[0]) | (f32_to_bf16_bits(z[1]) << 16);
-      o.y = f32_to_bf16_bits(z[2]) | (f32_to_bf16_bits(z[3]) << 16);
-      o.z = f32_to_bf16_bits(z[4]) | (f32_to_bf16_bits(z[5]) << 16);
-      o.w = f32_to_bf16_bits(z[6]) | (f32_to_bf16_bits(z[7]) << 16);
-      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + at) = o;
-    }
+  if (whole) {
+    store_n(a.out, at, a.out_f32, a.out_wide != 0, z);
   } else {
 #pragma unroll
-    for (int q = 0; q < 8; ++q)
+    for (int q = 0; q < N; ++q)
       if (col + q < a.n_out) {
         if (a.out_f32)
           static_cast<float*>(a.out)[at + q] = z[q];
@@ -155,30 +240,84 @@ __device__ __forceinline__ void epilogue8(const Args& a, int64_t row, int col, f
   }
 }
 
-// 4 floats of another CTA's shared memory, by its shared::cluster address.
-__device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-               : "r"(addr)
-               : "memory");
-  return v;
+// For outputs whose rows do not start on 16 bytes: column `col` of the rows
+// [row, row + n), n <= N; neighbouring threads take neighbouring columns. Eight
+// rows at a time keep the loads and functions of several in flight (one at a
+// time took 10 us more for 1024 x 777).
+template <int EPI, int N>
+__device__ __forceinline__ void epilogue_column(const Args& a, int64_t row, int n, int col,
+                                                float (&z)[N], float (&u)[N]) {
+  if (a.bias) {
+    const float b = ld1(a.bias, col, a.bias_f32);
+#pragma unroll
+    for (int q = 0; q < N; ++q) z[q] += b;
+    if (EPI == GLU) {
+      const float c = ld1(a.bias, a.n_out + col, a.bias_f32);
+#pragma unroll
+      for (int q = 0; q < N; ++q) u[q] += c;
+    }
+  }
+  activate<EPI>(a, z, u);
+  if (a.residual) {
+    float r[N];
+    const int64_t at = row * a.ldr + col;
+    if (a.res_f32) {
+#pragma unroll
+      for (int q = 0; q < N; ++q)
+        r[q] = static_cast<const float*>(a.residual)[at + (int64_t)min(q, n - 1) * a.ldr];
+    } else {
+#pragma unroll
+      for (int q = 0; q < N; ++q)
+        r[q] = bf16_bits_to_f32(
+            static_cast<const uint16_t*>(a.residual)[at + (int64_t)min(q, n - 1) * a.ldr]);
+    }
+#pragma unroll
+    for (int q = 0; q < N; ++q) z[q] = fmaf(a.res_scale, r[q], z[q]);
+  }
+  const int64_t at = row * a.ldo + col;
+  if (a.out_f32) {
+    float* o = static_cast<float*>(a.out) + at;
+#pragma unroll
+    for (int q = 0; q < N; ++q)
+      if (q < n) o[q * a.ldo] = z[q];
+  } else {
+    uint16_t* o = static_cast<uint16_t*>(a.out) + at;
+#pragma unroll
+    for (int q = 0; q < N; ++q)
+      if (q < n) o[q * a.ldo] = (uint16_t)f32_to_bf16_bits(z[q]);
+  }
+}
+
+// A bulk copy from this CTA's shared memory to CTA `to` of the cluster, which
+// completes on that CTA's mbarrier. dst, bar: the addresses here of what they
+// are there.
+__device__ __forceinline__ void bulk_to_cta(uint32_t dst, uint32_t src, uint32_t bytes,
+                                            uint32_t bar, int to) {
+  asm volatile(
+      "{\n\t.reg .b32 d, b;\n\t"
+      "mapa.shared::cluster.u32 d, %0, %4;\n\t"
+      "mapa.shared::cluster.u32 b, %3, %4;\n\t"
+      "cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [d], [%1], %2, [b];"
+      "\n\t}" ::"r"(dst),
+      "r"(src), "r"(bytes), "r"(bar), "r"(to)
+      : "memory");
 }
 
 // grid (cluster, w tiles, x tiles); GLU: the tile's 128 rows of w are 64 gate
 // rows and the up rows of the same features.
-template <int BT, bool GLU>
-__global__ void __launch_bounds__(THREADS, 2)
+template <int BT, int EPI>
+__global__ void __launch_bounds__(THREADS, 1)
     dense_split_kernel(const __grid_constant__ CUtensorMap tm_w,
                        const __grid_constant__ CUtensorMap tm_x, const Args a) {
   using L = Layout<BT>;
   constexpr int S = L::S;
-  constexpr int FEAT = GLU ? TILE_W / 2 : TILE_W;  // output columns of a tile
+  constexpr int FEAT = EPI == GLU ? TILE_W / 2 : TILE_W;  // output columns of a tile
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR);
   uint64_t* empty = full + S;
   uint64_t* done = empty + S;
+  uint64_t* received = done + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::OFF_MISC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::OFF_MISC + 4);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -196,6 +335,7 @@ __global__ void __launch_bounds__(THREADS, 2)
       mbar_init(&empty[i], 1);
     }
     mbar_init(done, 1);
+    mbar_init(received, 1);
     *abort_flag = 0;
     fence_mbar_init();
     tma_prefetch_desc(&tm_w);
@@ -222,7 +362,7 @@ __global__ void __launch_bounds__(THREADS, 2)
         mbar_arrive_expect_tx(&full[st], L::STG);
         uint8_t* dst = smem + st * L::STG;
         const int x = (k_lo + i) * BK;
-        if (GLU) {
+        if (EPI == GLU) {
           tma_load_2d(dst, &tm_w, &full[st], x, col0, pol_w);
           tma_load_2d(dst + A_STAGE / 2, &tm_w, &full[st], x, a.n_out + col0, pol_w);
         } else {
@@ -263,70 +403,158 @@ __global__ void __launch_bounds__(THREADS, 2)
   bool ok = mbar_wait(done, 0, nullptr, a.status);
   ok = __syncthreads_and(ok) != 0 && *abort_flag == 0;
   tc_fence_after();
-  float* part = reinterpret_cast<float*>(smem);
+  const int rows = min(BT, a.m - row0);
+  const int own = BT / split;  // this CTA's rows of x: from rank * own
+  const int mine = max(0, min(own, rows - rank * own));
+  const uint32_t part = smem_u32(smem);
   {
-    // Warp w reads TMEM lanes (rows of w) 32 (w % 4) .. and one half of the
-    // columns (rows of x).
+    // The partial tile [row of x][row of w]. Warp w reads TMEM lanes (rows of
+    // w) 32 (w % 4) .. and one half of the columns (rows of x).
     const int q = warp & 3, half = warp >> 2;
     constexpr int COLS = BT / 2 < 16 ? 16 : BT / 2;
     if (half * COLS < BT) {
 #pragma unroll
       for (int c = 0; c < COLS; c += 16) {
+        const int t0 = half * COLS + c;
+        if (t0 >= rows) break;
         uint32_t r[16];
-        tmem_ld16(tmem + ((uint32_t)(q * 32) << 16) + half * COLS + c, r);
-        tmem_ld_wait();
+        tmem_ld16(tmem + ((uint32_t)(q * 32) << 16) + t0, r);
+        tmem_ld_wait(r);
 #pragma unroll
         for (int e = 0; e < 16; ++e)
-          part[(half * COLS + c + e) * TILE_W + q * 32 + lane] = __uint_as_float(r[e]);
+          sts_u32(part + (uint32_t)(((t0 + e) * TILE_W + q * 32 + lane) * 4), r[e]);
       }
     }
   }
   tc_fence_before();
-  if (split > 1)
+  if (split > 1) {
+    fence_proxy_async_smem();  // the partials, for the bulk copies
+    if (threadIdx.x == 0)
+      mbar_arrive_expect_tx(received, (uint32_t)((split - 1) * mine * TILE_W * 4));
+    // Every CTA of the cluster is done with its stages, where the partials of
+    // the others now go.
     cluster_sync();
-  else
+    if ((int)threadIdx.x < split && (int)threadIdx.x != rank) {
+      const int to = threadIdx.x, n = max(0, min(own, rows - to * own));
+      if (n > 0)
+        bulk_to_cta(part + (uint32_t)(L::OFF_RECV + (rank - (rank > to)) * own * TILE_W * 4),
+                    part + (uint32_t)(to * own * TILE_W * 4), (uint32_t)(n * TILE_W * 4),
+                    smem_u32(received), to);
+    }
+    __syncwarp();
+    ok = mbar_wait(received, 0, nullptr, a.status) && ok;
+    __syncwarp();
+    cluster_arrive();  // this CTA has what it waits for
+  } else {
     __syncthreads();
+  }
   tc_fence_after();
   if (warp == 1) tmem_dealloc(tmem, L::TMEM_COLS);
 
-  // This CTA's share of the tile's outputs, 8 columns a thread.
+  // This CTA's rows: the partials in CTA order, 8 columns a thread.
   if (ok) {
-    constexpr int CH = FEAT / 8;
-    const int rows = min(BT, a.m - row0);
-    const int items = rows * CH;
-    const int lo = (int)((int64_t)items * rank / split), hi = (int)((int64_t)items * (rank + 1) / split);
-    const uint32_t base = smem_u32(part);
-    for (int i = lo + (int)threadIdx.x; i < hi; i += THREADS) {
-      const int t = i / CH, c = (i % CH) * 8;
-      if (col0 + c >= a.n_out) continue;
-      float z[8], u[8];
+    const int cols = min(FEAT, a.n_out - col0);
+    // Where CTA p's partials of the own rows are.
+    auto from = [&](int p) {
+      return part + (uint32_t)((p == rank ? rank * own * TILE_W * 4
+                                          : L::OFF_RECV + (p - (p > rank)) * own * TILE_W * 4));
+    };
+    if (a.out_vec) {
+      constexpr int CH = FEAT / 8;
+      for (int i = threadIdx.x; i < mine * CH; i += THREADS) {
+        const int t = i / CH, c = (i % CH) * 8;
+        if (c >= cols) continue;
+        float z[8], u[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) z[e] = u[e] = 0.0f;
-      const uint32_t off = base + (uint32_t)((t * TILE_W + c) * 4);
-      for (int p = 0; p < split; ++p) {
-        uint32_t at;
-        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(off), "r"(p));
-        const float4 x = ld_cluster_f4(at), y = ld_cluster_f4(at + 16);
-        z[0] += x.x; z[1] += x.y; z[2] += x.z; z[3] += x.w;
-        z[4] += y.x; z[5] += y.y; z[6] += y.z; z[7] += y.w;
-        if (GLU) {
-          const float4 v = ld_cluster_f4(at + FEAT * 4), w = ld_cluster_f4(at + FEAT * 4 + 16);
-          u[0] += v.x; u[1] += v.y; u[2] += v.z; u[3] += v.w;
-          u[4] += w.x; u[5] += w.y; u[6] += w.z; u[7] += w.w;
+        for (int e = 0; e < 8; ++e) z[e] = u[e] = 0.0f;
+        auto add = [](float (&v)[8], uint32_t p) {
+          const uint4 x = lds_u128(p), y = lds_u128(p + 16);
+          v[0] += __uint_as_float(x.x); v[1] += __uint_as_float(x.y);
+          v[2] += __uint_as_float(x.z); v[3] += __uint_as_float(x.w);
+          v[4] += __uint_as_float(y.x); v[5] += __uint_as_float(y.y);
+          v[6] += __uint_as_float(y.z); v[7] += __uint_as_float(y.w);
+        };
+        for (int p = 0; p < split; ++p) {
+          const uint32_t at = from(p) + (uint32_t)((t * TILE_W + c) * 4);
+          add(z, at);
+          if (EPI == GLU) add(u, at + FEAT * 4);
         }
+        epilogue<EPI>(a, row0 + rank * own + t, col0 + c, z, u);
       }
-      epilogue8(a, row0 + t, col0 + c, z, u);
+    } else {
+      const int c = threadIdx.x % FEAT;
+      if (c < cols)
+        for (int t = threadIdx.x / FEAT * 8; t < mine; t += THREADS / FEAT * 8) {
+          float z[8], u[8];
+#pragma unroll
+          for (int q = 0; q < 8; ++q) z[q] = u[q] = 0.0f;
+          for (int p = 0; p < split; ++p) {
+            // (Rows past the own ones are read within the shared memory, and
+            // dropped.)
+            const uint32_t at = from(p) + (uint32_t)((t * TILE_W + c) * 4);
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+              z[q] += lds_f32(at + q * TILE_W * 4);
+              if (EPI == GLU) u[q] += lds_f32(at + (q * TILE_W + FEAT) * 4);
+            }
+          }
+          epilogue_column<EPI>(a, row0 + rank * own + t, min(8, mine - t), col0 + c, z, u);
+        }
     }
   }
+  // A CTA's partials may still be on their way to another one until all have
+  // arrived.
   __syncwarp();
-  if (split > 1) cluster_sync();  // no CTA exits while another reads its tile
+  if (split > 1) cluster_wait();
 }
 
-template <int BT, bool GLU>
+// Clusters of `size` CTAs, one CTA per SM, resident at once on the current
+// device (asked once of each): as many as the split kernel with its largest
+// shared memory allows, which the pair kernel's equals.
+int resident_clusters(int size) {
+  constexpr int kMaxDevices = 64;
+  static std::atomic<int> cached[kMaxDevices][4] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const int i = size == 1 ? 0 : size == 2 ? 1 : size == 4 ? 2 : 3;
+  const bool keep = dev >= 0 && dev < kMaxDevices;
+  if (keep) {
+    const int n = cached[dev][i].load(std::memory_order_relaxed);
+    if (n) return n;
+  }
+  int n = num_sms() / size;
+  if (size > 1) {
+    using L = Layout<128>;
+    auto fn = dense_split_kernel<128, PLAIN>;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)size;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)size, (unsigned)std::max(1, n));
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = L::ALLOC;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int got = 0;
+    if (set_smem_limit(reinterpret_cast<const void*>(fn), L::ALLOC, "dense smem attribute") ==
+            DWM_OK &&
+        cudaOccupancyMaxActiveClusters(&got, fn, &cfg) == cudaSuccess && got > 0)
+      n = got;
+    else
+      (void)cudaGetLastError();
+  }
+  n = std::max(1, n);
+  if (keep) cached[dev][i].store(n, std::memory_order_relaxed);
+  return n;
+}
+
+template <int BT, int EPI>
 int launch_split(const void* x, int64_t ldx, const void* w, int64_t ldw, int n, int split,
                  const Args& a, cudaStream_t stream) {
   using L = Layout<BT>;
-  constexpr int FEAT = GLU ? TILE_W / 2 : TILE_W;
+  constexpr int FEAT = EPI == GLU ? TILE_W / 2 : TILE_W;
   DWM_CHECK_ARG((a.m + (int64_t)BT - 1) / BT <= 65535 && (a.n_out + (int64_t)FEAT - 1) / FEAT <= 65535,
                 "m=%d rows by %d columns exceed the grid", a.m, a.n_out);
   CUtensorMap tm_w, tm_x;
@@ -336,7 +564,7 @@ int launch_split(const void* x, int64_t ldx, const void* w, int64_t ldw, int n, 
   rc = encode_tmap_2d(&tm_x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, x, (uint64_t)a.k, (uint64_t)a.m,
                       (uint64_t)ldx * 2, BK, BT, CU_TENSOR_MAP_SWIZZLE_128B);
   if (rc) return rc;
-  rc = set_smem_limit(reinterpret_cast<const void*>(dense_split_kernel<BT, GLU>), L::ALLOC,
+  rc = set_smem_limit(reinterpret_cast<const void*>(dense_split_kernel<BT, EPI>), L::ALLOC,
                       "dense smem attribute");
   if (rc) return rc;
   cudaLaunchAttribute attr[1];
@@ -352,28 +580,355 @@ int launch_split(const void* x, int64_t ldx, const void* w, int64_t ldw, int n, 
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return check_cuda(cudaLaunchKernelEx(&cfg, dense_split_kernel<BT, GLU>, tm_w, tm_x, a),
+  return check_cuda(cudaLaunchKernelEx(&cfg, dense_split_kernel<BT, EPI>, tm_w, tm_x, a),
                     "dense_matmul launch");
+}
+
+// ---------------------------------------------------------------------------
+// Pair kernel (prompts). Two CTAs on neighbouring SMs (cta_group::2) share a
+// tile of 256 rows of x by 256 rows of w: each CTA loads its 128 rows of both
+// (one box each a k step), the even one issues the 256 x 256 x 16 UMMAs, and
+// each CTA's TMEM receives its 128 rows of x by all 256 columns, twice (the
+// epilogue of a tile overlaps the main loop of the next). Persistent: one pair
+// of SMs takes every ncl-th tile, eight rows of tiles at a time so that what
+// runs together shares its operands in L2. With SwiGLU the even CTA's half of
+// w's rows is the gate and the odd one's the up projection of 128 features, so
+// a feature's two products are two columns of one TMEM lane.
+//
+// Warps 0-7 epilogue (TMEM lane quarter w % 4, half w / 4 of the columns): a
+// row a lane, stored a 32-byte sector at a time; warp 8 TMA; warp 9 UMMA.
+//
+// Bound: the tensor cores.
+// ---------------------------------------------------------------------------
+namespace pair {
+
+constexpr int TILE = 256;      // rows of x, and of w, per tile
+constexpr int HALF = 128;      // per CTA
+constexpr int THREADS = 320;
+constexpr int EPI_WARPS = 8, TMA_WARP = 8, MMA_WARP = 9;
+constexpr int OP_STAGE = HALF * BK * 2;  // 16 KiB: one operand's k step
+constexpr int STG = 2 * OP_STAGE;
+constexpr int S = 6;
+constexpr int EPI_BYTES = 32 * 32 * 4;   // a warp's 32 x 32 f32
+constexpr int OFF_EPI = S * STG;
+constexpr int OFF_BAR = OFF_EPI + EPI_WARPS * EPI_BYTES;
+constexpr int OFF_MISC = OFF_BAR + (2 * S + 5) * 8;
+constexpr int ALLOC = OFF_MISC + 16 + 1024;  // slack for 1 KiB alignment
+static_assert(ALLOC <= 232448, "exceeds the 227 KiB per-CTA shared memory");
+constexpr int TMEM_COLS = 512;
+constexpr int GROUP_ROWS = 8;  // rows of tiles taken together
+
+__device__ __forceinline__ void tile_at(int idx, int mt, int nt, int& tm, int& tn) {
+  const int per = GROUP_ROWS * nt, g = idx / per;
+  const int rows = min(GROUP_ROWS, mt - g * GROUP_ROWS);
+  const int in = idx - g * per;
+  tm = g * GROUP_ROWS + in % rows;
+  tn = in / rows;
+}
+
+template <int EPI, bool VEC>  // VEC: rows of out start on 16 bytes
+__global__ void __launch_bounds__(THREADS, 1)
+    dense_pair_kernel(const __grid_constant__ CUtensorMap tm_x,
+                      const __grid_constant__ CUtensorMap tm_w, const Args a) {
+  constexpr int FEAT = EPI == GLU ? HALF : TILE;  // output columns of a tile
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + OFF_BAR);  // even CTA: both CTAs' copies landed
+  uint64_t* empty = full + S;          // each CTA: the pair's UMMAs done with the stage
+  uint64_t* acc_full = empty + S;      // each CTA: accumulator complete
+  uint64_t* acc_empty = acc_full + 2;  // even CTA: both CTAs drained it
+  uint64_t* drain = acc_empty + 2;     // each CTA: every UMMA complete
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + OFF_MISC);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + OFF_MISC + 4);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const int cl = (int)cluster_index(), ncl = (int)cluster_count();
+  const int mt = (a.m + TILE - 1) / TILE, nt = (a.n_out + FEAT - 1) / FEAT;
+  const int total = mt * nt;
+  const int kt = (a.k + BK - 1) / BK;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < S; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&acc_full[i], 1);
+      mbar_init(&acc_empty[i], 2 * EPI_WARPS);
+    }
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&tm_x);
+    tma_prefetch_desc(&tm_w);
+  }
+  if (warp == MMA_WARP) {
+    tmem_alloc_pair(tmem_slot, TMEM_COLS);
+    tmem_relinquish_pair();
+  }
+  // Barriers initialised and TMEM allocated in both CTAs before any
+  // cross-CTA arrival.
+  tc_fence_before();
+  cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const uint32_t full_0 = mapa_shared(full, 0);
+  const uint32_t acc_empty_0 = mapa_shared(acc_empty, 0);
+
+  if (warp < EPI_WARPS) {
+    const int q = warp & 3, half = warp >> 2;
+    const uint32_t stage = smem_u32(smem + OFF_EPI + warp * EPI_BYTES);
+    int slot = 0;
+    uint32_t ph = 0;
+    for (int idx = cl; idx < total; idx += ncl) {
+      int tm, tn;
+      tile_at(idx, mt, nt, tm, tn);
+      const int64_t row0 = (int64_t)tm * TILE + rank * HALF + q * 32;
+      const int col0 = tn * FEAT + half * (FEAT / 2);
+      const int valid = (int)min((int64_t)32, a.m - row0);  // rows, maybe none
+      if (!__all_sync(0xffffffffu, mbar_wait<64>(&acc_full[slot], ph, abort_flag, a.status))) break;
+      tc_fence_after();
+      const uint32_t acc =
+          tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(slot * TILE + half * (FEAT / 2));
+      constexpr int CHUNK = EPI == GLU ? 16 : 32;  // output columns a step
+      const int steps = valid <= 0 ? 0 : min(FEAT / 2, a.n_out - col0 + CHUNK - 1) / CHUNK;
+      // Two blocks of 16 columns a step: neighbours, or gate and up.
+      uint32_t r0[16], r1[16];
+      auto fetch = [&](int c) {
+        tmem_ld16(acc + c, r0);
+        tmem_ld16(acc + c + (EPI == GLU ? HALF : 16), r1);
+      };
+      if (steps > 0) fetch(0);
+      for (int i = 0; i < steps; ++i) {
+        const int c = i * CHUNK;
+        tmem_ld_wait(r0);
+        tmem_ld_wait(r1);
+        if (VEC) {
+          // A row a lane: 16 columns are 32 or 64 bytes of it.
+          float z[16], u[16];
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            z[j] = __uint_as_float(r0[j]);
+            u[j] = __uint_as_float(r1[j]);
+          }
+          if (i + 1 < steps) fetch(c + CHUNK);
+          if (lane < valid) {
+            epilogue<EPI>(a, row0 + lane, col0 + c, z, u);
+            if (EPI != GLU && col0 + c + 16 < a.n_out)
+              epilogue<EPI>(a, row0 + lane, col0 + c + 16, u, z);
+          }
+        } else {
+          // A column a lane (with SwiGLU two rows of 16 at a time), by way of
+          // shared memory: 16-byte blocks of a row, XORed with the row against
+          // bank conflicts.
+          auto block_at = [&](int rr, int j) {
+            return stage + (uint32_t)(rr * 128 + ((j ^ (rr & 7)) << 4));
+          };
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            sts_u128(block_at(lane, j), r0[4 * j], r0[4 * j + 1], r0[4 * j + 2], r0[4 * j + 3]);
+            sts_u128(block_at(lane, 4 + j), r1[4 * j], r1[4 * j + 1], r1[4 * j + 2],
+                     r1[4 * j + 3]);
+          }
+          __syncwarp();
+          if (i + 1 < steps) fetch(c + CHUNK);
+          const int col = lane % CHUNK;
+          if (col0 + c + col < a.n_out)
+            for (int rr = lane / CHUNK * 8; rr < valid; rr += 32 / CHUNK * 8) {
+              float z[8], u[8];
+#pragma unroll
+              for (int q = 0; q < 8; ++q) {
+                z[q] = lds_f32(block_at(rr + q, col / 4) + (uint32_t)(col % 4) * 4);
+                if (EPI == GLU)
+                  u[q] = lds_f32(block_at(rr + q, 4 + col / 4) + (uint32_t)(col % 4) * 4);
+              }
+              epilogue_column<EPI>(a, row0 + rr, min(8, valid - rr), col0 + c + col, z, u);
+            }
+          __syncwarp();
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_remote(acc_empty_0 + (uint32_t)(slot * 8));
+      if (++slot == 2) { slot = 0; ph ^= 1; }
+    }
+  } else if (warp == TMA_WARP) {
+    if (lane == 0) {
+      const uint64_t pol_w = policy_evict_last(), pol_x = policy_evict_normal();
+      int st = 0;
+      uint32_t ph = 0, armed = 0, par = 0;
+      bool ok = true;
+      for (int idx = cl; idx < total && ok; idx += ncl) {
+        int tm, tn;
+        tile_at(idx, mt, nt, tm, tn);
+        const int xrow = tm * TILE + (int)rank * HALF;
+        const int wrow = EPI == GLU ? tn * FEAT + (rank ? a.n_out : 0) : tn * FEAT + (int)rank * HALF;
+        for (int kk = 0; kk < kt; ++kk) {
+          if (!mbar_wait(&empty[st], ph ^ 1, abort_flag, a.status)) {
+            ok = false;
+            break;
+          }
+          if (rank == 0) mbar_arrive_expect_tx(&full[st], 2 * STG);
+          armed |= 1u << st;
+          par = (par & ~(1u << st)) | (ph << st);
+          const uint32_t bar = full_0 + (uint32_t)(st * 8);
+          uint8_t* dst = smem + st * STG;
+          tma_load_2d_pair(dst, &tm_x, bar, kk * BK, xrow, pol_x);
+          tma_load_2d_pair(dst + OP_STAGE, &tm_w, bar, kk * BK, wrow, pol_w);
+          if (++st == S) { st = 0; ph ^= 1; }
+        }
+      }
+      // Every stage this warp filled is released by the pair's UMMAs (so its
+      // copies have landed) before the CTA can exit.
+      for (int i = 0; i < S; ++i)
+        if (armed & (1u << i)) mbar_wait(&empty[i], (par >> i) & 1, nullptr, a.status);
+    }
+  } else {
+    if (rank == 0) {
+      const bool issuer = elect_one();
+      constexpr uint32_t idesc = idesc_bf16(TILE, TILE, false, false);
+      int st = 0, slot = 0;
+      uint32_t ph = 0, acc_ph = 0;
+      bool ok = true;
+      for (int idx = cl; idx < total && ok; idx += ncl) {
+        if (!__all_sync(0xffffffffu, mbar_wait(&acc_empty[slot], acc_ph ^ 1, abort_flag, a.status)))
+          break;
+        tc_fence_after();
+        const uint32_t d = tmem + (uint32_t)(slot * TILE);
+        for (int kk = 0; kk < kt; ++kk) {
+          if (!__all_sync(0xffffffffu, mbar_wait(&full[st], ph, abort_flag, a.status))) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          if (issuer) {
+            const uint32_t base = smem_u32(smem + st * STG);
+#pragma unroll
+            for (int j = 0; j < BK / 16; ++j)
+              umma_pair_bf16(d, smem_desc_sw128(base + j * 32, 16, 1024),
+                             smem_desc_sw128(base + OP_STAGE + j * 32, 16, 1024), idesc,
+                             (kk | j) != 0);
+            umma_commit_pair(&empty[st]);
+          }
+          __syncwarp();
+          if (++st == S) { st = 0; ph ^= 1; }
+        }
+        if (!ok) break;
+        if (issuer) umma_commit_pair(&acc_full[slot]);
+        __syncwarp();
+        if (++slot == 2) { slot = 0; acc_ph ^= 1; }
+      }
+      if (issuer) umma_commit_pair(drain);
+      __syncwarp();
+    }
+    // Both CTAs: every UMMA (which writes both TMEMs) completes before TMEM
+    // is released.
+    // The odd CTA waits here from the start, so its limit grows with the tiles.
+    if (lane == 0) {
+      const uint64_t t0 = globaltimer_ns(), limit = kWaitLimitNs * (uint64_t)(1 + total / ncl);
+      while (!mbar_try_wait(drain, 0)) {
+        __nanosleep(500);
+        if (globaltimer_ns() - t0 > limit) {
+          report(a.status, DWM_DEV_TIMEOUT);
+          break;
+        }
+      }
+    }
+  }
+  // Both CTAs are done with every barrier, shared tile and TMEM column.
+  __syncwarp();
+  tc_fence_before();
+  cluster_sync();
+  if (warp == MMA_WARP) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem, TMEM_COLS);
+  }
+  cluster_sync();
+}
+
+template <int EPI, bool VEC>
+int launch(const void* x, int64_t ldx, const void* w, int64_t ldw, int n, const Args& a,
+           cudaStream_t stream) {
+  constexpr int FEAT = EPI == GLU ? HALF : TILE;
+  const int64_t tiles = (int64_t)((a.m + (int64_t)TILE - 1) / TILE) *
+                        ((a.n_out + (int64_t)FEAT - 1) / FEAT);
+  DWM_CHECK_ARG(tiles < (1ll << 30), "m=%d rows by %d columns are too many tiles", a.m, a.n_out);
+  CUtensorMap tm_x, tm_w;
+  int rc = encode_tmap_2d(&tm_x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, x, (uint64_t)a.k, (uint64_t)a.m,
+                          (uint64_t)ldx * 2, BK, HALF, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (rc) return rc;
+  rc = encode_tmap_2d(&tm_w, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, w, (uint64_t)a.k, (uint64_t)n,
+                      (uint64_t)ldw * 2, BK, HALF, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (rc) return rc;
+  rc = set_smem_limit(reinterpret_cast<const void*>(dense_pair_kernel<EPI, VEC>), ALLOC,
+                      "dense pair smem attribute");
+  if (rc) return rc;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = ALLOC;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cfg.gridDim = dim3(2 * (unsigned)std::min<int64_t>(tiles, resident_clusters(2)));
+  return check_cuda(cudaLaunchKernelEx(&cfg, dense_pair_kernel<EPI, VEC>, tm_x, tm_w, a),
+                    "dense_matmul launch");
+}
+
+}  // namespace pair
+
+// The kernel and the split by what they take, in us, as fitted to times of both
+// at k = 512 .. 8192, n = 256 .. 8192, m = 1 .. 8192:
+//   split kernel  1.5 + waves * (max(0.23 * k steps of a CTA, w and x over HBM)
+//                                + 4 + (split > 1 ? 0.5 + 1.5 * rows of a tile / 128 : 0))
+//   pair kernel   6.5 + waves * max(0.27 * k steps, 4)
+// e.g. k = n = 4096, SwiGLU, m = 512: split 21.3 us, pair 26.9; m = 1024: 42.1
+// and 29.4. One CTA per SM in both: a wave is as many clusters as fit (of 8
+// CTAs fewer than 18, since a cluster stays within a GPC).
+template <int EPI>
+int run_epi(const void* x, int64_t ldx, const void* w, int64_t ldw, int n, const Args& a,
+            cudaStream_t stream) {
+  const int bt = a.m <= 16 ? 16 : a.m <= 32 ? 32 : a.m <= 64 ? 64 : 128;
+  const int feat = EPI == GLU ? TILE_W / 2 : TILE_W, pfeat = EPI == GLU ? 128 : 256;
+  const int64_t tiles = (int64_t)((a.n_out + feat - 1) / feat) * ((a.m + bt - 1) / bt);
+  const int64_t ptiles = (int64_t)((a.n_out + pfeat - 1) / pfeat) * ((a.m + 255) / 256);
+  const int kt = (a.k + BK - 1) / BK;
+  auto waves = [](int64_t tiles, int cluster) {
+    const int64_t c = resident_clusters(cluster);
+    return (float)((tiles + c - 1) / c);
+  };
+  const float hbm = 2.0f * (float)a.k * ((float)a.m + (float)n) / 6.5e6f;
+  int split = 1;
+  float best = 0.0f;
+  for (int s = 1; s <= MAX_CLUSTER && (s == 1 || kt >= 2 * s); s *= 2) {
+    const float v = waves(tiles, s);
+    const float t = 1.5f + v * (std::max(0.23f * (float)((kt + s - 1) / s), hbm / v) + 4.0f +
+                                (s > 1 ? 0.5f + 1.5f * (float)bt / 128.0f : 0.0f));
+    if (s == 1 || t < best) {
+      best = t;
+      split = s;
+    }
+  }
+  const float t_pair = 6.5f + waves(ptiles, 2) * std::max(0.27f * (float)kt, 4.0f);
+  if (t_pair < best)
+    return a.out_vec ? pair::launch<EPI, true>(x, ldx, w, ldw, n, a, stream)
+                     : pair::launch<EPI, false>(x, ldx, w, ldw, n, a, stream);
+  if (bt == 16) return launch_split<16, EPI>(x, ldx, w, ldw, n, split, a, stream);
+  if (bt == 32) return launch_split<32, EPI>(x, ldx, w, ldw, n, split, a, stream);
+  if (bt == 64) return launch_split<64, EPI>(x, ldx, w, ldw, n, split, a, stream);
+  return launch_split<128, EPI>(x, ldx, w, ldw, n, split, a, stream);
 }
 
 int run(const void* x, int64_t ldx, const void* w, int64_t ldw, int n, const Args& a,
         cudaStream_t stream) {
-  const bool glu = a.act == DWM_ACT_SWIGLU || a.act == DWM_ACT_SWIGLU_CLAMP;
-  const int bt = a.m <= 16 ? 16 : a.m <= 32 ? 32 : a.m <= 64 ? 64 : 128;
-  const int feat = glu ? TILE_W / 2 : TILE_W;
-  const int64_t tiles = (int64_t)((a.n_out + feat - 1) / feat) * ((a.m + bt - 1) / bt);
-  const int kt = (a.k + BK - 1) / BK;
-  // Two CTAs per SM; at least two k steps a CTA.
-  int split = 1;
-  while (split < MAX_CLUSTER && tiles * split * 2 <= 2 * num_sms() && kt >= 4 * split) split *= 2;
-#define DWM_DENSE_SPLIT(BT)                                                     \
-  return glu ? launch_split<BT, true>(x, ldx, w, ldw, n, split, a, stream)      \
-             : launch_split<BT, false>(x, ldx, w, ldw, n, split, a, stream)
-  if (bt == 16) DWM_DENSE_SPLIT(16);
-  if (bt == 32) DWM_DENSE_SPLIT(32);
-  if (bt == 64) DWM_DENSE_SPLIT(64);
-  DWM_DENSE_SPLIT(128);
-#undef DWM_DENSE_SPLIT
+  if (a.act == DWM_ACT_NONE) return run_epi<PLAIN>(x, ldx, w, ldw, n, a, stream);
+  if (a.act == DWM_ACT_SWIGLU || a.act == DWM_ACT_SWIGLU_CLAMP)
+    return run_epi<GLU>(x, ldx, w, ldw, n, a, stream);
+  return run_epi<POINT>(x, ldx, w, ldw, n, a, stream);
 }
 
 }  // namespace dense
@@ -437,8 +992,10 @@ extern "C" int dwm_dense_matmul(const void* x, int64_t ldx, const void* w, int64
   a.bias_f32 = bias_dtype == DWM_F32;
   a.res_f32 = residual_dtype == DWM_F32;
   a.out_f32 = out_dtype == DWM_F32;
+  a.bias_vec = bias && addr(bias) % 16 == 0 && (!glu || (int64_t)n_out * bes % 16 == 0);
   a.res_vec = residual && addr(residual) % 16 == 0 && ldr * res % 16 == 0;
   a.out_vec = addr(out) % 16 == 0 && ldo * oes % 16 == 0;
+  a.out_wide = addr(out) % 32 == 0 && ldo * oes % 32 == 0;
   a.limit = act_limit;
   a.res_scale = residual_scale;
   a.status = status_ptr();
