@@ -129,10 +129,12 @@ class DeviceError(RuntimeError):
 
 
 def require_built() -> None:
-    """Raise ImportError if libdw_moe.so has not been built (without mapping it)."""
-    if not os.path.exists(LIB_PATH):
-        raise ImportError(
-            f"{LIB_PATH} not found: build it with `python __graft_entry__.py` (nvcc, sm_100a)")
+    """Raise ImportError if libdw_moe.so or its binding has not been built
+    (without mapping them)."""
+    for path in (LIB_PATH, os.path.join(_HERE, "_bind.so")):
+        if not os.path.exists(path):
+            raise ImportError(
+                f"{path} not found: build it with `python __graft_entry__.py` (nvcc, sm_100a)")
 
 
 def load():
@@ -157,6 +159,23 @@ def load():
 
 def lib():
     return load()
+
+
+_bind = None
+
+
+def bind():
+    """The native binding (csrc/bind.cpp) of the calls that take torch tensors,
+    wired to libdw_moe.so; raise ImportError if it is absent."""
+    global _bind
+    if _bind is None:
+        load()
+        with _lock:
+            if _bind is None:
+                from . import _bind as mod
+                mod.init(LIB_PATH)
+                _bind = mod
+    return _bind
 
 
 def last_error() -> str:

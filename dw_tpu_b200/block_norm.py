@@ -14,11 +14,10 @@ def pre_norm(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = 
     """The norm before a block: ``norm(x) * weight (+ bias)`` of x [t, h] (bf16
     or f32), ``kind`` "rms" or "layer"; statistics in f32. ``out`` (which may
     be ``x``) is written and returned if given. Inference only: no gradient."""
-    ops.no_grad_needed(x, weight, bias)
-    if out is None:
-        out = torch.empty(x.shape, dtype=out_dtype, device=x.device)
-    ops.block_norm_out(x, out, weight=weight, bias=bias, eps=eps, kind=kind)
-    return out
+    if weight is None:
+        raise ValueError("pre_norm needs a weight")
+    return ops.block_norm_out(x, out, weight=weight, bias=bias, eps=eps, kind=kind,
+                              h_dtype=out_dtype)[1]
 
 
 def post_norm(y: torch.Tensor, residual: torch.Tensor, *,
@@ -39,15 +38,9 @@ def post_norm(y: torch.Tensor, residual: torch.Tensor, *,
     [h], or an element [t, h]. h is formed from the f32 r. ``residual_out`` may be
     ``residual`` (the stream updated in place) and ``out`` may be ``y``.
     Inference only: no gradient."""
-    ops.no_grad_needed(y, residual, norm_weight, norm_bias, gate, next_weight, next_bias)
-    if residual_out is None:
-        residual_out = torch.empty(residual.shape, dtype=residual.dtype, device=residual.device)
-    if next_weight is None:
-        if out is not None or next_bias is not None:
-            raise ValueError("out and next_bias need next_weight")
-    elif out is None:
-        out = torch.empty(residual.shape, dtype=out_dtype, device=residual.device)
-    ops.block_norm_out(residual, out, weight=next_weight, bias=next_bias, y=y,
-                       r_out=residual_out, norm_weight=norm_weight, norm_bias=norm_bias,
-                       gate=gate, scale=scale, residual_scale=residual_scale, eps=eps, kind=kind)
-    return residual_out, out
+    if next_weight is None and (out is not None or next_bias is not None):
+        raise ValueError("out and next_bias need next_weight")
+    return ops.block_norm_out(residual, out, weight=next_weight, bias=next_bias, y=y,
+                              r_out=residual_out, norm_weight=norm_weight, norm_bias=norm_bias,
+                              gate=gate, scale=scale, residual_scale=residual_scale, eps=eps,
+                              kind=kind, h_dtype=out_dtype)

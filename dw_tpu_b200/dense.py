@@ -29,20 +29,13 @@ def dense_matmul(x: torch.Tensor, w: torch.Tensor, *, bias: torch.Tensor | None 
     bf16 or f32; ``out_dtype`` is bf16 by default. ``out`` (which may be
     ``residual``) is written and returned if given. Inference only: no
     gradient."""
-    if act not in _ACTS:
+    code = _ACTS.get(act, -1)
+    if code < 0:
         raise ValueError(f"act {act!r} not supported (one of {sorted(k for k in _ACTS if k)})")
-    code = _ACTS[act]
     if code == L.ACT_SWIGLU_CLAMP and act_limit is None:
         raise ValueError("swiglu_clamp needs act_limit")
-    ops.no_grad_needed(x, w, bias, residual)
-    if out is None:
-        if x.dim() != 2 or w.dim() != 2:
-            raise ValueError("x and w must be 2-D")
-        n = w.shape[0]
-        if code in (L.ACT_SWIGLU, L.ACT_SWIGLU_CLAMP):
-            n //= 2
-        out = torch.empty((x.shape[0], n), dtype=out_dtype or torch.bfloat16, device=x.device)
-    elif out_dtype is not None and out.dtype != out_dtype:
+    if out is not None and out_dtype is not None and out.dtype != out_dtype:
         raise ValueError(f"out is {out.dtype}, out_dtype {out_dtype}")
     return ops.dense_matmul_out(x, w, out, bias=bias, act=code, act_limit=act_limit or 0.0,
-                                residual=residual, residual_scale=residual_scale)
+                                residual=residual, residual_scale=residual_scale,
+                                out_dtype=out_dtype or torch.bfloat16)

@@ -411,49 +411,16 @@ def e8m0_decode_out(codes, out, stream=None):
 # Around the expert layer: grouped routing, dense products, block norms
 # ----------------------------------------------------------------------------
 
-def _same_device(first, *others):
-    """All given tensors on one CUDA device; returns its index."""
-    dev = first.device
-    if dev.type != "cuda":
-        raise ValueError("dw_tpu_b200 ops take CUDA tensors (no CPU path)")
-    for t in others:
-        if t is not None and t.device != dev:
-            raise ValueError(f"tensors on different devices: {dev} and {t.device}")
-    return dev.index
-
-
-def no_grad_needed(*tensors):
-    """Refuses inputs that autograd would expect a gradient for: these ops are
-    for inference and record none."""
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
-                raise ValueError("inference only: an input requires a gradient (call under "
-                                 "torch.no_grad() or detach it)")
-
-
-def _rows(t, name, shape=None, dtypes=(torch.bfloat16, torch.float32)):
-    """A 2-D tensor with unit stride along its rows; returns its row stride."""
-    if t.dim() != 2 or (shape is not None and t.shape != shape):
-        raise ValueError(f"{name} must be {'2-D' if shape is None else list(shape)}, got "
-                         f"{list(t.shape)}")
-    if t.dtype not in dtypes:
-        raise ValueError(f"{name} dtype {t.dtype} not supported")
-    ld, unit = t.stride()
-    if unit != 1 and t.shape[1] > 1:
-        raise ValueError(f"{name} must have unit stride along its rows")
-    return ld
-
-
-def _vector(t, name, n, dtypes=(torch.bfloat16, torch.float32)):
-    if t.dim() != 1 or t.shape[0] != n or t.dtype not in dtypes:
-        raise ValueError(f"{name} must be a bf16 or f32 vector of {n}, got {list(t.shape)} "
-                         f"{t.dtype}")
-    if n > 1 and t.stride(0) != 1:
-        raise ValueError(f"{name} must be contiguous")
-
-
 _GROUP_SCORES = {"max": L.GROUP_MAX, "top2": L.GROUP_TOP2}
+_NORMS = {"rms": L.NORM_RMS, "layer": L.NORM_LAYER}
+_FLOATS = {torch.bfloat16: L.BF16, torch.float32: L.F32}
+
+
+def _code(table, key, what):
+    try:
+        return table[key]
+    except (KeyError, TypeError):
+        raise ValueError(f"unknown {what} {key!r} (one of {list(table)})") from None
 
 
 def route_grouped_topk_out(logits, top_k, num_groups, topk_groups, ids_out, w32_out=None,
@@ -461,131 +428,51 @@ def route_grouped_topk_out(logits, top_k, num_groups, topk_groups, ids_out, w32_
                            renormalize=True, routed_scale=1.0, bias=None, num_valid_tokens=None,
                            stream=None):
     """Group-limited routing of logits [t, e] (dwm_route_grouped_topk): ids_out
-    int32 [t, top_k], w32_out f32 and / or w16_out bf16 of the same shape."""
-    dev = _same_device(logits, ids_out, w32_out, w16_out, bias)
-    if dev != torch.cuda.current_device():
-        with torch.cuda.device(dev):
-            return route_grouped_topk_out(
-                logits, top_k, num_groups, topk_groups, ids_out, w32_out, w16_out,
-                scoring_fn=scoring_fn, group_score=group_score, renormalize=renormalize,
-                routed_scale=routed_scale, bias=bias, num_valid_tokens=num_valid_tokens,
-                stream=stream)
-    ld = _rows(logits, "logits")
-    t, e = logits.shape
-    if scoring_fn not in _SCORING:
-        raise ValueError(f"unknown scoring_fn {scoring_fn!r}")
-    if group_score not in _GROUP_SCORES:
-        raise ValueError(f"unknown group_score {group_score!r}")
-    for o, dt in ((ids_out, torch.int32), (w32_out, torch.float32), (w16_out, torch.bfloat16)):
-        if o is not None and (o.shape != (t, top_k) or o.dtype != dt or not o.is_contiguous()):
-            raise ValueError(f"outputs must be contiguous [{t}, {top_k}], ids int32, weights "
-                             f"f32 / bf16; got {list(o.shape)} {o.dtype}")
-    if bias is not None:
-        _vector(bias, "bias", e, (torch.float32,))
-    rc = L.lib().dwm_route_grouped_topk(
-        logits.data_ptr(), L.dtype_code(logits.dtype), ld, t, e, int(top_k), int(num_groups),
-        int(topk_groups), _SCORING[scoring_fn], _GROUP_SCORES[group_score],
-        int(bool(renormalize)), float(routed_scale), L.ptr(bias),
-        -1 if num_valid_tokens is None else max(0, int(num_valid_tokens)), ids_out.data_ptr(),
-        L.ptr(w32_out), L.ptr(w16_out), L.stream_ptr() if stream is None else stream)
-    L.check(rc, "route_grouped_topk")
+    int32 [t, top_k], w32_out f32 and / or w16_out bf16 of the same shape.
+    Logits rows may be strided."""
+    if ids_out is None:
+        raise ValueError("ids_out is required")
+    L.bind().route_grouped_topk(
+        logits, top_k, num_groups, topk_groups, _code(_SCORING, scoring_fn, "scoring_fn"),
+        _code(_GROUP_SCORES, group_score, "group_score"), int(bool(renormalize)), routed_scale,
+        bias, -1 if num_valid_tokens is None else max(0, num_valid_tokens), L.F32, ids_out,
+        w32_out, w16_out, stream)
+
+
+def route_grouped_topk_new(logits, top_k, num_groups, topk_groups, dtype, scoring_fn, group_score,
+                           renormalize, routed_scale, bias, num_valid_tokens):
+    """The same into new tensors: (weights of ``dtype``, bf16 or f32, and ids)."""
+    return L.bind().route_grouped_topk(
+        logits, top_k, num_groups, topk_groups, _code(_SCORING, scoring_fn, "scoring_fn"),
+        _code(_GROUP_SCORES, group_score, "group_score"), int(bool(renormalize)), routed_scale,
+        bias, -1 if num_valid_tokens is None else max(0, num_valid_tokens), _FLOATS[dtype], None,
+        None, None, None)
 
 
 def dense_matmul_out(x, w, out, *, bias=None, act=L.ACT_NONE, act_limit=0.0, residual=None,
-                     residual_scale=1.0, stream=None):
+                     residual_scale=1.0, out_dtype=torch.bfloat16, stream=None):
     """out <- residual_scale * residual + act(x w^T + bias) (dwm_dense_matmul):
     x bf16 [m, k], w bf16 [n, k], bias [n], residual and out [m, n] (n / 2 with
-    SwiGLU), bf16 or f32. Rows may be strided; ``out`` may be ``residual``."""
-    dev = _same_device(x, w, out, bias, residual)
-    if dev != torch.cuda.current_device():
-        with torch.cuda.device(dev):
-            return dense_matmul_out(x, w, out, bias=bias, act=act, act_limit=act_limit,
-                                    residual=residual, residual_scale=residual_scale,
-                                    stream=stream)
-    ldx = _rows(x, "x", None, (torch.bfloat16,))
-    ldw = _rows(w, "w", None, (torch.bfloat16,))
-    m, k = x.shape
-    n = w.shape[0]
-    if w.shape[1] != k:
-        raise ValueError(f"x has k={k}, w k={w.shape[1]}")
-    n_out = n // 2 if act in (L.ACT_SWIGLU, L.ACT_SWIGLU_CLAMP) else n
-    ldo = _rows(out, "out", (m, n_out))
-    ldr = 0 if residual is None else _rows(residual, "residual", (m, n_out))
-    if bias is not None:
-        _vector(bias, "bias", n)
-    rc = L.lib().dwm_dense_matmul(
-        x.data_ptr(), ldx, w.data_ptr(), ldw, m, n, k, L.ptr(bias),
-        L.F32 if bias is None else L.dtype_code(bias.dtype), act, float(act_limit),
-        L.ptr(residual), L.F32 if residual is None else L.dtype_code(residual.dtype), ldr,
-        float(residual_scale), out.data_ptr(), L.dtype_code(out.dtype), ldo,
-        L.stream_ptr() if stream is None else stream)
-    L.check(rc, "dense_matmul")
-    return out
-
-
-_NORMS = {"rms": L.NORM_RMS, "layer": L.NORM_LAYER}
+    SwiGLU), bf16 or f32. Rows may be strided; ``out`` may be ``residual``, or
+    None: a new tensor of ``out_dtype``. Returns out."""
+    return L.bind().dense_matmul(x, w, bias, act, act_limit, residual, residual_scale, out,
+                                 _code(_FLOATS, out_dtype, "out_dtype"), stream)
 
 
 def block_norm_out(residual, h_out=None, *, weight=None, bias=None, y=None, r_out=None,
                    norm_weight=None, norm_bias=None, gate=None, scale=1.0, residual_scale=1.0,
-                   eps=1e-6, kind="rms", stream=None):
+                   eps=1e-6, kind="rms", h_dtype=torch.bfloat16, stream=None):
     """r_out <- residual_scale * residual + scale * gate * n2(y) and
     h_out <- n1(r) (dwm_block_norm); without ``y`` only h_out <- n1(residual).
-    n1 has ``weight`` / ``bias``, n2 ``norm_weight`` / ``norm_bias`` (without a
-    weight it is the identity). gate [t, 1], [h] or [t, h] in y's dtype; r_out
-    has residual's dtype. Rows may be strided; an output may be one of the row
-    inputs in place."""
-    dev = _same_device(residual, h_out, weight, bias, y, r_out, norm_weight, norm_bias, gate)
-    if dev != torch.cuda.current_device():
-        with torch.cuda.device(dev):
-            return block_norm_out(residual, h_out, weight=weight, bias=bias, y=y, r_out=r_out,
-                                  norm_weight=norm_weight, norm_bias=norm_bias, gate=gate,
-                                  scale=scale, residual_scale=residual_scale, eps=eps, kind=kind,
-                                  stream=stream)
-    if kind not in _NORMS:
-        raise ValueError(f"unknown norm kind {kind!r}")
-    ldres = _rows(residual, "residual")
-    shape = residual.shape
-    t, h = shape
-    ldy = ldr = ldh = ldg = 0
-    if (y is None) != (r_out is None):
-        raise ValueError("y and r_out go together")
-    if y is not None:
-        ldy = _rows(y, "y", shape)
-        ldr = _rows(r_out, "r_out", shape, (residual.dtype,))
-    if h_out is not None:
-        ldh = _rows(h_out, "h_out", shape)
-    wdt = None
-    for name, v in (("weight", weight), ("bias", bias), ("norm_weight", norm_weight),
-                    ("norm_bias", norm_bias)):
-        if v is not None:
-            _vector(v, name, h)
-            if wdt is not None and v.dtype != wdt:
-                raise ValueError("the norms' weights and biases must share one dtype")
-            wdt = v.dtype
-    if norm_bias is not None and norm_weight is None:
-        raise ValueError("norm_bias needs norm_weight")
-    if (bias is not None or h_out is not None) and (weight is None or h_out is None):
-        raise ValueError("h_out, weight and bias belong together: h_out = norm(r) * weight + bias")
-    mode = L.GATE_NONE
-    if gate is not None:
-        if y is None or gate.dtype != y.dtype:
-            raise ValueError("gate goes with y and has its dtype")
-        if gate.dim() == 1:
-            _vector(gate, "gate", h)
-            mode = L.GATE_CHANNEL
-        else:
-            ldg = _rows(gate, "gate", (t, 1) if gate.shape[-1] == 1 else shape)
-            mode = L.GATE_TOKEN if gate.shape[1] == 1 else L.GATE_FULL
-    rc = L.lib().dwm_block_norm(
-        L.ptr(y), L.BF16 if y is None else L.dtype_code(y.dtype), ldy, residual.data_ptr(),
-        L.dtype_code(residual.dtype), ldres, t, h, _NORMS[kind], float(eps),
-        int(norm_weight is not None), L.ptr(norm_weight), L.ptr(norm_bias), L.ptr(gate), mode, ldg,
-        float(scale), float(residual_scale), L.ptr(weight), L.ptr(bias),
-        L.BF16 if wdt is None else L.dtype_code(wdt), L.ptr(r_out), ldr, L.ptr(h_out),
-        L.BF16 if h_out is None else L.dtype_code(h_out.dtype), ldh,
-        L.stream_ptr() if stream is None else stream)
-    L.check(rc, "block_norm")
+    n1 has ``weight`` / ``bias`` (without a weight there is no h_out), n2
+    ``norm_weight`` / ``norm_bias`` (without a weight it is the identity). gate
+    [t, 1], [h] or [t, h] in y's dtype; r_out has residual's dtype. Rows may be
+    strided; an output may be one of the row inputs in place, or None: a new
+    tensor (h_out of ``h_dtype``). Returns (r_out, h_out)."""
+    return L.bind().block_norm(
+        residual, y, norm_weight, norm_bias, gate, scale, residual_scale, weight, bias, eps,
+        _code(_NORMS, kind, "norm kind"), r_out, h_out, _code(_FLOATS, h_dtype, "out_dtype"),
+        weight is not None, stream)
 
 
 # ----------------------------------------------------------------------------

@@ -50,19 +50,13 @@ def route_grouped_topk(gating_output: torch.Tensor, top_k: int, num_groups: int,
     logits = gating_output
     if logits.dtype not in (torch.bfloat16, torch.float32):
         logits = logits.float()
-    ops.no_grad_needed(logits, bias)
-    t = logits.shape[0]
-    ids = torch.empty((t, top_k), dtype=torch.int32, device=logits.device)
-    narrow = dtype == torch.bfloat16
-    w = torch.empty((t, top_k), dtype=torch.bfloat16 if narrow else torch.float32,
-                    device=logits.device)
-    ops.route_grouped_topk_out(logits, top_k, num_groups, topk_groups, ids,
-                               None if narrow else w, w if narrow else None,
-                               scoring_fn=scoring_fn, group_score=group_score,
-                               renormalize=renormalize, routed_scale=routed_scale,
-                               bias=None if bias is None else bias.float().contiguous(),
-                               num_valid_tokens=num_valid_tokens)
-    return w.to(dtype), ids
+    if bias is not None and (bias.dtype != torch.float32 or not bias.is_contiguous()):
+        bias = bias.float().contiguous()
+    w, ids = ops.route_grouped_topk_new(
+        logits, top_k, num_groups, topk_groups,
+        torch.bfloat16 if dtype == torch.bfloat16 else torch.float32, scoring_fn, group_score,
+        renormalize, routed_scale, bias, num_valid_tokens)
+    return (w if w.dtype == dtype else w.to(dtype)), ids
 
 
 def route_hash(gating_output: torch.Tensor, hash_ids: torch.Tensor, renormalize: bool = True,
