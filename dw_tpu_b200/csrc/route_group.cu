@@ -8,13 +8,22 @@
 // the way they are computed. Without a bias the experts are ordered by their
 // logits, which every scoring function preserves.
 //
-// One warp per token; lane l holds experts l, l + 32, ...
+// A token takes 8, 16 or 32 lanes of a warp: each lane holds a run of at most 64
+// experts of one group in registers, so that the scan for the largest is the
+// same few instructions for the experts of 4, 2 or 1 tokens. The lanes work in
+// f32 and note how far apart the values are where a choice was made. Where two
+// are closer than the f32 error (a few tokens in a hundred for random logits),
+// the groups or the picks in question are compared in 64 bits; a token that
+// this does not settle is done again in 64 bits by the whole warp (8-12 us, which
+// one token of 1024 would make the time of all). Bound: instruction issue.
+#include <algorithm>
+
 #include "common.cuh"
 
 namespace dwm {
 namespace route_group {
 
-constexpr int WARPS = 4;
+constexpr int WARPS = 2;
 
 struct Args {
   const void* logits;
@@ -22,6 +31,9 @@ struct Args {
   const float* bias;
   int t, e, top_k, groups, keep, per;
   int scoring, top2, renorm, num_valid;
+  // 2^lpt_log lanes a token, 2^lg_log lanes a group, run experts a lane; vec:
+  // every run starts on 16 bytes and is a whole number of 16-byte loads.
+  int lpt_log, lg_log, run, vec;
   float scale;
   int32_t* ids;
   float* w32;
@@ -68,11 +80,15 @@ __device__ __forceinline__ void warp_best(uint64_t& key, int& idx) {
   }
 }
 
+struct Pick {
+  int id;
+  float weight;
+};
+
 // Row `tok` in 64 bits: lane j < top_k returns the j-th expert and weight.
 // buf: e keys of this warp's shared memory.
 template <int LD>
-__device__ void route_row64(const Args& a, int64_t tok, uint64_t* buf, int lane, int& id,
-                            float& weight) {
+__device__ __noinline__ Pick route_row64(const Args& a, int64_t tok, uint64_t* buf, int lane) {
   const int64_t row = tok * a.ld;
   double mx = -INFINITY, sum = 0.0;
   if (a.scoring == DWM_SCORE_SOFTMAX) {
@@ -125,7 +141,7 @@ __device__ void route_row64(const Args& a, int64_t tok, uint64_t* buf, int lane,
   __syncwarp();
 
   double s = 0.0;
-  id = 0;
+  int id = 0;
   for (int k = 0; k < a.top_k; ++k) {
     uint64_t bk = 0;
     int bi = 0x7fffffff;
@@ -144,24 +160,425 @@ __device__ void route_row64(const Args& a, int64_t tok, uint64_t* buf, int lane,
     for (int k = 0; k < a.top_k; ++k) total += __shfl_sync(0xffffffffu, s, k);
     s = total == 0.0 ? 0.0 : s / total;
   }
-  weight = (float)(s * (double)a.scale);
+  return {id, (float)(s * (double)a.scale)};
+}
+
+// 32-bit keys of numbers (not NaN), ordered as the 64-bit ones.
+__device__ __forceinline__ uint32_t key32(float v) {
+  const int b = __float_as_int(v + 0.0f);
+  return (uint32_t)b ^ ((uint32_t)(b >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float value32(uint32_t key) {
+  return __uint_as_float(key >> 31 ? key ^ 0x80000000u : ~key);
+}
+
+// The f32 score, for the weights (FULL) to a few steps of itself. For the order
+// it and its sum with a bias are off by less than MARGIN / 2 of the largest
+// |score| + |bias|: expf and division by a few steps (2^-24 each), the exponent's
+// own rounding by 2^-24 |x| where the score's slope is at most 1 / (4 |x|), and
+// for softmax the sum over the experts by 2^-21.
+constexpr float MARGIN = 1e-6f;
+template <bool FULL>
+__device__ __forceinline__ float score32(float x, int scoring, float mx, float inv_sum) {
+  // (mx is 0 where every logit is -inf.)
+  if (scoring == DWM_SCORE_SOFTMAX) return expf(x == mx ? 0.0f : x - mx) * inv_sum;
+  if (scoring == DWM_SCORE_SIGMOID)
+    return FULL ? 1.0f / (1.0f + expf(-x)) : sigmoid_fast(x);
+  return sqrtf(fmaxf(x, 0.0f) + log1pf(expf(-fabsf(x))));
+}
+
+// Within a lane the keys are made unique: their low bits, as many as KPL places
+// take, are the place in the run, the lowest place the largest. That takes up
+// to 2^bits steps off the value.
+template <int KPL>
+struct Packed {
+  static constexpr uint32_t PLACES = KPL <= 32 ? 31 : 63;
+  // The difference of two values that packing may hide, of the larger.
+  static constexpr float HIDDEN = (KPL <= 32 ? 2.0f : 4.0f) / 262144.0f;
+  static __device__ __forceinline__ float value(uint32_t key) {
+    return value32(key >> 31 ? key & ~PLACES : key | PLACES);
+  }
+};
+constexpr int DEEP = 6;  // a lane's largest that are kept sorted
+
+// Sum or maximum over a token's lanes.
+__device__ __forceinline__ float seg_sum(float v, int lpt) {
+  for (int o = lpt / 2; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+template <class T>
+__device__ __forceinline__ T seg_max(T v, int lpt) {
+  for (int o = lpt / 2; o; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+
+// The largest of the keys (below `limit`, if BELOW), descending (0: no more).
+template <bool BELOW, int KPL>
+__device__ __forceinline__ void largest(const uint32_t (&key)[KPL], uint32_t limit,
+                                        uint32_t (&l)[DEEP]) {
+#pragma unroll
+  for (int j = 0; j < DEEP; ++j) l[j] = 0;
+#pragma unroll
+  for (int i = 0; i < KPL; ++i) {
+    uint32_t k = !BELOW || key[i] < limit ? key[i] : 0u;
+#pragma unroll
+    for (int j = 0; j < DEEP && j <= i; ++j) {
+      const uint32_t t = min(l[j], k);
+      l[j] = max(l[j], k);
+      k = t;
+    }
+  }
+}
+
+// KPL: places in a lane's run; WHOLE: every group's lanes use them all.
+template <int LD, int KPL, bool WHOLE>
+__global__ void __launch_bounds__(32 * WARPS) route_grouped_kernel(const Args a) {
+  using P = Packed<KPL>;
+  constexpr uint32_t PLACES = P::PLACES;
+  extern __shared__ uint64_t smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint64_t* buf = smem + warp * a.e;
+  const int lpt = 1 << a.lpt_log, sl = lane & (lpt - 1), seg = lane & ~(lpt - 1);
+  const uint32_t seg_mask = (lpt == 32 ? 0xFFFFFFFFu : (1u << lpt) - 1u) << seg;
+  const int g = sl >> a.lg_log, part = sl & ((1 << a.lg_log) - 1);
+  const bool in_group = g < a.groups;
+  // This lane's experts: places [0, count) from expert `first`.
+  const int start = part * a.run;
+  const int count = in_group ? max(0, min(a.run, a.per - start)) : 0;
+  const int first = count > 0 ? g * a.per + start : 0;
+  auto has = [&](int i) { return WHOLE ? true : i < count; };
+  const bool biased = a.bias != nullptr;
+  const int tpw = 32 >> a.lpt_log;  // tokens a warp
+  const int64_t stride = (int64_t)gridDim.x * WARPS * tpw;
+  for (int64_t base = ((int64_t)blockIdx.x * WARPS + warp) * tpw; base < a.t; base += stride) {
+    const int64_t tok = base + (lane >> a.lpt_log);
+    const bool live = tok < a.t;
+    const bool real = live && (a.num_valid < 0 || tok < a.num_valid);
+    const int64_t row = (live ? tok : base) * a.ld;
+
+    float v[KPL];
+    if (a.vec) {
+      // (count is a.run or 0, a multiple of a 16-byte load.)
+      constexpr int PER = LD == DWM_BF16 ? 8 : 4;
+#pragma unroll
+      for (int i = 0; i < KPL; i += PER) {
+        const int64_t at = row + first + (has(i) ? i : 0);
+        if constexpr (LD == DWM_BF16) {
+          const uint4 q = *reinterpret_cast<const uint4*>(
+              static_cast<const uint16_t*>(a.logits) + at);
+          const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (i + j < KPL)
+              v[i + j] = __uint_as_float(j & 1 ? w[j / 2] & 0xFFFF0000u : w[j / 2] << 16);
+        } else {
+          const float4 q =
+              *reinterpret_cast<const float4*>(static_cast<const float*>(a.logits) + at);
+          const float w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (i + j < KPL) v[i + j] = w[j];
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < KPL; ++i)
+        v[i] = load_logit<LD>(a.logits, row + first + (has(i) ? i : 0));
+    }
+
+    bool nan = false;
+    float mx = 0.0f, inv_sum = 1.0f;
+    if (a.scoring == DWM_SCORE_SOFTMAX) {
+      mx = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < KPL; ++i) mx = fmaxf(mx, v[i]);  // (an absent one repeats the first)
+      mx = seg_max(count > 0 ? mx : -INFINITY, lpt);
+      if (mx == -INFINITY) mx = 0.0f;
+      if (biased || !a.renorm) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < KPL; ++i) {
+          const float s = score32<true>(v[i], DWM_SCORE_SOFTMAX, mx, 1.0f);
+          if (has(i)) sum += s;
+        }
+        sum = seg_sum(count > 0 ? sum : 0.0f, lpt);
+        inv_sum = sum > 0.0f ? 1.0f / sum : 1.0f;
+      }
+    }
+    float size = 0.0f;  // the largest |score| + |bias|
+    if (biased) {
+      auto choices = [&](int scoring) {
+#pragma unroll
+        for (int i = 0; i < KPL; ++i) {
+          const float s = score32<false>(v[i], scoring, mx, inv_sum);
+          const float b = a.bias[first + (has(i) ? i : 0)];
+          size = fmaxf(size, fabsf(s) + (fabsf(b) < INFINITY ? fabsf(b) : 0.0f));
+          v[i] = s + b;
+        }
+      };
+      if (a.scoring == DWM_SCORE_SOFTMAX)
+        choices(DWM_SCORE_SOFTMAX);
+      else if (a.scoring == DWM_SCORE_SIGMOID)
+        choices(DWM_SCORE_SIGMOID);
+      else
+        choices(DWM_SCORE_SQRTSOFTPLUS);
+      size = seg_max(size, lpt);
+    }
+    uint32_t key[KPL];
+#pragma unroll
+    for (int i = 0; i < KPL; ++i) {
+      nan |= isnan(v[i]);
+      const uint32_t k = (key32(v[i]) & ~PLACES) | (PLACES - (uint32_t)i);
+      key[i] = has(i) ? k : 0u;
+    }
+    bool unsure = nan;  // not decided in f32
+    uint32_t l[DEEP];
+    largest<false>(key, 0u, l);
+    auto expert = [&](uint32_t k) { return first + (int)(PLACES - (k & PLACES)); };
+
+    // bf16 logits without a bias fit the keys whole; otherwise the values are
+    // formed again where the keys are too coarse.
+    const bool exact = LD == DWM_BF16 && !biased;
+    auto choice = [&](int e) {
+      const float x = load_logit<LD>(a.logits, row + e);
+      return biased ? score32<false>(x, a.scoring, mx, inv_sum) + a.bias[e] : x;
+    };
+    auto choice64 = [&](int e) {
+      const double x = load_logit<LD>(a.logits, row + e);
+      return biased ? score(x, a.scoring, 0.0, 1.0) + (double)a.bias[e] : x;
+    };
+    // What the values of a lane's packed keys up to k are below, in 64 bits.
+    auto bound = [&](uint32_t k) {
+      const double x = P::value(k & ~PLACES);
+      return x + (biased ? (double)(2.0f * MARGIN + P::HIDDEN) * size
+                         : (double)P::HIDDEN * fabs(x));
+    };
+    auto value = [&](uint32_t k) { return exact ? P::value(k & ~PLACES) : choice(expert(k)); };
+    uint32_t m1 = count > 0 ? key32(value(l[0])) : 0u;
+    uint32_t m2 = a.top2 && count > 0 && l[1] ? key32(value(l[1])) : 0u;
+    for (int o = (1 << a.lg_log) / 2; o; o >>= 1) {
+      const uint32_t n1 = __shfl_xor_sync(0xffffffffu, m1, o),
+                     n2 = __shfl_xor_sync(0xffffffffu, m2, o);
+      m2 = max(min(m1, n1), max(m2, n2));
+      m1 = max(m1, n1);
+    }
+    uint32_t gkey = m1;
+    if (a.top2 && m2) {
+      float p = value32(m1), q = value32(m2);
+      if (!biased) {
+        p = score32<true>(p, a.scoring, mx, 1.0f);
+        q = score32<true>(q, a.scoring, mx, 1.0f);
+      }
+      gkey = key32(p + q);
+      unsure |= isnan(p + q);
+    }
+    int rank = 0;
+    for (int q = 0; q < a.groups; ++q) {
+      const uint32_t k = __shfl_sync(0xffffffffu, gkey, seg + (q << a.lg_log));
+      rank += k > gkey || (k == gkey && q < g);
+    }
+    bool open = in_group && rank < a.keep;
+    // In 64 bits a softmax's sum takes every expert; without a bias the order
+    // does not need it.
+    const bool settles = !(biased && a.scoring == DWM_SCORE_SOFTMAX);
+    if (a.keep < a.groups && (biased || a.top2)) {
+      const float in = value32(~seg_max(open ? ~gkey : 0u, lpt));  // the least of the open
+      const float out = value32(seg_max(in_group && !open ? gkey : 0u, lpt));
+      // (Without a bias a sum of two scores is off relative to itself, unless it
+      // is next to the f32 underflow.)
+      const bool close = biased ? !(in - out > 2.0f * MARGIN * size)
+                                : !(in > 1e-30f && in - out > 16.0f * MARGIN * in);
+      if (__any_sync(0xffffffffu, close && real)) {
+        // The groups' values in 64 bits, from each lane's first four.
+        double c[4], d1 = -INFINITY, d2 = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          c[j] = l[j] ? choice64(expert(l[j])) : -INFINITY;
+          d2 = fmax(d2, fmin(d1, c[j]));
+          d1 = fmax(d1, c[j]);
+        }
+        // A fifth that may be one of the two largest: not settled.
+        bool sure = settles && (!l[4] || (a.top2 ? d2 : d1) > bound(l[4]));
+        for (int o = (1 << a.lg_log) / 2; o; o >>= 1) {
+          const double n1 = __shfl_xor_sync(0xffffffffu, d1, o),
+                       n2 = __shfl_xor_sync(0xffffffffu, d2, o);
+          d2 = fmax(fmin(d1, n1), fmax(d2, n2));
+          d1 = fmax(d1, n1);
+        }
+        double gv = d1;
+        if (a.top2 && a.per > 1)
+          gv = biased ? d1 + d2
+                      : score(d1, a.scoring, (double)mx, 1.0) + score(d2, a.scoring, (double)mx, 1.0);
+        rank = 0;
+        for (int q = 0; q < a.groups; ++q) {
+          const double k = __shfl_sync(0xffffffffu, gv, seg + (q << a.lg_log));
+          rank += k > gv || (k == gv && q < g);
+        }
+        if (close) {
+          open = in_group && rank < a.keep;
+          unsure |= !sure;
+        }
+      }
+    }
+
+    // The top k, the largest of the lanes' largest each time.
+    if (!open || count == 0) l[0] = 0;
+    int left = open ? count : 0;  // in l or below it
+    const int n_open = a.keep * a.per;
+    uint32_t top = 0;  // the last pick's packed value
+    int last_id = 0, slot_id[4] = {0, 0, 0, 0};
+    auto pick = [&](int k) {
+      top = seg_max(l[0] & ~PLACES, lpt);
+      // Of equal ones the lowest lane's, whose experts come first.
+      const uint32_t who = __ballot_sync(0xffffffffu, (l[0] & ~PLACES) == top) & seg_mask;
+      const int winner = __ffs(who) - 1;
+      last_id = __shfl_sync(0xffffffffu, expert(l[0]), winner);
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+        if (k == s * lpt + sl) slot_id[s] = last_id;
+      uint32_t taken = 0;
+      if (lane == winner) {
+        taken = l[0];
+#pragma unroll
+        for (int j = 0; j + 1 < DEEP; ++j) l[j] = l[j + 1];
+        l[DEEP - 1] = 0;
+        --left;
+      }
+      // More than DEEP of one lane: the next ones from its keys.
+      const bool empty = taken && !l[0] && left > 0;
+      if (__any_sync(0xffffffffu, empty)) {
+        if (empty) largest<true>(key, taken, l);
+      }
+    };
+    const int rounds = a.top_k + (!exact && a.top_k < n_open);
+    bool close = false;
+    float last = 0.0f;
+    for (int k = 0; k < rounds; ++k) {
+      const int before = last_id;
+      pick(k);
+      if (!exact) {
+        const float x = P::value(top);
+        const float far = biased ? (2.0f * MARGIN + P::HIDDEN) * size
+                                 : P::HIDDEN * fmaxf(fabsf(x), fabsf(last));
+        if (k > 0 && !(last - x > far)) {
+          const float p = choice(before), q = choice(last_id);
+          bool sure = biased ? p - q > 2.0f * MARGIN * size : p > q;
+          // Equal logits and biases are a tie in 64 bits too.
+          if (!sure)
+            sure = load_logit<LD>(a.logits, row + before) ==
+                       load_logit<LD>(a.logits, row + last_id) &&
+                   (!biased || a.bias[before] == a.bias[last_id]);
+          close |= !sure;
+        }
+        last = x;
+      }
+    }
+    if (__any_sync(0xffffffffu, close && real)) {
+      // Up to three picks more, then all of them in the order of their 64-bit
+      // values; what was not picked has to be below the last that is chosen.
+      const int all = min(min(a.top_k + 4, n_open), 4 * lpt);
+      for (int k = rounds; k < all; ++k) pick(k);
+      double c[4];
+      int place[4] = {0, 0, 0, 0}, id[4];
+#pragma unroll
+      for (int s = 0; s < 4; ++s) c[s] = s * lpt + sl < all ? choice64(slot_id[s]) : 0.0;
+      double least = 0.0;  // the value at the place top_k - 1
+      for (int k = 0; k < all; ++k) {
+        const int of = seg + (k & (lpt - 1)), s = k >> a.lpt_log;
+        const double v =
+            __shfl_sync(0xffffffffu, s == 0 ? c[0] : s == 1 ? c[1] : s == 2 ? c[2] : c[3], of);
+        const int e = __shfl_sync(
+            0xffffffffu,
+            s == 0 ? slot_id[0] : s == 1 ? slot_id[1] : s == 2 ? slot_id[2] : slot_id[3], of);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) place[j] += v > c[j] || (v == c[j] && e < slot_id[j]);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) id[j] = slot_id[j];
+      for (int k = 0; k < all; ++k) {
+        const int of = seg + (k & (lpt - 1)), s = k >> a.lpt_log;
+        const int to = __shfl_sync(
+            0xffffffffu, s == 0 ? place[0] : s == 1 ? place[1] : s == 2 ? place[2] : place[3], of);
+        const int e = __shfl_sync(
+            0xffffffffu,
+            s == 0 ? slot_id[0] : s == 1 ? slot_id[1] : s == 2 ? slot_id[2] : slot_id[3], of);
+        const double v =
+            __shfl_sync(0xffffffffu, s == 0 ? c[0] : s == 1 ? c[1] : s == 2 ? c[2] : c[3], of);
+        if (to == a.top_k - 1) least = v;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (to == j * lpt + sl) id[j] = e;
+      }
+      if (close) {
+        unsure |= !settles || (all < n_open && !(least > bound(top)));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) slot_id[j] = id[j];
+      }
+    }
+
+    // Weights: slot s of lane sl is the pick s * lpt + sl.
+    float w[4], total = 0.0f;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      w[s] = 0.0f;
+      if (s * lpt + sl < a.top_k)
+        w[s] = score32<true>(load_logit<LD>(a.logits, row + slot_id[s]), a.scoring, mx, inv_sum);
+      total += w[s];
+    }
+    if (a.renorm) total = seg_sum(total, lpt);
+    // What one lane of a token is unsure of, all are.
+    const uint32_t doubts = __ballot_sync(0xffffffffu, unsure && real && in_group);
+    if (live && !(doubts & seg_mask)) {
+      const float scale = !a.renorm ? a.scale : total == 0.0f ? 0.0f : a.scale;
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        const int k = s * lpt + sl;
+        if (k < a.top_k) {
+          const float x = (a.renorm && total != 0.0f ? w[s] / total : w[s]) * scale;
+          const int64_t at = tok * a.top_k + k;
+          a.ids[at] = real ? slot_id[s] : 0;
+          if (a.w32) a.w32[at] = real ? x : 0.0f;
+          if (a.w16) a.w16[at] = real ? (uint16_t)f32_to_bf16_bits(x) : (uint16_t)0;
+        }
+      }
+    }
+    for (uint32_t again = doubts; again;) {
+      const int of = (__ffs(again) - 1) >> a.lpt_log;
+      again &= ~((lpt == 32 ? 0xFFFFFFFFu : (1u << lpt) - 1u) << (of << a.lpt_log));
+      const Pick p = route_row64<LD>(a, base + of, buf, lane);
+      if (lane < a.top_k) {
+        const int64_t at = (base + of) * a.top_k + lane;
+        a.ids[at] = p.id;
+        if (a.w32) a.w32[at] = p.weight;
+        if (a.w16) a.w16[at] = (uint16_t)f32_to_bf16_bits(p.weight);
+      }
+      __syncwarp();
+    }
+  }
+}
+
+template <int LD, int KPL>
+int launch(const Args& a, cudaStream_t s) {
+  const int64_t tokens = (int64_t)WARPS * (32 >> a.lpt_log);  // a CTA's
+  const unsigned grid =
+      (unsigned)std::min<int64_t>((a.t + tokens - 1) / tokens, (int64_t)num_sms() * 64);
+  const size_t smem = (size_t)WARPS * a.e * sizeof(uint64_t);  // at most 32 KB
+  if (a.run == KPL && a.per % a.run == 0)
+    route_grouped_kernel<LD, KPL, true><<<grid, 32 * WARPS, smem, s>>>(a);
+  else
+    route_grouped_kernel<LD, KPL, false><<<grid, 32 * WARPS, smem, s>>>(a);
+  return check_cuda(cudaGetLastError(), "route_grouped_topk launch");
 }
 
 template <int LD>
-__global__ void __launch_bounds__(32 * WARPS) route_grouped_kernel(const Args a) {
-  extern __shared__ uint64_t keys[];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t tok = (int64_t)blockIdx.x * WARPS + warp;
-  if (tok >= a.t) return;
-  int id = 0;
-  float w = 0.0f;
-  if (a.num_valid < 0 || tok < a.num_valid)
-    route_row64<LD>(a, tok, keys + warp * a.e, lane, id, w);
-  if (lane < a.top_k) {
-    a.ids[tok * a.top_k + lane] = id;
-    if (a.w32) a.w32[tok * a.top_k + lane] = w;
-    if (a.w16) a.w16[tok * a.top_k + lane] = (uint16_t)f32_to_bf16_bits(w);
-  }
+int run(const Args& a, cudaStream_t s) {
+  if (a.run <= 4) return launch<LD, 4>(a, s);
+  if (a.run <= 8) return launch<LD, 8>(a, s);
+  if (a.run <= 16) return launch<LD, 16>(a, s);
+  if (a.run <= 20) return launch<LD, 20>(a, s);
+  if (a.run <= 24) return launch<LD, 24>(a, s);
+  if (a.run <= 32) return launch<LD, 32>(a, s);
+  return launch<LD, 64>(a, s);
 }
 
 }  // namespace route_group
@@ -212,12 +629,20 @@ extern "C" int dwm_route_grouped_topk(const void* logits, int logits_dtype, int6
   a.ids = topk_ids;
   a.w32 = topk_weights_f32;
   a.w16 = static_cast<uint16_t*>(topk_weights_bf16);
+  // Lanes: a power of two of groups, each of as many lanes as leave at most 32
+  // experts a lane (64 where the warp has no more lanes), 8 a token at least.
+  int groups_log = 0;
+  while ((1 << groups_log) < num_groups) ++groups_log;
+  a.lg_log = 0;
+  while (groups_log + a.lg_log < 5 &&
+         ((a.per + (1 << a.lg_log) - 1) >> a.lg_log > 32 || groups_log + a.lg_log < 3))
+    ++a.lg_log;
+  a.lpt_log = groups_log + a.lg_log;
+  a.run = (a.per + (1 << a.lg_log) - 1) >> a.lg_log;
+  const int es = logits_dtype == DWM_F32 ? 4 : 2;
+  a.vec = a.per % a.run == 0 && a.run * es % 16 == 0 && (t == 1 || ld_logits * es % 16 == 0) &&
+          (reinterpret_cast<uintptr_t>(logits) & 15) == 0;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const unsigned grid = (unsigned)((t + route_group::WARPS - 1) / route_group::WARPS);
-  const size_t smem = (size_t)route_group::WARPS * e * sizeof(uint64_t);  // at most 32 KB
-  if (logits_dtype == DWM_BF16)
-    route_group::route_grouped_kernel<DWM_BF16><<<grid, 32 * route_group::WARPS, smem, s>>>(a);
-  else
-    route_group::route_grouped_kernel<DWM_F32><<<grid, 32 * route_group::WARPS, smem, s>>>(a);
-  return check_cuda(cudaGetLastError(), "route_grouped_topk launch");
+  return logits_dtype == DWM_BF16 ? route_group::run<DWM_BF16>(a, s)
+                                  : route_group::run<DWM_F32>(a, s);
 }
