@@ -349,6 +349,8 @@ __global__ void __launch_bounds__(THREADS, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  overlap_wait();
+  overlap_next();
 
   if (warp == 0) {
     if (lane == 0) {
@@ -567,20 +569,10 @@ int launch_split(const void* x, int64_t ldx, const void* w, int64_t ldw, int n, 
   rc = set_smem_limit(reinterpret_cast<const void*>(dense_split_kernel<BT, EPI>), L::ALLOC,
                       "dense smem attribute");
   if (rc) return rc;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)split;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)split, (unsigned)((a.n_out + FEAT - 1) / FEAT),
-                     (unsigned)((a.m + BT - 1) / BT));
-  cfg.blockDim = dim3(THREADS);
-  cfg.dynamicSmemBytes = L::ALLOC;
-  cfg.stream = stream;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return check_cuda(cudaLaunchKernelEx(&cfg, dense_split_kernel<BT, EPI>, tm_w, tm_x, a),
+  return check_cuda(overlap_launch(dense_split_kernel<BT, EPI>,
+                                   dim3((unsigned)split, (unsigned)((a.n_out + FEAT - 1) / FEAT),
+                                        (unsigned)((a.m + BT - 1) / BT)),
+                                   dim3(THREADS), L::ALLOC, split, stream, tm_w, tm_x, a),
                     "dense_matmul launch");
 }
 
@@ -672,6 +664,8 @@ __global__ void __launch_bounds__(THREADS, 1)
   cluster_sync();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  overlap_wait();
+  overlap_next();
   const uint32_t full_0 = mapa_shared(full, 0);
   const uint32_t acc_empty_0 = mapa_shared(acc_empty, 0);
 
@@ -863,19 +857,10 @@ int launch(const void* x, int64_t ldx, const void* w, int64_t ldw, int n, const 
   rc = set_smem_limit(reinterpret_cast<const void*>(dense_pair_kernel<EPI, VEC>), ALLOC,
                       "dense pair smem attribute");
   if (rc) return rc;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = 2;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.blockDim = dim3(THREADS);
-  cfg.dynamicSmemBytes = ALLOC;
-  cfg.stream = stream;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  cfg.gridDim = dim3(2 * (unsigned)std::min<int64_t>(tiles, resident_clusters(2)));
-  return check_cuda(cudaLaunchKernelEx(&cfg, dense_pair_kernel<EPI, VEC>, tm_x, tm_w, a),
+  return check_cuda(
+      overlap_launch(dense_pair_kernel<EPI, VEC>,
+                     dim3(2 * (unsigned)std::min<int64_t>(tiles, resident_clusters(2))),
+                     dim3(THREADS), ALLOC, 2, stream, tm_x, tm_w, a),
                     "dense_matmul launch");
 }
 

@@ -347,6 +347,8 @@ __global__ void __launch_bounds__(max_threads<VEC, CPT>(false)) block_norm_kerne
   __shared__ __align__(16) float part[4][32];
   const Group g{(int)threadIdx.x, (int)blockDim.x, 0, part};
   const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+  overlap_wait();
+  overlap_next();
   if (row >= a.t) return;  // a whole warp of a CTA with a warp a row
   int col[CPT];
   bool in[CPT];
@@ -433,6 +435,8 @@ __global__ void __launch_bounds__(max_threads<VEC, CPT>(true), 1)
   }
   g.clear_parts();
   __syncthreads();
+  overlap_wait();
+  overlap_next();
   int col[CPT];
   bool in[CPT];
   columns<VEC, CPT>(a, g, col, in);
@@ -560,16 +564,19 @@ int launch(Args a, cudaStream_t s) {
       const int rc = set_smem_limit(reinterpret_cast<const void*>(fn), budget, "norm smem attribute");
       if (rc) return rc;
       a.status = status_ptr();
-      fn<<<(unsigned)num_sms(), dim3((unsigned)threads, (unsigned)groups),
-           (size_t)5 * a.vec_bytes + (size_t)groups * a.stages * a.stage_bytes, s>>>(a);
-      return check_cuda(cudaGetLastError(), "block_norm launch");
+      return check_cuda(
+          overlap_launch(fn, dim3((unsigned)num_sms()), dim3((unsigned)threads, (unsigned)groups),
+                         (size_t)5 * a.vec_bytes + (size_t)groups * a.stages * a.stage_bytes, 1, s,
+                         a),
+          "block_norm launch");
     }
   }
   // A warp a row, four a CTA, or a CTA a row.
   const int rows = threads == 32 ? 4 : 1;
-  block_norm_kernel<VEC, CPT, YD, RD, WD>
-      <<<(unsigned)((a.t + rows - 1) / rows), dim3((unsigned)threads, (unsigned)rows), 0, s>>>(a);
-  return check_cuda(cudaGetLastError(), "block_norm launch");
+  return check_cuda(overlap_launch(block_norm_kernel<VEC, CPT, YD, RD, WD>,
+                                   dim3((unsigned)((a.t + rows - 1) / rows)),
+                                   dim3((unsigned)threads, (unsigned)rows), 0, 1, s, a),
+                    "block_norm launch");
 }
 
 template <int VEC, int YD, int RD, int WD>

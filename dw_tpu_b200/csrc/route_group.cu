@@ -250,6 +250,8 @@ __global__ void __launch_bounds__(32 * WARPS) route_grouped_kernel(const Args a)
   const bool biased = a.bias != nullptr;
   const int tpw = 32 >> a.lpt_log;  // tokens a warp
   const int64_t stride = (int64_t)gridDim.x * WARPS * tpw;
+  overlap_wait();
+  overlap_next();
   for (int64_t base = ((int64_t)blockIdx.x * WARPS + warp) * tpw; base < a.t; base += stride) {
     const int64_t tok = base + (lane >> a.lpt_log);
     const bool live = tok < a.t;
@@ -563,11 +565,10 @@ int launch(const Args& a, cudaStream_t s) {
   const unsigned grid =
       (unsigned)std::min<int64_t>((a.t + tokens - 1) / tokens, (int64_t)num_sms() * 64);
   const size_t smem = (size_t)WARPS * a.e * sizeof(uint64_t);  // at most 32 KB
-  if (a.run == KPL && a.per % a.run == 0)
-    route_grouped_kernel<LD, KPL, true><<<grid, 32 * WARPS, smem, s>>>(a);
-  else
-    route_grouped_kernel<LD, KPL, false><<<grid, 32 * WARPS, smem, s>>>(a);
-  return check_cuda(cudaGetLastError(), "route_grouped_topk launch");
+  auto fn = a.run == KPL && a.per % a.run == 0 ? route_grouped_kernel<LD, KPL, true>
+                                               : route_grouped_kernel<LD, KPL, false>;
+  return check_cuda(overlap_launch(fn, dim3(grid), dim3(32 * WARPS), smem, 1, s, a),
+                    "route_grouped_topk launch");
 }
 
 template <int LD>
