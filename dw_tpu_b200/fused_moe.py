@@ -117,10 +117,23 @@ class MoELayer:
         t = hidden.shape[0]
         if t > self.max_tokens:
             raise ValueError(f"{t} tokens exceed max_tokens={self.max_tokens}")
-        rows = t * self.top_k
         ids, w16 = self.ids[:t], self.w16[:t]
         ops.route_topk_out(logits, self.top_k, ids, w16_out=w16, scoring_fn=self.scoring_fn,
                            renormalize=self.renormalize)
+        if out is None:
+            out = torch.empty((t, self.w.hidden_size), dtype=torch.bfloat16,
+                              device=hidden.device)
+        return self.experts(hidden, ids, w16, out)
+
+    def experts(self, hidden: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor,
+                out: torch.Tensor) -> torch.Tensor:
+        """The layer after its routing: out [t, H] (bf16 or f32) <- the weighted
+        sum of the experts ``ids`` int32 [t, top_k] with ``weights`` (bf16 or
+        f32) [t, top_k] on hidden [t, H]."""
+        t = hidden.shape[0]
+        if t > self.max_tokens:
+            raise ValueError(f"{t} tokens exceed max_tokens={self.max_tokens}")
+        rows = t * self.top_k
         ops.permute_out(ids, self.w.num_experts, self.group_sizes,
                         token_indices_sorted=self.tok[:rows], revert=self.revert[:rows])
         x = self.x[:rows]
@@ -132,11 +145,7 @@ class MoELayer:
         y = self.y[:rows]
         ops.gmm_fp4_out(h1, self.w.w2, self.w.s2, self.group_sizes, y, layout=self.w.layout,
                         variant=self.gemm_variant)
-        if out is None:
-            out = torch.empty((t, self.w.hidden_size), dtype=torch.bfloat16,
-                              device=hidden.device)
-        ops.combine_out(y, self.revert[:rows], w16, self.top_k, out)
-        return out
+        return ops.combine_out(y, self.revert[:rows], weights, self.top_k, out)
 
     __call__ = forward
 
