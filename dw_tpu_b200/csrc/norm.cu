@@ -55,26 +55,62 @@ __device__ __forceinline__ int bytes_of(int runtime) {
   return is_f32<D>(runtime) ? 4 : 2;
 }
 
-// A thread works on pairs of its elements (VEC = 1: on one element a pair).
-__host__ __device__ constexpr int pairs(int vec) { return vec == 1 ? 1 : vec / 2; }
+// A thread's loads of a row: CPT of VEC elements, load c at column
+// (i + c * threads) * VEC. VEC = 8: 16-byte loads (the host has checked the
+// alignment), the threads a run-time number; VEC = 1: an element each, T threads,
+// so that the offsets of a thread's loads are constants, the first sure_loads of
+// them within the row for every row that the launch gives this CPT.
+template <int CPT, int T>
+__host__ __device__ constexpr int sure_loads() {
+  return T == 512 ? (CPT > 16 ? CPT - 8 : CPT - 2) : T == 128 ? 2 : 0;
+}
+template <int VEC, int CPT, int T>
+struct Cols {
+  int h, first;
+  int col[VEC == 8 ? CPT : 1];
+  bool in_[VEC == 8 ? CPT : 1];
 
-// A thread's CPT x VEC elements of a row as they were loaded. VEC = 8: one or
-// two 16-byte loads (the host has checked the alignment); VEC = 1: one element.
-// Element j of load c sits at column (i + c * threads) * VEC + j.
-template <int VEC, int CPT, int D>
+  __device__ __forceinline__ Cols(int h, int i, int threads) : h(h), first(i) {
+    if constexpr (VEC == 8) {
+      // Loads past the row's end read its first elements, which nothing uses.
+#pragma unroll
+      for (int c = 0; c < CPT; ++c) {
+        col[c] = (i + c * threads) * VEC;
+        in_[c] = col[c] < h;  // h is a multiple of VEC
+        if (!in_[c]) col[c] = 0;
+      }
+    }
+  }
+  __device__ __forceinline__ int at(int c) const {
+    return VEC == 8 ? col[c % (VEC == 8 ? CPT : 1)] : first + c * T;
+  }
+  __device__ __forceinline__ bool in(int c) const {
+    return VEC == 8 ? in_[c % (VEC == 8 ? CPT : 1)]
+                    : c < sure_loads<CPT, T>() || first + c * T < h;
+  }
+};
+
+// Its elements are worked on in pairs: two neighbours of a load, or (VEC = 1)
+// those of two loads. Elements past the end of the row are 0 with VEC = 1.
+__host__ __device__ constexpr int pairs(int vec, int cpt) { return vec == 8 ? 4 * cpt : cpt / 2; }
+
+// The elements as they were loaded.
+template <int VEC, int CPT, int T, int D>
 struct Raw {
   static constexpr int W = VEC == 1 ? 1 : D == BF ? 4 : 8;  // words per load
+  static constexpr int NP = pairs(VEC, CPT);
+  using C = Cols<VEC, CPT, T>;
   uint32_t u[CPT][W];
 
   // From global memory. One branch on the type for all loads, so that they
   // are issued together.
-  __device__ __forceinline__ void load(const void* p, const int (&col)[CPT], int f32) {
+  __device__ __forceinline__ void load(const void* p, const C& cols, int f32) {
     if (is_f32<D>(f32)) {
 #pragma unroll
       for (int c = 0; c < CPT; ++c) {
-        const uint8_t* q = static_cast<const uint8_t*>(p) + col[c] * 4;
+        const uint8_t* q = static_cast<const uint8_t*>(p) + cols.at(c) * 4;
         if constexpr (VEC == 1) {
-          u[c][0] = *reinterpret_cast<const uint32_t*>(q);
+          u[c][0] = cols.in(c) ? *reinterpret_cast<const uint32_t*>(q) : 0u;
         } else {
           put(c, 0, *reinterpret_cast<const uint4*>(q));
           put(c, 4, *reinterpret_cast<const uint4*>(q + 16));
@@ -83,22 +119,22 @@ struct Raw {
     } else {
 #pragma unroll
       for (int c = 0; c < CPT; ++c) {
-        const uint8_t* q = static_cast<const uint8_t*>(p) + col[c] * 2;
+        const uint8_t* q = static_cast<const uint8_t*>(p) + cols.at(c) * 2;
         if constexpr (VEC == 1)
-          u[c][0] = *reinterpret_cast<const uint16_t*>(q);
+          u[c][0] = cols.in(c) ? *reinterpret_cast<const uint16_t*>(q) : 0u;
         else
           put(c, 0, *reinterpret_cast<const uint4*>(q));
       }
     }
   }
   // From shared memory.
-  __device__ __forceinline__ void load_s(uint32_t p, const int (&col)[CPT], int f32) {
+  __device__ __forceinline__ void load_s(uint32_t p, const C& cols, int f32) {
     if (is_f32<D>(f32)) {
 #pragma unroll
       for (int c = 0; c < CPT; ++c) {
-        const uint32_t q = p + (uint32_t)col[c] * 4;
+        const uint32_t q = p + (uint32_t)cols.at(c) * 4;
         if constexpr (VEC == 1) {
-          u[c][0] = lds_u32(q);
+          u[c][0] = cols.in(c) ? lds_u32(q) : 0u;
         } else {
           put(c, 0, lds_u128(q));
           put(c, 4, lds_u128(q + 16));
@@ -107,9 +143,9 @@ struct Raw {
     } else {
 #pragma unroll
       for (int c = 0; c < CPT; ++c) {
-        const uint32_t q = p + (uint32_t)col[c] * 2;
+        const uint32_t q = p + (uint32_t)cols.at(c) * 2;
         if constexpr (VEC == 1)
-          u[c][0] = lds_u16(q);
+          u[c][0] = cols.in(c) ? lds_u16(q) : 0u;
         else
           put(c, 0, lds_u128(q));
       }
@@ -118,53 +154,69 @@ struct Raw {
   __device__ __forceinline__ void put(int c, int w, const uint4& x) {
     u[c][w % W] = x.x; u[c][(w + 1) % W] = x.y; u[c][(w + 2) % W] = x.z; u[c][(w + 3) % W] = x.w;
   }
-  // Elements 2 j and 2 j + 1 of load c (VEC = 1: the one element, and 0).
   template <bool F>
-  __device__ __forceinline__ F2 at(int c, int j) const {
-    if constexpr (VEC == 1)
-      return f2(__uint_as_float(F ? u[c][0] : u[c][0] << 16), 0.0f);
-    else if (F)
-      return f2(__uint_as_float(u[c][(2 * j) % W]), __uint_as_float(u[c][(2 * j + 1) % W]));
-    else
+  __device__ __forceinline__ F2 at(int p) const {
+    if constexpr (VEC == 1) {
+      const uint32_t a = u[2 * p][0], b = u[2 * p + 1][0];
+      return F ? f2(__uint_as_float(a), __uint_as_float(b))
+               : f2(__uint_as_float(a << 16), __uint_as_float(b << 16));
+    } else {
+      const int c = p / 4, j = p % 4;
+      if (F) return f2(__uint_as_float(u[c][(2 * j) % W]), __uint_as_float(u[c][(2 * j + 1) % W]));
       return f2(__uint_as_float(u[c][j] << 16), __uint_as_float(u[c][j] & 0xFFFF0000u));
+    }
   }
   // v <- f(v, elements) for all pairs; again one branch on the type.
   template <class F>
-  __device__ __forceinline__ void into(F2 (&v)[CPT][pairs(VEC)], int f32, const F& f) const {
+  __device__ __forceinline__ void into(F2 (&v)[NP], int f32, const F& f) const {
     if (is_f32<D>(f32)) {
 #pragma unroll
-      for (int c = 0; c < CPT; ++c)
-#pragma unroll
-        for (int q = 0; q < pairs(VEC); ++q) v[c][q] = f(v[c][q], at<true>(c, q));
+      for (int p = 0; p < NP; ++p) v[p] = f(v[p], at<true>(p));
     } else {
 #pragma unroll
-      for (int c = 0; c < CPT; ++c)
-#pragma unroll
-        for (int q = 0; q < pairs(VEC); ++q) v[c][q] = f(v[c][q], at<false>(c, q));
+      for (int p = 0; p < NP; ++p) v[p] = f(v[p], at<false>(p));
     }
   }
 };
 
-template <int VEC>
-__device__ __forceinline__ void st(uint8_t* p, bool f32, const F2 (&v)[pairs(VEC)]) {
-  float e[2 * pairs(VEC)];
-#pragma unroll
-  for (int q = 0; q < pairs(VEC); ++q) f2_split(v[q], e[2 * q], e[2 * q + 1]);
+// The pairs to their places in the row at `row`.
+template <int VEC, int CPT, int T>
+__device__ __forceinline__ void store(uint8_t* row, bool f32, const Cols<VEC, CPT, T>& cols,
+                                      const F2 (&v)[pairs(VEC, CPT)]) {
   if constexpr (VEC == 8) {
-    if (f32) {
-      float4* q = reinterpret_cast<float4*>(p);
-      q[0] = make_float4(e[0], e[1], e[2], e[3]);
-      q[1] = make_float4(e[4], e[5], e[6], e[7]);
-    } else {
-      *reinterpret_cast<uint4*>(p) =
-          make_uint4(f32x2_to_bf16x2(e[0], e[1]), f32x2_to_bf16x2(e[2], e[3]),
-                     f32x2_to_bf16x2(e[4], e[5]), f32x2_to_bf16x2(e[6], e[7]));
+#pragma unroll
+    for (int c = 0; c < CPT; ++c) {
+      if (!cols.in(c)) continue;
+      float e[8];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) f2_split(v[4 * c + q], e[2 * q], e[2 * q + 1]);
+      if (f32) {
+        float4* q = reinterpret_cast<float4*>(row + cols.at(c) * 4);
+        q[0] = make_float4(e[0], e[1], e[2], e[3]);
+        q[1] = make_float4(e[4], e[5], e[6], e[7]);
+      } else {
+        *reinterpret_cast<uint4*>(row + cols.at(c) * 2) =
+            make_uint4(f32x2_to_bf16x2(e[0], e[1]), f32x2_to_bf16x2(e[2], e[3]),
+                       f32x2_to_bf16x2(e[4], e[5]), f32x2_to_bf16x2(e[6], e[7]));
+      }
     }
   } else {
-    if (f32)
-      *reinterpret_cast<float*>(p) = e[0];
-    else
-      *reinterpret_cast<uint16_t*>(p) = (uint16_t)f32_to_bf16_bits(e[0]);
+    if (f32) {
+#pragma unroll
+      for (int c = 0; c < CPT; ++c) {
+        float e[2];
+        f2_split(v[c / 2], e[0], e[1]);
+        if (cols.in(c)) *reinterpret_cast<float*>(row + cols.at(c) * 4) = e[c % 2];
+      }
+    } else {
+#pragma unroll
+      for (int c = 0; c < CPT; ++c) {
+        float e[2];
+        f2_split(v[c / 2], e[0], e[1]);
+        if (cols.in(c))
+          *reinterpret_cast<uint16_t*>(row + cols.at(c) * 2) = (uint16_t)f32_to_bf16_bits(e[c % 2]);
+      }
+    }
   }
 }
 
@@ -209,46 +261,47 @@ struct Group {
 
 // u <- norm(u) * w + b over a row. read_done() runs once every thread of the
 // row has all of its elements of u.
-template <int VEC, int CPT, int WD, class Vec, class Done>
-__device__ __forceinline__ void normalise(F2 (&u)[CPT][pairs(VEC)], const bool (&in)[CPT],
+template <int VEC, int CPT, int T, int WD, class Vec, class Done>
+__device__ __forceinline__ void normalise(F2 (&u)[pairs(VEC, CPT)], const Cols<VEC, CPT, T>& cols,
                                           const Args& a, const Group& g, int slot, float inv_h,
                                           const Vec& vec, int weight, int bias,
                                           const Done& read_done) {
+  constexpr int NP = pairs(VEC, CPT);
   auto total = [](F2 x) {
     float lo, hi;
     f2_split(x, lo, hi);
     return lo + hi;
   };
+  // (VEC = 1: what is past the end is 0.)
+  auto in = [&](int p) { return VEC == 1 || cols.in(p / 4); };
   if (a.layer) {
     F2 s = f2(0.0f, 0.0f);
 #pragma unroll
-    for (int c = 0; c < CPT; ++c)
-      if (in[c]) {
-#pragma unroll
-        for (int q = 0; q < pairs(VEC); ++q) s = f2_add(s, u[c][q]);
-      }
+    for (int p = 0; p < NP; ++p)
+      if (in(p)) s = f2_add(s, u[p]);
     const float mean = g.sum(total(s), slot, [] {}) * inv_h;
-    // The second half of a VEC = 1 pair stays 0.
-    const F2 minus = f2(-mean, VEC == 1 ? 0.0f : -mean);
+    const F2 minus = f2(-mean, -mean);
 #pragma unroll
-    for (int c = 0; c < CPT; ++c)
-#pragma unroll
-      for (int q = 0; q < pairs(VEC); ++q) u[c][q] = f2_add(u[c][q], minus);
+    for (int p = 0; p < NP; ++p) {
+      u[p] = f2_add(u[p], minus);
+      if (VEC == 1 && 2 * p + 1 >= sure_loads<CPT, T>()) {
+        float lo, hi;
+        f2_split(u[p], lo, hi);
+        u[p] = f2(cols.in(2 * p) ? lo : 0.0f, cols.in(2 * p + 1) ? hi : 0.0f);
+      }
+    }
   }
   F2 s2 = f2(0.0f, 0.0f);
 #pragma unroll
-  for (int c = 0; c < CPT; ++c)
-    if (in[c]) {
-#pragma unroll
-      for (int q = 0; q < pairs(VEC); ++q) s2 = f2_fma(u[c][q], u[c][q], s2);
-    }
+  for (int p = 0; p < NP; ++p)
+    if (in(p)) s2 = f2_fma(u[p], u[p], s2);
   const float rstd = rsqrtf(g.sum(total(s2), slot + 1, read_done) * inv_h + a.eps);
   const F2 rstd2 = f2(rstd, rstd);
-  vec(weight, [&](const Raw<VEC, CPT, WD>& w) {
+  vec(weight, [&](const Raw<VEC, CPT, T, WD>& w) {
     w.into(u, a.w_f32, [&](F2 v, F2 x) { return f2_mul(f2_mul(v, rstd2), x); });
   });
   if (a.vec[bias])
-    vec(bias, [&](const Raw<VEC, CPT, WD>& b) {
+    vec(bias, [&](const Raw<VEC, CPT, T, WD>& b) {
       b.into(u, a.w_f32, [](F2 v, F2 x) { return f2_add(v, x); });
     });
 }
@@ -258,48 +311,34 @@ __device__ __forceinline__ void normalise(F2 (&u)[CPT][pairs(VEC)], const bool (
 // where the caller has loaded them ahead, or from where they lie. r_out and
 // h_out point to the row. read_done() runs once every thread has the row's
 // elements.
-template <int VEC, int CPT, int YD, int RD, int WD, class Y, class Res, class Gate, class Vec,
-          class Done>
+template <int VEC, int CPT, int T, int YD, int RD, int WD, class Y, class Res, class Gate,
+          class Vec, class Done>
 __device__ __forceinline__ void do_row(const Args& a, const Group& g, uint8_t* r_out,
-                                       uint8_t* h_out, float inv_h, const int (&col)[CPT],
-                                       const bool (&in)[CPT], float gate_tok, const Y& y,
+                                       uint8_t* h_out, float inv_h,
+                                       const Cols<VEC, CPT, T>& cols, float gate_tok, const Y& y,
                                        const Res& res, const Gate& gate, const Vec& vec,
                                        const Done& read_done) {
-  F2 v[CPT][pairs(VEC)];
+  using RawY = Raw<VEC, CPT, T, YD>;
+  using RawR = Raw<VEC, CPT, T, RD>;
+  F2 v[pairs(VEC, CPT)];
   if (a.y) {
-    y([&](const Raw<VEC, CPT, YD>& x) {
-      x.into(v, a.y_f32, [](F2, F2 e) { return e; });
-    });
-    if (a.inner) normalise<VEC, CPT, WD>(v, in, a, g, 0, inv_h, vec, W2, B2, [] {});
+    y([&](const RawY& x) { x.into(v, a.y_f32, [](F2, F2 e) { return e; }); });
+    if (a.inner)
+      normalise<VEC, CPT, T, WD>(v, cols, a, g, 0, inv_h, vec, W2, B2, [] {});
     if (a.gate_mode >= DWM_GATE_CHANNEL)
-      gate([&](const Raw<VEC, CPT, YD>& x) {
-        x.into(v, a.y_f32, [](F2 u, F2 e) { return f2_mul(u, e); });
-      });
+      gate([&](const RawY& x) { x.into(v, a.y_f32, [](F2 u, F2 e) { return f2_mul(u, e); }); });
     const F2 scale = f2(a.scale * gate_tok, a.scale * gate_tok);
     const F2 res_scale = f2(a.res_scale, a.res_scale);
-    res([&](const Raw<VEC, CPT, RD>& x) {
+    res([&](const RawR& x) {
       x.into(v, a.res_f32, [&](F2 u, F2 e) { return f2_fma(scale, u, f2_mul(res_scale, e)); });
     });
-    const int es = bytes_of<RD>(a.res_f32);
-#pragma unroll
-    for (int c = 0; c < CPT; ++c)
-      if (in[c]) st<VEC>(r_out + col[c] * es, es == 4, v[c]);
+    store<VEC, CPT, T>(r_out, is_f32<RD>(a.res_f32), cols, v);
   } else {
-    res([&](const Raw<VEC, CPT, RD>& x) {
-      x.into(v, a.res_f32, [](F2, F2 e) { return e; });
-    });
+    res([&](const RawR& x) { x.into(v, a.res_f32, [](F2, F2 e) { return e; }); });
   }
   if (a.h_out) {
-    normalise<VEC, CPT, WD>(v, in, a, g, 2, inv_h, vec, W1, B1, read_done);
-    if (a.h_f32) {
-#pragma unroll
-      for (int c = 0; c < CPT; ++c)
-        if (in[c]) st<VEC>(h_out + col[c] * 4, true, v[c]);
-    } else {
-#pragma unroll
-      for (int c = 0; c < CPT; ++c)
-        if (in[c]) st<VEC>(h_out + col[c] * 2, false, v[c]);
-    }
+    normalise<VEC, CPT, T, WD>(v, cols, a, g, 2, inv_h, vec, W1, B1, read_done);
+    store<VEC, CPT, T>(h_out, a.h_f32 != 0, cols, v);
   } else {
     g.sync();
     read_done();
@@ -314,18 +353,6 @@ __device__ __forceinline__ float token_gate(const Args& a, int64_t row) {
              : bf16_bits_to_f32(static_cast<const uint16_t*>(a.gate)[row * a.ldg]);
 }
 
-// Loads past the row's end read its first elements, which nothing uses.
-template <int VEC, int CPT>
-__device__ __forceinline__ void columns(const Args& a, const Group& g, int (&col)[CPT],
-                                        bool (&in)[CPT]) {
-#pragma unroll
-  for (int c = 0; c < CPT; ++c) {
-    col[c] = (g.i + c * g.threads) * VEC;
-    in[c] = col[c] < a.h;  // h is a multiple of VEC
-    if (!in[c]) col[c] = 0;
-  }
-}
-
 __device__ __forceinline__ const uint8_t* row_ptr(const void* p, int64_t row, int64_t ld, int es) {
   return static_cast<const uint8_t*>(p) + row * ld * es;
 }
@@ -337,12 +364,12 @@ __device__ __forceinline__ uint8_t* row_ptr(void* p, int64_t row, int64_t ld, in
 // streaming kernel 1024 (64 registers each) unless a thread has 32 elements.
 template <int VEC, int CPT>
 constexpr int max_threads(bool stream) {
-  return VEC * CPT > 16 || (VEC == 8 && !stream) ? 512 : 1024;
+  return VEC * CPT > 16 || !stream ? 512 : 1024;
 }
 
 // A few rows: one group a row, every load of a row issued before its first
 // sum, so that a row costs one memory latency. threadIdx.y: the CTA's groups.
-template <int VEC, int CPT, int YD, int RD, int WD>
+template <int VEC, int CPT, int T, int YD, int RD, int WD>
 __global__ void __launch_bounds__(max_threads<VEC, CPT>(false)) block_norm_kernel(const Args a) {
   __shared__ __align__(16) float part[4][32];
   const Group g{(int)threadIdx.x, (int)blockDim.x, 0, part};
@@ -350,34 +377,32 @@ __global__ void __launch_bounds__(max_threads<VEC, CPT>(false)) block_norm_kerne
   overlap_wait();
   overlap_next();
   if (row >= a.t) return;  // a whole warp of a CTA with a warp a row
-  int col[CPT];
-  bool in[CPT];
-  columns<VEC, CPT>(a, g, col, in);
+  const Cols<VEC, CPT, T> cols(a.h, g.i, g.threads);
   const int ye = bytes_of<YD>(a.y_f32), re = bytes_of<RD>(a.res_f32);
   const uint8_t* pg = row_ptr(a.gate, a.gate_mode == DWM_GATE_FULL ? row : 0, a.ldg, ye);
   // Up to 16 elements a thread everything is loaded ahead; the gate and the
   // weights of more would not fit the registers.
   constexpr bool AHEAD = VEC == 8 && CPT <= 2;
-  Raw<VEC, CPT, YD> y, gate;
-  Raw<VEC, CPT, RD> res;
-  Raw<VEC, CPT, WD> w2, w1;
-  if (a.y) y.load(row_ptr(a.y, row, a.ldy, ye), col, a.y_f32);
-  res.load(row_ptr(a.res, row, a.ldres, re), col, a.res_f32);
+  Raw<VEC, CPT, T, YD> y, gate;
+  Raw<VEC, CPT, T, RD> res;
+  Raw<VEC, CPT, T, WD> w2, w1;
+  if (a.y) y.load(row_ptr(a.y, row, a.ldy, ye), cols, a.y_f32);
+  res.load(row_ptr(a.res, row, a.ldres, re), cols, a.res_f32);
   if (AHEAD) {
-    if (a.inner) w2.load(a.vec[W2], col, a.w_f32);
-    if (a.gate_mode >= DWM_GATE_CHANNEL) gate.load(pg, col, a.y_f32);
-    if (a.h_out) w1.load(a.vec[W1], col, a.w_f32);
+    if (a.inner) w2.load(a.vec[W2], cols, a.w_f32);
+    if (a.gate_mode >= DWM_GATE_CHANNEL) gate.load(pg, cols, a.y_f32);
+    if (a.h_out) w1.load(a.vec[W1], cols, a.w_f32);
   }
   const float tok = token_gate<YD>(a, row);
   if (g.threads > 32) {
     g.clear_parts();
     g.sync();
   }
-  do_row<VEC, CPT, YD, RD, WD>(
+  do_row<VEC, CPT, T, YD, RD, WD>(
       a, g, row_ptr(a.r_out, row, a.ldr, re), row_ptr(a.h_out, row, a.ldh, a.h_f32 ? 4 : 2),
-      1.0f / (float)a.h, col, in, tok, [&](auto f) { f(y); }, [&](auto f) { f(res); },
+      1.0f / (float)a.h, cols, tok, [&](auto f) { f(y); }, [&](auto f) { f(res); },
       [&](auto f) {
-        if (!AHEAD) gate.load(pg, col, a.y_f32);
+        if (!AHEAD) gate.load(pg, cols, a.y_f32);
         f(gate);
       },
       [&](int which, auto f) {
@@ -386,8 +411,8 @@ __global__ void __launch_bounds__(max_threads<VEC, CPT>(false)) block_norm_kerne
         } else if (AHEAD && which == W1) {
           f(w1);
         } else {
-          Raw<VEC, CPT, WD> x;
-          x.load(a.vec[which], col, a.w_f32);
+          Raw<VEC, CPT, T, WD> x;
+          x.load(a.vec[which], cols, a.w_f32);
           f(x);
         }
       },
@@ -415,7 +440,7 @@ __device__ __forceinline__ void bulk_row(uint32_t dst, const uint8_t* p, int byt
 constexpr int MAX_STAGES = 8;
 constexpr int MAX_GROUPS = 16;
 
-template <int VEC, int CPT, int YD, int RD, int WD>
+template <int VEC, int CPT, int T, int YD, int RD, int WD>
 __global__ void __launch_bounds__(max_threads<VEC, CPT>(true), 1)
     block_norm_stream_kernel(const Args a) {
   __shared__ __align__(16) float part[MAX_GROUPS][4][32];
@@ -437,9 +462,7 @@ __global__ void __launch_bounds__(max_threads<VEC, CPT>(true), 1)
   __syncthreads();
   overlap_wait();
   overlap_next();
-  int col[CPT];
-  bool in[CPT];
-  columns<VEC, CPT>(a, g, col, in);
+  const Cols<VEC, CPT, T> cols(a.h, g.i, g.threads);
   const float inv_h = 1.0f / (float)a.h;
   const int64_t first = (int64_t)blockIdx.x * groups + gi, step = (int64_t)gridDim.x * groups;
   const bool full_gate = a.gate_mode == DWM_GATE_FULL;
@@ -497,38 +520,38 @@ __global__ void __launch_bounds__(max_threads<VEC, CPT>(true), 1)
     auto lead = [&](const void* p, int64_t ld, int es) {
       return VEC == 8 ? 0u : (uint32_t)reinterpret_cast<uint64_t>(row_ptr(p, row, ld, es)) & 15u;
     };
-    do_row<VEC, CPT, YD, RD, WD>(
-        a, g, r_out, h_out, inv_h, col, in, tok,
+    do_row<VEC, CPT, T, YD, RD, WD>(
+        a, g, r_out, h_out, inv_h, cols, tok,
         [&](auto f) {
-          Raw<VEC, CPT, YD> x;
-          x.load_s(at + lead(a.y, a.ldy, ye), col, a.y_f32);
+          Raw<VEC, CPT, T, YD> x;
+          x.load_s(at + lead(a.y, a.ldy, ye), cols, a.y_f32);
           f(x);
         },
         [&](auto f) {
-          Raw<VEC, CPT, RD> x;
-          x.load_s(at + a.off_res + lead(a.res, a.ldres, re), col, a.res_f32);
+          Raw<VEC, CPT, T, RD> x;
+          x.load_s(at + a.off_res + lead(a.res, a.ldres, re), cols, a.res_f32);
           f(x);
         },
         [&](auto f) {
           if (full_gate) {
-            Raw<VEC, CPT, YD> x;
-            x.load_s(at + a.off_gate + lead(a.gate, a.ldg, ye), col, a.y_f32);
+            Raw<VEC, CPT, T, YD> x;
+            x.load_s(at + a.off_gate + lead(a.gate, a.ldg, ye), cols, a.y_f32);
             f(x);
           } else {
-            Raw<VEC, CPT, YD> x;
+            Raw<VEC, CPT, T, YD> x;
             if (a.vec_bytes)
-              x.load_s(vectors + CHANNEL_GATE * a.vec_bytes, col, a.y_f32);
+              x.load_s(vectors + CHANNEL_GATE * a.vec_bytes, cols, a.y_f32);
             else
-              x.load(a.gate, col, a.y_f32);
+              x.load(a.gate, cols, a.y_f32);
             f(x);
           }
         },
         [&](int which, auto f) {
-          Raw<VEC, CPT, WD> x;
+          Raw<VEC, CPT, T, WD> x;
           if (a.vec_bytes)
-            x.load_s(vectors + which * a.vec_bytes, col, a.w_f32);
+            x.load_s(vectors + which * a.vec_bytes, cols, a.w_f32);
           else
-            x.load(a.vec[which], col, a.w_f32);
+            x.load(a.vec[which], cols, a.w_f32);
           f(x);
         },
         [&] {
@@ -543,11 +566,11 @@ __global__ void __launch_bounds__(max_threads<VEC, CPT>(true), 1)
     for (int i = 0; i < a.stages; ++i) mbar_wait(&full[gi][i], ph ^ (i >= s), nullptr, a.status);
 }
 
-template <int VEC, int CPT, int YD, int RD, int WD>
+template <int VEC, int CPT, int T, int YD, int RD, int WD>
 int launch(Args a, cudaStream_t s) {
   const int n = (a.h + VEC - 1) / VEC;  // loads a row
   // A group: as many warps as the row takes with CPT loads a thread.
-  const int threads = ((n + CPT - 1) / CPT + 31) / 32 * 32;
+  const int threads = T ? T : ((n + CPT - 1) / CPT + 31) / 32 * 32;
   const int groups = std::min(MAX_GROUPS, max_threads<VEC, CPT>(true) / threads);
   if ((int64_t)a.t > 2 * (int64_t)num_sms() * groups) {
     auto room = [&](int f32) { return (a.h * (f32 ? 4 : 2) + 15) / 16 * 16 + (VEC == 1 ? 16 : 0); };
@@ -560,7 +583,7 @@ int launch(Args a, cudaStream_t s) {
     const int left = budget - 5 * a.vec_bytes;
     a.stages = std::min(MAX_STAGES, left / (groups * a.stage_bytes));
     if (a.stages >= 2) {
-      auto fn = block_norm_stream_kernel<VEC, CPT, YD, RD, WD>;
+      auto fn = block_norm_stream_kernel<VEC, CPT, T, YD, RD, WD>;
       const int rc = set_smem_limit(reinterpret_cast<const void*>(fn), budget, "norm smem attribute");
       if (rc) return rc;
       a.status = status_ptr();
@@ -573,7 +596,7 @@ int launch(Args a, cudaStream_t s) {
   }
   // A warp a row, four a CTA, or a CTA a row.
   const int rows = threads == 32 ? 4 : 1;
-  return check_cuda(overlap_launch(block_norm_kernel<VEC, CPT, YD, RD, WD>,
+  return check_cuda(overlap_launch(block_norm_kernel<VEC, CPT, T, YD, RD, WD>,
                                    dim3((unsigned)((a.t + rows - 1) / rows)),
                                    dim3((unsigned)threads, (unsigned)rows), 0, 1, s, a),
                     "block_norm launch");
@@ -585,16 +608,26 @@ int by_width(const Args& a, cudaStream_t s) {
   const bool many = a.t > 2 * num_sms();
   if constexpr (VEC == 8) {
     // Few rows: a load a thread.
-    if (n <= 32 || (!many && n <= 512)) return launch<8, 1, YD, RD, WD>(a, s);
-    if (n <= 1024) return launch<8, 2, YD, RD, WD>(a, s);
-    return launch<8, 4, YD, RD, WD>(a, s);
+    if (n <= 32 || (!many && n <= 512)) return launch<8, 1, 0, YD, RD, WD>(a, s);
+    if (n <= 1024) return launch<8, 2, 0, YD, RD, WD>(a, s);
+    return launch<8, 4, 0, YD, RD, WD>(a, s);
   } else {
-    if (n <= 8192) return launch<1, 8, YD, RD, WD>(a, s);
-    return launch<1, 16, YD, RD, WD>(a, s);
+    // (sure_loads goes by these.)
+    if (n <= 32 * 8) return launch<1, 8, 32, YD, RD, WD>(a, s);
+    if (n <= 128 * 8) return launch<1, 8, 128, YD, RD, WD>(a, s);
+    if (n <= 512 * 4) return launch<1, 4, 512, YD, RD, WD>(a, s);
+    if (n <= 512 * 6) return launch<1, 6, 512, YD, RD, WD>(a, s);
+    if (n <= 512 * 8) return launch<1, 8, 512, YD, RD, WD>(a, s);
+    if (n <= 512 * 10) return launch<1, 10, 512, YD, RD, WD>(a, s);
+    if (n <= 512 * 12) return launch<1, 12, 512, YD, RD, WD>(a, s);
+    if (n <= 512 * 14) return launch<1, 14, 512, YD, RD, WD>(a, s);
+    if (n <= 512 * 16) return launch<1, 16, 512, YD, RD, WD>(a, s);
+    if (n <= 512 * 24) return launch<1, 24, 512, YD, RD, WD>(a, s);
+    return launch<1, 32, 512, YD, RD, WD>(a, s);
   }
 }
 
-// Rows of at most 32 elements a thread of 512 (VEC = 1: 16 a thread of 1024).
+// Rows of at most 32 elements a thread of 512.
 constexpr int MAX_H = 16384;
 
 int run(const Args& a, bool vec, cudaStream_t s) {
