@@ -189,8 +189,8 @@ __device__ __forceinline__ void activate(const Args& a, float (&z)[N], float (&u
 // with SwiGLU, the up products u): bias, activation, residual, one rounding.
 // Rows of out start on 16 bytes (Args::out_vec).
 template <int EPI, int N>
-__device__ __forceinline__ void epilogue(const Args& a, int64_t row, int col, float (&z)[N],
-                                         float (&u)[N]) {
+__device__ __forceinline__ void bias_and_act(const Args& a, int col, float (&z)[N],
+                                             float (&u)[N]) {
   const bool whole = col + N <= a.n_out;
   if (a.bias) {
     float b[N];
@@ -212,6 +212,12 @@ __device__ __forceinline__ void epilogue(const Args& a, int64_t row, int col, fl
     }
   }
   activate<EPI>(a, z, u);
+}
+template <int EPI, int N>
+__device__ __forceinline__ void epilogue(const Args& a, int64_t row, int col, float (&z)[N],
+                                         float (&u)[N]) {
+  const bool whole = col + N <= a.n_out;
+  bias_and_act<EPI>(a, col, z, u);
   if (a.residual) {
     const int64_t at = row * a.ldr + col;
     if (whole && a.res_vec) {
@@ -587,8 +593,11 @@ int launch_split(const void* x, int64_t ldx, const void* w, int64_t ldw, int n, 
 // w's rows is the gate and the odd one's the up projection of 128 features, so
 // a feature's two products are two columns of one TMEM lane.
 //
-// Warps 0-7 epilogue (TMEM lane quarter w % 4, half w / 4 of the columns): a
-// row a lane, stored a 32-byte sector at a time; warp 8 TMA; warp 9 UMMA.
+// Warps 0-7 epilogue (TMEM lane quarter w % 4, half w / 4 of the columns): a row
+// a lane, 32 columns at a time through swizzled shared memory and TMA, the
+// residual in and the result out (16-byte accesses of a row a lane instead cost
+// 32 cache lines an instruction: 1024 x 2048 x 4096 with an f32 residual took 26
+// us); warp 8 TMA; warp 9 UMMA.
 //
 // Bound: the tensor cores.
 // ---------------------------------------------------------------------------
@@ -600,13 +609,21 @@ constexpr int THREADS = 320;
 constexpr int EPI_WARPS = 8, TMA_WARP = 8, MMA_WARP = 9;
 constexpr int OP_STAGE = HALF * BK * 2;  // 16 KiB: one operand's k step
 constexpr int STG = 2 * OP_STAGE;
-constexpr int S = 6;
-constexpr int EPI_BYTES = 32 * 32 * 4;   // a warp's 32 x 32 f32
-constexpr int OFF_EPI = S * STG;
-constexpr int OFF_BAR = OFF_EPI + EPI_WARPS * EPI_BYTES;
-constexpr int OFF_MISC = OFF_BAR + (2 * S + 5) * 8;
-constexpr int ALLOC = OFF_MISC + 16 + 1024;  // slack for 1 KiB alignment
-static_assert(ALLOC <= 232448, "exceeds the 227 KiB per-CTA shared memory");
+constexpr int BOX = 32;                  // rows and columns of an epilogue step
+constexpr int OUT_BYTES = BOX * BOX * 4;  // a warp's: one f32 step or two bf16 ones
+// RES: the residual comes by TMA, into room for two f32 or four bf16 steps a
+// warp, which leaves four k steps of operands instead of six.
+template <bool RES>
+struct Layout {
+  static constexpr int S = RES ? 4 : 6;
+  static constexpr int RES_BYTES = RES ? 2 * OUT_BYTES : 0;
+  static constexpr int OFF_OUT = S * STG;
+  static constexpr int OFF_RES = OFF_OUT + EPI_WARPS * OUT_BYTES;
+  static constexpr int OFF_BAR = OFF_RES + EPI_WARPS * RES_BYTES;
+  static constexpr int OFF_MISC = OFF_BAR + (2 * S + 5 + 4 * EPI_WARPS) * 8;
+  static constexpr int ALLOC = OFF_MISC + 16 + 1024;  // slack for 1 KiB alignment
+  static_assert(ALLOC <= 232448, "exceeds the 227 KiB per-CTA shared memory");
+};
 constexpr int TMEM_COLS = 512;
 constexpr int GROUP_ROWS = 8;  // rows of tiles taken together
 
@@ -618,20 +635,34 @@ __device__ __forceinline__ void tile_at(int idx, int mt, int nt, int& tm, int& t
   tn = in / rows;
 }
 
-template <int EPI, bool VEC>  // VEC: rows of out start on 16 bytes
+// Byte offset of 16-byte chunk c of row r in a box of 32 rows of 32 elements, as
+// TMA swizzles it: 64-byte rows (bf16) or 128-byte rows (f32).
+__device__ __forceinline__ uint32_t box_at(int r, int c, int f32) {
+  return f32 ? (uint32_t)(r * 128 + ((c ^ (r & 7)) << 4))
+             : (uint32_t)(r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
+}
+
+// VEC: rows of out and of the residual start on 16 bytes; RES: there is one
+// (without VEC it is read where it is added).
+template <int EPI, bool VEC, bool RES>
 __global__ void __launch_bounds__(THREADS, 1)
     dense_pair_kernel(const __grid_constant__ CUtensorMap tm_x,
-                      const __grid_constant__ CUtensorMap tm_w, const Args a) {
+                      const __grid_constant__ CUtensorMap tm_w,
+                      const __grid_constant__ CUtensorMap tm_out,
+                      const __grid_constant__ CUtensorMap tm_res, const Args a) {
+  using L = Layout<RES>;
+  constexpr int S = L::S;
   constexpr int FEAT = EPI == GLU ? HALF : TILE;  // output columns of a tile
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + OFF_BAR);  // even CTA: both CTAs' copies landed
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR);  // even CTA: both CTAs' copies landed
   uint64_t* empty = full + S;          // each CTA: the pair's UMMAs done with the stage
   uint64_t* acc_full = empty + S;      // each CTA: accumulator complete
   uint64_t* acc_empty = acc_full + 2;  // even CTA: both CTAs drained it
   uint64_t* drain = acc_empty + 2;     // each CTA: every UMMA complete
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + OFF_MISC);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + OFF_MISC + 4);
+  uint64_t* res_full = drain + 1;      // [EPI_WARPS][4]: a residual step has landed
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::OFF_MISC);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::OFF_MISC + 4);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
   const int cl = (int)cluster_index(), ncl = (int)cluster_count();
@@ -649,6 +680,8 @@ __global__ void __launch_bounds__(THREADS, 1)
       mbar_init(&acc_empty[i], 2 * EPI_WARPS);
     }
     mbar_init(drain, 1);
+    if (RES)
+      for (int i = 0; i < 4 * EPI_WARPS; ++i) mbar_init(&res_full[i], 1);
     *abort_flag = 0;
     fence_mbar_init();
     tma_prefetch_desc(&tm_x);
@@ -671,64 +704,178 @@ __global__ void __launch_bounds__(THREADS, 1)
 
   if (warp < EPI_WARPS) {
     const int q = warp & 3, half = warp >> 2;
-    const uint32_t stage = smem_u32(smem + OFF_EPI + warp * EPI_BYTES);
+    const uint32_t stage = smem_u32(smem + L::OFF_OUT + warp * OUT_BYTES);
+    uint8_t* res_smem = smem + L::OFF_RES + warp * L::RES_BYTES;
+    const uint32_t res_at = smem_u32(res_smem);
+    const int out_step = a.out_f32 ? OUT_BYTES : OUT_BYTES / 2;  // bytes of a step
+    const int res_step = a.res_f32 ? OUT_BYTES : OUT_BYTES / 2, res_ring = a.res_f32 ? 2 : 4;
+    int out_buf = 0, res_buf = 0;
+    uint32_t res_ph = 0;
     int slot = 0;
     uint32_t ph = 0;
+    bool res_ok = true;
     for (int idx = cl; idx < total; idx += ncl) {
       int tm, tn;
       tile_at(idx, mt, nt, tm, tn);
       const int64_t row0 = (int64_t)tm * TILE + rank * HALF + q * 32;
       const int col0 = tn * FEAT + half * (FEAT / 2);
       const int valid = (int)min((int64_t)32, a.m - row0);  // rows, maybe none
-      if (!__all_sync(0xffffffffu, mbar_wait<64>(&acc_full[slot], ph, abort_flag, a.status))) break;
+      // Steps of 32 output columns, of two blocks of 16.
+      const int cols = valid <= 0 ? 0 : min(FEAT / 2, a.n_out - col0);
+      const int steps = (cols + BOX - 1) / BOX, blocks = (cols + 15) / 16;
+      auto fetch_res = [&](int i) {  // lane 0: step i into the ring's place for it
+        const int at = (res_buf + i) % res_ring;
+        uint64_t* bar = &res_full[warp * 4 + at];
+        mbar_arrive_expect_tx(bar, (uint32_t)res_step);
+        tma_load_2d(res_smem + at * res_step, &tm_res, bar, col0 + i * BOX, (int)row0,
+                    policy_evict_first());
+      };
+      if (RES && lane == 0) {
+        for (int i = 0; i < min(steps, res_ring); ++i) fetch_res(i);
+        for (int i = res_ring; i < steps; ++i)
+          tma_prefetch_2d(&tm_res, col0 + i * BOX, (int)row0);
+      }
+      // Bias of four of the warp's columns (SwiGLU: of the gate's in the first
+      // 16 lanes, of the up projection's in the others).
+      float bias[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      if (VEC && a.bias) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int c = min(col0 + (EPI == GLU ? lane & 15 : lane) * 4 + j, a.n_out - 1);
+          bias[j] = ld1(a.bias, c + (EPI == GLU && lane >= 16 ? a.n_out : 0), a.bias_f32);
+        }
+      }
+      if (!__all_sync(0xffffffffu, mbar_wait<64>(&acc_full[slot], ph, abort_flag, a.status))) {
+        // The residual's copies in flight land before the exit.
+        if (RES && lane == 0)
+          for (int i = 0; i < min(steps, res_ring); ++i) {
+            const int at = (res_buf + i) % res_ring;
+            mbar_wait(&res_full[warp * 4 + at], (res_ph >> at) & 1u, nullptr, a.status);
+          }
+        break;
+      }
       tc_fence_after();
       const uint32_t acc =
           tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(slot * TILE + half * (FEAT / 2));
-      constexpr int CHUNK = EPI == GLU ? 16 : 32;  // output columns a step
-      const int steps = valid <= 0 ? 0 : min(FEAT / 2, a.n_out - col0 + CHUNK - 1) / CHUNK;
-      // Two blocks of 16 columns a step: neighbours, or gate and up.
       uint32_t r0[16], r1[16];
       auto fetch = [&](int c) {
         tmem_ld16(acc + c, r0);
-        tmem_ld16(acc + c + (EPI == GLU ? HALF : 16), r1);
+        if (EPI == GLU) tmem_ld16(acc + c + HALF, r1);
       };
-      if (steps > 0) fetch(0);
-      for (int i = 0; i < steps; ++i) {
-        const int c = i * CHUNK;
+      if (blocks > 0) fetch(0);
+      for (int b = 0; b < blocks; ++b) {
+        const int c = b * 16;
         tmem_ld_wait(r0);
-        tmem_ld_wait(r1);
+        if (EPI == GLU) tmem_ld_wait(r1);
         if (VEC) {
-          // A row a lane: 16 columns are 32 or 64 bytes of it.
           float z[16], u[16];
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
             z[j] = __uint_as_float(r0[j]);
-            u[j] = __uint_as_float(r1[j]);
+            u[j] = EPI == GLU ? __uint_as_float(r1[j]) : 0.0f;
           }
-          if (i + 1 < steps) fetch(c + CHUNK);
-          if (lane < valid) {
-            epilogue<EPI>(a, row0 + lane, col0 + c, z, u);
-            if (EPI != GLU && col0 + c + 16 < a.n_out)
-              epilogue<EPI>(a, row0 + lane, col0 + c + 16, u, z);
+          if (b + 1 < blocks) fetch(c + 16);
+          if (a.bias) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              z[j] += __shfl_sync(0xffffffffu, bias[j & 3], (c + j) >> 2);
+              if (EPI == GLU) u[j] += __shfl_sync(0xffffffffu, bias[j & 3], 16 + ((c + j) >> 2));
+            }
+          }
+          activate<EPI>(a, z, u);
+          if (RES) {
+            if ((b & 1) == 0)
+              res_ok &= mbar_wait(&res_full[warp * 4 + res_buf], (res_ph >> res_buf) & 1u,
+                                  abort_flag, a.status);
+            const uint32_t from = res_at + (uint32_t)(res_buf * res_step);
+            float r[16];
+            if (a.res_f32) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const uint4 x = lds_u128(from + box_at(lane, (b & 1) * 4 + j, 1));
+                r[4 * j] = __uint_as_float(x.x); r[4 * j + 1] = __uint_as_float(x.y);
+                r[4 * j + 2] = __uint_as_float(x.z); r[4 * j + 3] = __uint_as_float(x.w);
+              }
+            } else {
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {
+                const uint4 x = lds_u128(from + box_at(lane, (b & 1) * 2 + j, 0));
+                const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  r[8 * j + 2 * e] = __uint_as_float(w[e] << 16);
+                  r[8 * j + 2 * e + 1] = __uint_as_float(w[e] & 0xFFFF0000u);
+                }
+              }
+            }
+#pragma unroll
+            for (int j = 0; j < 16; ++j) z[j] = fmaf(a.res_scale, r[j], z[j]);
+          }
+          if ((b & 1) == 0) {
+            // The store that last read this buffer is done with it.
+            if (lane == 0) {
+              if (a.out_f32)
+                bulk_wait_read<0>();
+              else
+                bulk_wait_read<1>();
+            }
+            __syncwarp();
+          }
+          const uint32_t to = stage + (uint32_t)(out_buf * out_step);
+          if (a.out_f32) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              sts_u128(to + box_at(lane, (b & 1) * 4 + j, 1), __float_as_uint(z[4 * j]),
+                       __float_as_uint(z[4 * j + 1]), __float_as_uint(z[4 * j + 2]),
+                       __float_as_uint(z[4 * j + 3]));
+          } else {
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+              sts_u128(to + box_at(lane, (b & 1) * 2 + j, 0),
+                       f32x2_to_bf16x2(z[8 * j], z[8 * j + 1]),
+                       f32x2_to_bf16x2(z[8 * j + 2], z[8 * j + 3]),
+                       f32x2_to_bf16x2(z[8 * j + 4], z[8 * j + 5]),
+                       f32x2_to_bf16x2(z[8 * j + 6], z[8 * j + 7]));
+          }
+          if ((b & 1) == 1 || b + 1 == blocks) {
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              // (Columns and rows past the end are not stored.)
+              tma_store_2d(&tm_out, to, col0 + (b >> 1) * BOX, (int)row0);
+              bulk_commit();
+            }
+            if (!a.out_f32) out_buf ^= 1;
+            if (RES) {
+              // Every lane has read the step: its place takes the next but few.
+              res_ph ^= 1u << res_buf;
+              if (lane == 0 && (b >> 1) + res_ring < steps) {
+                uint64_t* bar = &res_full[warp * 4 + res_buf];
+                mbar_arrive_expect_tx(bar, (uint32_t)res_step);
+                tma_load_2d(res_smem + res_buf * res_step, &tm_res, bar,
+                            col0 + ((b >> 1) + res_ring) * BOX, (int)row0, policy_evict_first());
+              }
+              if (++res_buf == res_ring) res_buf = 0;
+            }
           }
         } else {
-          // A column a lane (with SwiGLU two rows of 16 at a time), by way of
-          // shared memory: 16-byte blocks of a row, XORed with the row against
-          // bank conflicts.
+          // A column a lane, two rows of 16 at a time, by way of shared memory:
+          // 16-byte blocks of a row of 32, XORed with the row against conflicts.
           auto block_at = [&](int rr, int j) {
             return stage + (uint32_t)(rr * 128 + ((j ^ (rr & 7)) << 4));
           };
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             sts_u128(block_at(lane, j), r0[4 * j], r0[4 * j + 1], r0[4 * j + 2], r0[4 * j + 3]);
-            sts_u128(block_at(lane, 4 + j), r1[4 * j], r1[4 * j + 1], r1[4 * j + 2],
-                     r1[4 * j + 3]);
+            if (EPI == GLU)
+              sts_u128(block_at(lane, 4 + j), r1[4 * j], r1[4 * j + 1], r1[4 * j + 2],
+                       r1[4 * j + 3]);
           }
           __syncwarp();
-          if (i + 1 < steps) fetch(c + CHUNK);
-          const int col = lane % CHUNK;
+          if (b + 1 < blocks) fetch(c + 16);
+          const int col = lane % 16;
           if (col0 + c + col < a.n_out)
-            for (int rr = lane / CHUNK * 8; rr < valid; rr += 32 / CHUNK * 8) {
+            for (int rr = lane / 16 * 8; rr < valid; rr += 16) {
               float z[8], u[8];
 #pragma unroll
               for (int q = 0; q < 8; ++q) {
@@ -746,6 +893,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       if (lane == 0) mbar_arrive_remote(acc_empty_0 + (uint32_t)(slot * 8));
       if (++slot == 2) { slot = 0; ph ^= 1; }
     }
+    if (VEC && lane == 0) bulk_wait_all();  // before this CTA's shared memory goes
   } else if (warp == TMA_WARP) {
     if (lane == 0) {
       const uint64_t pol_w = policy_evict_last(), pol_x = policy_evict_normal();
@@ -840,28 +988,38 @@ __global__ void __launch_bounds__(THREADS, 1)
   cluster_sync();
 }
 
-template <int EPI, bool VEC>
+template <int EPI, bool VEC, bool RES>
 int launch(const void* x, int64_t ldx, const void* w, int64_t ldw, int n, const Args& a,
            cudaStream_t stream) {
+  using L = Layout<RES>;
   constexpr int FEAT = EPI == GLU ? HALF : TILE;
   const int64_t tiles = (int64_t)((a.m + (int64_t)TILE - 1) / TILE) *
                         ((a.n_out + (int64_t)FEAT - 1) / FEAT);
   DWM_CHECK_ARG(tiles < (1ll << 30), "m=%d rows by %d columns are too many tiles", a.m, a.n_out);
-  CUtensorMap tm_x, tm_w;
+  CUtensorMap tm_x, tm_w, tm_out, tm_res;
   int rc = encode_tmap_2d(&tm_x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, x, (uint64_t)a.k, (uint64_t)a.m,
                           (uint64_t)ldx * 2, BK, HALF, CU_TENSOR_MAP_SWIZZLE_128B);
   if (rc) return rc;
   rc = encode_tmap_2d(&tm_w, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, w, (uint64_t)a.k, (uint64_t)n,
                       (uint64_t)ldw * 2, BK, HALF, CU_TENSOR_MAP_SWIZZLE_128B);
   if (rc) return rc;
-  rc = set_smem_limit(reinterpret_cast<const void*>(dense_pair_kernel<EPI, VEC>), ALLOC,
+  auto box_map = [&](CUtensorMap* map, const void* p, int64_t ld, int f32) {
+    return encode_tmap_2d(
+        map, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, p,
+        (uint64_t)a.n_out, (uint64_t)a.m, (uint64_t)ld * (f32 ? 4 : 2), BOX, BOX,
+        f32 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
+  };
+  tm_out = tm_res = tm_x;  // (unused without VEC, without RES)
+  if (VEC && (rc = box_map(&tm_out, a.out, a.ldo, a.out_f32))) return rc;
+  if (RES && (rc = box_map(&tm_res, a.residual, a.ldr, a.res_f32))) return rc;
+  rc = set_smem_limit(reinterpret_cast<const void*>(dense_pair_kernel<EPI, VEC, RES>), L::ALLOC,
                       "dense pair smem attribute");
   if (rc) return rc;
   return check_cuda(
-      overlap_launch(dense_pair_kernel<EPI, VEC>,
+      overlap_launch(dense_pair_kernel<EPI, VEC, RES>,
                      dim3(2 * (unsigned)std::min<int64_t>(tiles, resident_clusters(2))),
-                     dim3(THREADS), ALLOC, 2, stream, tm_x, tm_w, a),
-                    "dense_matmul launch");
+                     dim3(THREADS), L::ALLOC, 2, stream, tm_x, tm_w, tm_out, tm_res, a),
+      "dense_matmul launch");
 }
 
 }  // namespace pair
@@ -900,8 +1058,10 @@ int run_epi(const void* x, int64_t ldx, const void* w, int64_t ldw, int n, const
   }
   const float t_pair = 6.5f + waves(ptiles, 2) * std::max(0.27f * (float)kt, 4.0f);
   if (t_pair < best)
-    return a.out_vec ? pair::launch<EPI, true>(x, ldx, w, ldw, n, a, stream)
-                     : pair::launch<EPI, false>(x, ldx, w, ldw, n, a, stream);
+    return !a.out_vec || (a.residual && !a.res_vec)
+               ? pair::launch<EPI, false, false>(x, ldx, w, ldw, n, a, stream)
+           : a.residual ? pair::launch<EPI, true, true>(x, ldx, w, ldw, n, a, stream)
+                        : pair::launch<EPI, true, false>(x, ldx, w, ldw, n, a, stream);
   if (bt == 16) return launch_split<16, EPI>(x, ldx, w, ldw, n, split, a, stream);
   if (bt == 32) return launch_split<32, EPI>(x, ldx, w, ldw, n, split, a, stream);
   if (bt == 64) return launch_split<64, EPI>(x, ldx, w, ldw, n, split, a, stream);
