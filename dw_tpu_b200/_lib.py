@@ -120,6 +120,9 @@ SIGNATURES = {
     "dwm_ep_destroy": ([_P], _I),
 }
 
+# Codes of the floating types that the operators around the expert layer take.
+FLOATS = {torch.bfloat16: BF16, torch.float32: F32}
+
 _lib = None
 _lock = threading.Lock()
 

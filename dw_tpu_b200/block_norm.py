@@ -5,7 +5,10 @@ from __future__ import annotations
 
 import torch
 
-from . import ops
+from . import _lib as L
+from .ops import code_of
+
+_NORMS = {"rms": L.NORM_RMS, "layer": L.NORM_LAYER}
 
 
 def pre_norm(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *,
@@ -16,8 +19,9 @@ def pre_norm(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = 
     be ``x``) is written and returned if given. Inference only: no gradient."""
     if weight is None:
         raise ValueError("pre_norm needs a weight")
-    return ops.block_norm_out(x, out, weight=weight, bias=bias, eps=eps, kind=kind,
-                              h_dtype=out_dtype)[1]
+    return L.bind().block_norm(x, None, None, None, None, 1.0, 1.0, weight, bias, eps,
+                               code_of(_NORMS, kind, "norm kind"), None, out,
+                               code_of(L.FLOATS, out_dtype, "out_dtype"), True, None)[1]
 
 
 def post_norm(y: torch.Tensor, residual: torch.Tensor, *,
@@ -40,7 +44,9 @@ def post_norm(y: torch.Tensor, residual: torch.Tensor, *,
     Inference only: no gradient."""
     if next_weight is None and (out is not None or next_bias is not None):
         raise ValueError("out and next_bias need next_weight")
-    return ops.block_norm_out(residual, out, weight=next_weight, bias=next_bias, y=y,
-                              r_out=residual_out, norm_weight=norm_weight, norm_bias=norm_bias,
-                              gate=gate, scale=scale, residual_scale=residual_scale, eps=eps,
-                              kind=kind, h_dtype=out_dtype)
+    if y is None:
+        raise ValueError("post_norm needs y")
+    return L.bind().block_norm(residual, y, norm_weight, norm_bias, gate, scale, residual_scale,
+                               next_weight, next_bias, eps, code_of(_NORMS, kind, "norm kind"),
+                               residual_out, out, code_of(L.FLOATS, out_dtype, "out_dtype"),
+                               next_weight is not None, None)

@@ -15,7 +15,9 @@
 // are closer than the f32 error (a few tokens in a hundred for random logits),
 // the groups or the picks in question are compared in 64 bits; a token that
 // this does not settle is done again in 64 bits by the whole warp (8-12 us, which
-// one token of 1024 would make the time of all). Bound: instruction issue.
+// one token of 1024 would make the time of all). Bound: instruction issue; a
+// single token takes 6.3 us of dependent instructions, 32771 tokens of 160
+// experts 21 us where their bytes take 3.4 (in 64 bits throughout: 83).
 #include <algorithm>
 
 #include "common.cuh"
@@ -631,7 +633,9 @@ extern "C" int dwm_route_grouped_topk(const void* logits, int logits_dtype, int6
   a.w32 = topk_weights_f32;
   a.w16 = static_cast<uint16_t*>(topk_weights_bf16);
   // Lanes: a power of two of groups, each of as many lanes as leave at most 32
-  // experts a lane (64 where the warp has no more lanes), 8 a token at least.
+  // experts a lane (64 where the warp has no more lanes), 8 a token at least. (All
+  // 32 lanes a token for small batches were no faster: the shorter runs save what
+  // the longer reductions cost.)
   int groups_log = 0;
   while ((1 << groups_log) < num_groups) ++groups_log;
   a.lg_log = 0;

@@ -6,7 +6,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib as L
-from . import ops
+from .ops import code_of
 
 _ACTS = {None: L.ACT_NONE, "silu": L.ACT_SILU, "gelu": L.ACT_GELU,
          "gelu_tanh": L.ACT_GELU_TANH, "swiglu": L.ACT_SWIGLU,
@@ -36,6 +36,5 @@ def dense_matmul(x: torch.Tensor, w: torch.Tensor, *, bias: torch.Tensor | None 
         raise ValueError("swiglu_clamp needs act_limit")
     if out is not None and out_dtype is not None and out.dtype != out_dtype:
         raise ValueError(f"out is {out.dtype}, out_dtype {out_dtype}")
-    return ops.dense_matmul_out(x, w, out, bias=bias, act=code, act_limit=act_limit or 0.0,
-                                residual=residual, residual_scale=residual_scale,
-                                out_dtype=out_dtype or torch.bfloat16)
+    return L.bind().dense_matmul(x, w, bias, code, act_limit or 0.0, residual, residual_scale, out,
+                                 code_of(L.FLOATS, out_dtype or torch.bfloat16, "out_dtype"), None)

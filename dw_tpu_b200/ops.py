@@ -413,10 +413,10 @@ def e8m0_decode_out(codes, out, stream=None):
 
 _GROUP_SCORES = {"max": L.GROUP_MAX, "top2": L.GROUP_TOP2}
 _NORMS = {"rms": L.NORM_RMS, "layer": L.NORM_LAYER}
-_FLOATS = {torch.bfloat16: L.BF16, torch.float32: L.F32}
 
 
-def _code(table, key, what):
+def code_of(table, key, what):
+    """table[key], or ValueError naming ``what``."""
     try:
         return table[key]
     except (KeyError, TypeError):
@@ -433,8 +433,8 @@ def route_grouped_topk_out(logits, top_k, num_groups, topk_groups, ids_out, w32_
     if ids_out is None:
         raise ValueError("ids_out is required")
     L.bind().route_grouped_topk(
-        logits, top_k, num_groups, topk_groups, _code(_SCORING, scoring_fn, "scoring_fn"),
-        _code(_GROUP_SCORES, group_score, "group_score"), int(bool(renormalize)), routed_scale,
+        logits, top_k, num_groups, topk_groups, code_of(_SCORING, scoring_fn, "scoring_fn"),
+        code_of(_GROUP_SCORES, group_score, "group_score"), int(bool(renormalize)), routed_scale,
         bias, -1 if num_valid_tokens is None else max(0, num_valid_tokens), L.F32, ids_out,
         w32_out, w16_out, stream)
 
@@ -443,9 +443,9 @@ def route_grouped_topk_new(logits, top_k, num_groups, topk_groups, dtype, scorin
                            renormalize, routed_scale, bias, num_valid_tokens):
     """The same into new tensors: (weights of ``dtype``, bf16 or f32, and ids)."""
     return L.bind().route_grouped_topk(
-        logits, top_k, num_groups, topk_groups, _code(_SCORING, scoring_fn, "scoring_fn"),
-        _code(_GROUP_SCORES, group_score, "group_score"), int(bool(renormalize)), routed_scale,
-        bias, -1 if num_valid_tokens is None else max(0, num_valid_tokens), _FLOATS[dtype], None,
+        logits, top_k, num_groups, topk_groups, code_of(_SCORING, scoring_fn, "scoring_fn"),
+        code_of(_GROUP_SCORES, group_score, "group_score"), int(bool(renormalize)), routed_scale,
+        bias, -1 if num_valid_tokens is None else max(0, num_valid_tokens), L.FLOATS[dtype], None,
         None, None, None)
 
 
@@ -456,7 +456,7 @@ def dense_matmul_out(x, w, out, *, bias=None, act=L.ACT_NONE, act_limit=0.0, res
     SwiGLU), bf16 or f32. Rows may be strided; ``out`` may be ``residual``, or
     None: a new tensor of ``out_dtype``. Returns out."""
     return L.bind().dense_matmul(x, w, bias, act, act_limit, residual, residual_scale, out,
-                                 _code(_FLOATS, out_dtype, "out_dtype"), stream)
+                                 code_of(L.FLOATS, out_dtype, "out_dtype"), stream)
 
 
 def block_norm_out(residual, h_out=None, *, weight=None, bias=None, y=None, r_out=None,
@@ -471,7 +471,7 @@ def block_norm_out(residual, h_out=None, *, weight=None, bias=None, y=None, r_ou
     tensor (h_out of ``h_dtype``). Returns (r_out, h_out)."""
     return L.bind().block_norm(
         residual, y, norm_weight, norm_bias, gate, scale, residual_scale, weight, bias, eps,
-        _code(_NORMS, kind, "norm kind"), r_out, h_out, _code(_FLOATS, h_dtype, "out_dtype"),
+        code_of(_NORMS, kind, "norm kind"), r_out, h_out, code_of(L.FLOATS, h_dtype, "out_dtype"),
         weight is not None, stream)
 
 
