@@ -124,8 +124,14 @@ int size32(int64_t v, const char* name) {
   TORCH_CHECK_VALUE(v <= INT32_MAX, name, "=", v, " is too large");
   return (int)v;
 }
-Tensor empty(int64_t m, int64_t n, at::ScalarType dt, c10::Device dev) {
+// A new output, of the current stream's memory: a call on a stream of its own
+// brings its outputs.
+Tensor fresh(int64_t m, int64_t n, at::ScalarType dt, c10::Device dev, PyObject* stream) {
+  TORCH_CHECK_VALUE(stream == Py_None, "a call with a stream of its own needs its outputs given");
   return at::empty({m, n}, at::TensorOptions().dtype(dt).device(dev));
+}
+Tensor fresh(int64_t m, int64_t n, int code, c10::Device dev, PyObject* stream) {
+  return fresh(m, n, type_of(code), dev, stream);
 }
 
 // ---- the calls -------------------------------------------------------------
@@ -165,7 +171,7 @@ PyObject* dense_matmul(PyObject*, PyObject* const* v, Py_ssize_t n_args) {
     same_device(dev, *out, "out");
     no_grad(out);
   } else {
-    out = empty(m, n_out, type_of(int32(v[8], "out_dtype")), dev);
+    out = fresh(m, n_out, int32(v[8], "out_dtype"), dev, v[9]);
   }
   const int64_t ldo = rows(*out, "out", m, n_out);
   check_rc(g_dense(x.data_ptr(), ldx, w.data_ptr(), ldw, m, n, k, data(bias),
@@ -203,9 +209,9 @@ PyObject* route_grouped_topk(PyObject*, PyObject* const* v, Py_ssize_t n_args) {
   const bool own = !ids;
   if (own) {
     TORCH_CHECK_VALUE(top_k >= 1 && top_k <= 32, "top_k=", top_k, " must be in [1, 32]");
-    ids = empty(t, top_k, at::kInt, dev);
-    (int32(v[10], "dtype") == DWM_F32 ? w32 : w16) =
-        empty(t, top_k, type_of(int32(v[10], "dtype")), dev);
+    const int type = int32(v[10], "dtype");
+    ids = fresh(t, top_k, at::kInt, dev, v[14]);
+    (type == DWM_F32 ? w32 : w16) = fresh(t, top_k, type, dev, v[14]);
   } else {
     auto given = [&](const Opt& o, at::ScalarType type, const char* name) {
       if (!o) return;
@@ -293,7 +299,7 @@ PyObject* block_norm(PyObject*, PyObject* const* v, Py_ssize_t n_args) {
       TORCH_CHECK_VALUE(r_out->scalar_type() == res.scalar_type(),
                         "r_out must have residual's dtype");
     } else {
-      r_out = empty(t, h, res.scalar_type(), dev);
+      r_out = fresh(t, h, res_dt, dev, v[15]);
     }
     ldr = rows(*r_out, "r_out", t, h);
   }
@@ -303,7 +309,7 @@ PyObject* block_norm(PyObject*, PyObject* const* v, Py_ssize_t n_args) {
       same_device(dev, *h_out, "h_out");
       no_grad(h_out);
     } else {
-      h_out = empty(t, h, type_of(int32(v[13], "h_dtype")), dev);
+      h_out = fresh(t, h, int32(v[13], "h_dtype"), dev, v[15]);
     }
     ldh = rows(*h_out, "h_out", t, h);
     h_dt = dtype_of(*h_out, "h_out");

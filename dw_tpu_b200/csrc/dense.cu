@@ -169,8 +169,9 @@ __device__ __forceinline__ void activate(const Args& a, float (&z)[N], float (&u
     if (a.act == DWM_ACT_SWIGLU_CLAMP) {
 #pragma unroll
       for (int q = 0; q < N; ++q) {
-        z[q] = fminf(z[q], a.limit);
-        u[q] = fminf(fmaxf(u[q], -a.limit), a.limit);
+        // (A NaN stays one.)
+        z[q] = z[q] > a.limit ? a.limit : z[q];
+        u[q] = u[q] > a.limit ? a.limit : u[q] < -a.limit ? -a.limit : u[q];
       }
     }
     if (a.out_f32) {
@@ -745,13 +746,16 @@ __global__ void __launch_bounds__(THREADS, 1)
           bias[j] = ld1(a.bias, c + (EPI == GLU && lane >= 16 ? a.n_out : 0), a.bias_f32);
         }
       }
-      if (!__all_sync(0xffffffffu, mbar_wait<64>(&acc_full[slot], ph, abort_flag, a.status))) {
-        // The residual's copies in flight land before the exit.
+      // The residual's copies in flight, of `left` steps, land before the exit.
+      auto land = [&](int left) {
         if (RES && lane == 0)
-          for (int i = 0; i < min(steps, res_ring); ++i) {
+          for (int i = 0; i < min(left, res_ring); ++i) {
             const int at = (res_buf + i) % res_ring;
             mbar_wait(&res_full[warp * 4 + at], (res_ph >> at) & 1u, nullptr, a.status);
           }
+      };
+      if (!__all_sync(0xffffffffu, mbar_wait<64>(&acc_full[slot], ph, abort_flag, a.status))) {
+        land(steps);
         break;
       }
       tc_fence_after();
@@ -784,9 +788,14 @@ __global__ void __launch_bounds__(THREADS, 1)
           }
           activate<EPI>(a, z, u);
           if (RES) {
-            if ((b & 1) == 0)
-              res_ok &= mbar_wait(&res_full[warp * 4 + res_buf], (res_ph >> res_buf) & 1u,
-                                  abort_flag, a.status);
+            if ((b & 1) == 0 &&
+                !__all_sync(0xffffffffu, mbar_wait(&res_full[warp * 4 + res_buf],
+                                                   (res_ph >> res_buf) & 1u, abort_flag,
+                                                   a.status))) {
+              land(steps - (b >> 1));
+              res_ok = false;
+              break;
+            }
             const uint32_t from = res_at + (uint32_t)(res_buf * res_step);
             float r[16];
             if (a.res_f32) {
@@ -888,6 +897,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           __syncwarp();
         }
       }
+      if (!res_ok) break;
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive_remote(acc_empty_0 + (uint32_t)(slot * 8));
@@ -1091,6 +1101,8 @@ extern "C" int dwm_dense_matmul(const void* x, int64_t ldx, const void* w, int64
   const bool glu = act == DWM_ACT_SWIGLU || act == DWM_ACT_SWIGLU_CLAMP;
   DWM_CHECK_ARG(m >= 0 && n >= 1 && k >= 8, "bad shape m=%d n=%d k=%d", m, n, k);
   DWM_CHECK_ARG(k % 8 == 0, "k=%d must be a multiple of 8", k);
+  // (Coordinates of whole tiles are 32-bit numbers.)
+  DWM_CHECK_ARG(std::max({m, n, k}) <= INT32_MAX - 1024, "m=%d n=%d k=%d are too large", m, n, k);
   DWM_CHECK_ARG(act >= DWM_ACT_NONE && act <= DWM_ACT_GELU_TANH, "unknown activation %d", act);
   DWM_CHECK_ARG(!glu || n % 2 == 0, "SwiGLU needs [gate | up] halves: n=%d is odd", n);
   DWM_CHECK_ARG(act != DWM_ACT_SWIGLU_CLAMP || act_limit > 0.0f, "act_limit must be positive");

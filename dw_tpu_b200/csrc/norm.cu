@@ -309,11 +309,11 @@ __device__ __forceinline__ void normalise(F2 (&u)[pairs(VEC, CPT)], const Cols<V
 // One row: both norms, gate, residual, stores. y, res, gate and vec (a weight
 // or bias) are functions that hand their loaded elements on: from registers
 // where the caller has loaded them ahead, or from where they lie. r_out and
-// h_out point to the row. read_done() runs once every thread has the row's
-// elements.
+// h_out point to the row. slot: of the sums of n1 (n2's have 0 and 1). read_done()
+// runs once every thread has the row's elements.
 template <int VEC, int CPT, int T, int YD, int RD, int WD, class Y, class Res, class Gate,
           class Vec, class Done>
-__device__ __forceinline__ void do_row(const Args& a, const Group& g, uint8_t* r_out,
+__device__ __forceinline__ void do_row(const Args& a, const Group& g, int slot, uint8_t* r_out,
                                        uint8_t* h_out, float inv_h,
                                        const Cols<VEC, CPT, T>& cols, float gate_tok, const Y& y,
                                        const Res& res, const Gate& gate, const Vec& vec,
@@ -337,7 +337,7 @@ __device__ __forceinline__ void do_row(const Args& a, const Group& g, uint8_t* r
     res([&](const RawR& x) { x.into(v, a.res_f32, [](F2, F2 e) { return e; }); });
   }
   if (a.h_out) {
-    normalise<VEC, CPT, T, WD>(v, cols, a, g, 2, inv_h, vec, W1, B1, read_done);
+    normalise<VEC, CPT, T, WD>(v, cols, a, g, slot, inv_h, vec, W1, B1, read_done);
     store<VEC, CPT, T>(h_out, a.h_f32 != 0, cols, v);
   } else {
     g.sync();
@@ -399,7 +399,7 @@ __global__ void __launch_bounds__(max_threads<VEC, CPT>(false)) block_norm_kerne
     g.sync();
   }
   do_row<VEC, CPT, T, YD, RD, WD>(
-      a, g, row_ptr(a.r_out, row, a.ldr, re), row_ptr(a.h_out, row, a.ldh, a.h_f32 ? 4 : 2),
+      a, g, 2, row_ptr(a.r_out, row, a.ldr, re), row_ptr(a.h_out, row, a.ldh, a.h_f32 ? 4 : 2),
       1.0f / (float)a.h, cols, tok, [&](auto f) { f(y); }, [&](auto f) { f(res); },
       [&](auto f) {
         if (!AHEAD) gate.load(pg, cols, a.y_f32);
@@ -506,7 +506,7 @@ __global__ void __launch_bounds__(max_threads<VEC, CPT>(true), 1)
     }
     __syncthreads();
   }
-  int s = 0;
+  int s = 0, slot = 2;
   uint32_t ph = 0;
   uint8_t* r_out = row_ptr(a.r_out, first, a.ldr, re);
   uint8_t* h_out = row_ptr(a.h_out, first, a.ldh, he);
@@ -521,7 +521,7 @@ __global__ void __launch_bounds__(max_threads<VEC, CPT>(true), 1)
       return VEC == 8 ? 0u : (uint32_t)reinterpret_cast<uint64_t>(row_ptr(p, row, ld, es)) & 15u;
     };
     do_row<VEC, CPT, T, YD, RD, WD>(
-        a, g, r_out, h_out, inv_h, cols, tok,
+        a, g, slot, r_out, h_out, inv_h, cols, tok,
         [&](auto f) {
           Raw<VEC, CPT, T, YD> x;
           x.load_s(at + lead(a.y, a.ldy, ye), cols, a.y_f32);
@@ -559,6 +559,9 @@ __global__ void __launch_bounds__(max_threads<VEC, CPT>(true), 1)
         });
     r_out += step * a.ldr * re;
     h_out += step * a.ldh * he;
+    // An RMS norm without n2 has one barrier a row: a warp that is ahead must not
+    // write its next sum where another still reads this row's.
+    if (!a.inner) slot ^= 2;
     if (++s == a.stages) { s = 0; ph ^= 1; }
   }
   // A copy that a wait gave up on lands before the exit.
@@ -682,6 +685,12 @@ extern "C" int dwm_block_norm(const void* y, int y_dtype, int64_t ldy, const voi
                   "without y there is only h = norm(residual)");
   }
   DWM_CHECK_ARG(!h_out || w1, "the norm before the next block needs its weight");
+  auto aligned = [&](const void* p, int d) { return reinterpret_cast<uintptr_t>(p) % es(d) == 0; };
+  DWM_CHECK_ARG((!y || aligned(y, y_dtype)) && (!gate || aligned(gate, y_dtype)) &&
+                    aligned(residual, residual_dtype) && aligned(r_out, residual_dtype) &&
+                    aligned(h_out, h_dtype) && aligned(w1, w_dtype) && aligned(b1, w_dtype) &&
+                    aligned(w2, w_dtype) && aligned(b2, w_dtype),
+                "misaligned pointer");
   DWM_CHECK_ARG((!y || ldy >= h || t == 1) && (ldres >= h || t == 1) &&
                     (!r_out || ldr >= h || t == 1) && (!h_out || ldh >= h || t == 1) &&
                     (gate_mode != DWM_GATE_FULL || ldg >= h || t == 1) &&

@@ -614,6 +614,21 @@ extern "C" int dwm_route_grouped_topk(const void* logits, int logits_dtype, int6
   DWM_CHECK_ARG(t <= 1 || ld_logits >= e, "ld_logits is shorter than a row");
   DWM_CHECK_ARG(t == 0 || (logits && topk_ids), "NULL pointer");
   if (t == 0) return DWM_OK;
+  const int es = logits_dtype == DWM_F32 ? 4 : 2;
+  auto misaligned = [](const void* p, int size) { return reinterpret_cast<uintptr_t>(p) % size; };
+  DWM_CHECK_ARG(!misaligned(logits, es) && !misaligned(bias, 4) && !misaligned(topk_ids, 4) &&
+                    !misaligned(topk_weights_f32, 4) && !misaligned(topk_weights_bf16, 2),
+                "misaligned pointer");
+  // Tokens are written while others are read.
+  const int64_t picks = (int64_t)t * top_k;
+  const RowSpan outs[3] = {row_span(topk_ids, 1, picks, picks, 4),
+                           row_span(topk_weights_f32, 1, picks, picks, 4),
+                           row_span(topk_weights_bf16, 1, picks, picks, 2)};
+  for (int i = 0; i < 3; ++i)
+    DWM_CHECK_ARG(!rows_overlap(outs[i], row_span(logits, t, e, ld_logits, es)) &&
+                      !rows_overlap(outs[i], row_span(bias, 1, e, e, 4)) &&
+                      !rows_overlap(outs[i], outs[(i + 1) % 3]),
+                  "an output overlaps an input or another output");
   route_group::Args a;
   a.logits = logits;
   a.ld = ld_logits;
@@ -644,7 +659,6 @@ extern "C" int dwm_route_grouped_topk(const void* logits, int logits_dtype, int6
     ++a.lg_log;
   a.lpt_log = groups_log + a.lg_log;
   a.run = (a.per + (1 << a.lg_log) - 1) >> a.lg_log;
-  const int es = logits_dtype == DWM_F32 ? 4 : 2;
   a.vec = a.per % a.run == 0 && a.run * es % 16 == 0 && (t == 1 || ld_logits * es % 16 == 0) &&
           (reinterpret_cast<uintptr_t>(logits) & 15) == 0;
   cudaStream_t s = static_cast<cudaStream_t>(stream);

@@ -84,7 +84,9 @@ class MoEBlock:
                                    group_score=self.group_score, renormalize=layer.renormalize,
                                    routed_scale=self.routed_scale, bias=self.router_bias,
                                    num_valid_tokens=num_valid_tokens)
-        y = layer.experts(h, ids, w16, self.routed[:t])
+        y = self.routed[:t]
+        if t:
+            layer.experts(h, ids, w16, y)
         if self.shared_w13 is not None:
             clamp = layer.act_limit > 0.0
             s1 = dense_matmul(h, self.shared_w13, act="swiglu_clamp" if clamp else "swiglu",

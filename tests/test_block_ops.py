@@ -143,3 +143,37 @@ def test_python_refusals_without_gpu():
         dw.post_norm(x, x, out=x)
     with pytest.raises(ValueError, match="gradient"):
         dw.route_grouped_topk(x.float().requires_grad_(), 4, 8, 4)
+
+
+@pytest.mark.parametrize("kw,message", [
+    (dict(m=2 ** 31 - 100), "too large"), (dict(n=2 ** 31 - 100), "too large"),
+    (dict(k=2 ** 31 - 104), "too large"),
+])
+def test_dense_sizes_past_the_tiles(lib, kw, message):
+    from dw_tpu_b200 import _lib
+    assert _dense(lib, **kw) == -1
+    assert message in _lib.last_error()
+
+
+@pytest.mark.parametrize("kw,message", [
+    (dict(logits=FAKE + 2), "misaligned"), (dict(ids=2 * FAKE + 2), "misaligned"),
+    (dict(bias=FAKE + 1), "misaligned"), (dict(w32=FAKE + 2), "misaligned"),
+    (dict(w16=FAKE + 1), "misaligned"), (dict(ids=FAKE + 16), "overlaps"),
+    (dict(w16=2 * FAKE + 56), "overlaps"), (dict(w32=2 * FAKE), "overlaps"),
+    (dict(bias=2 * FAKE + 60), "overlaps"),
+])
+def test_route_memory_refusals(lib, kw, message):
+    from dw_tpu_b200 import _lib
+    assert _route(lib, **kw) == -1
+    assert message in _lib.last_error()
+
+
+@pytest.mark.parametrize("kw", [
+    dict(y=MB + 1), dict(res=2 * MB + 1), dict(rdt=1, res=2 * MB + 2), dict(w1=4 * MB + 1),
+    dict(w2=3 * MB + 1), dict(b1=7 * MB + 1), dict(b2=7 * MB + 1), dict(r=5 * MB + 1),
+    dict(ho=6 * MB + 1), dict(hdt=1, ho=6 * MB + 2), dict(gate=7 * MB + 1, gmode=2),
+])
+def test_norm_misaligned(lib, kw):
+    from dw_tpu_b200 import _lib
+    assert _norm(lib, **kw) == -1
+    assert "misaligned" in _lib.last_error()

@@ -174,6 +174,44 @@ def test_dense_rows_are_their_own(dw, m):
     assert bool(got[0].isinf().all()) and bool(got[m + 1].isinf().all())
 
 
+@pytest.mark.parametrize("n,pad,off", [(1544, 0, 0), (1544, 24, 8), (1546, 0, 0), (1544, 3, 1)])
+@pytest.mark.parametrize("res,out_dtype", [(None, BF), (BF, BF), (F32, BF), (BF, F32), (F32, F32)])
+def test_dense_many_rows(dw, n, pad, off, res, out_dtype):
+    """Rows for several 256-row tiles (the last of one row), every epilogue with a
+    residual of either type, in rows that start on 16 bytes and that do not;
+    what lies between the rows stays as it was."""
+    m, k = 2049, 1032
+    x, w, b = _randn(1, m, k), _randn(2, n, k, scale=k ** -0.5), _randn(3, n, scale=0.3)
+    for act in (None, "gelu_tanh", "swiglu_clamp"):
+        cols = n // 2 if act == "swiglu_clamp" else n
+        r = None
+        if res is not None:
+            r = torch.full((m, cols + pad + off), math.nan, dtype=res, device="cuda")
+            r[:, off:off + cols] = _randn(4, m, cols, dtype=res)
+            r = r[:, off:off + cols]
+        buf = torch.full((m + 1, cols + pad + off), -7.0, dtype=out_dtype, device="cuda")
+        out = buf[:m, off:off + cols]
+        args = dict(bias=b, act=act, act_limit=LIMIT, residual_scale=0.75)
+        ref, tol = _dense_ref(x, w, b, act, r, 0.75, out_dtype)
+        got = dw.dense_matmul(x, w, residual=r, out=out, **args)
+        assert got is out
+        _close(out, ref, tol, f"{act}")
+        if res == out_dtype:  # in place
+            again = r.clone() if pad == 0 else r
+            dw.dense_matmul(x, w, residual=again, out=again, **args)
+            assert torch.equal(again, out)
+        out.fill_(-7.0)
+        assert bool((buf == -7.0).all())
+
+
+@pytest.mark.parametrize("m", [3, 700])
+def test_dense_clamp_keeps_nan(dw, m):
+    x, w = _randn(1, m, 128), _randn(2, 512, 128)
+    x[1, 7] = math.nan
+    got = dw.dense_matmul(x, w, act="swiglu_clamp", act_limit=1.0)
+    assert bool(got[1].isnan().all()) and not bool(got[0].isnan().any())
+
+
 def test_dense_empty(dw):
     assert dw.dense_matmul(_randn(1, 0, 64), _randn(2, 32, 64)).shape == (0, 32)
 
@@ -491,6 +529,46 @@ def test_post_norm_forms_and_types(dw, gate, inner, nxt, h):
             assert hn is None
 
 
+@pytest.mark.parametrize("t,h", [(5000, 100), (4999, 512), (2500, 333), (1301, 4096), (1300, 2000),
+                                 (700, 5003), (601, 8192), (401, 9001), (307, 16384)])
+@pytest.mark.parametrize("gate", ["none", "token", "channel", "full"])
+def test_norm_many_rows(dw, t, h, gate):
+    """More rows than the CTAs take at once, in every form; again in place, and
+    several times over: the same bits."""
+    for i, (ydt, rdt, wdt, hdt) in enumerate([(BF, BF, BF, BF), (BF, F32, F32, BF),
+                                              (F32, BF, BF, F32)]):
+        kind = ("rms", "layer")[(i + h) % 2]
+        y, x = _randn(i, t, h, mean=0.2, dtype=ydt), _randn(i + 9, t, h, scale=2.0, dtype=rdt)
+        w, b = _randn(3, h, mean=1.0, dtype=wdt), _randn(4, h, dtype=wdt)
+        g = _gate(gate, t, h, ydt)
+        for inner, nxt in ((True, True), (False, True), (True, False)):
+            args = dict(norm_weight=w if inner else None, gate=g, scale=0.75, residual_scale=1.5,
+                        next_weight=w if nxt else None, next_bias=b if nxt else None, eps=EPS,
+                        kind=kind, out_dtype=hdt)
+            r, hn = dw.post_norm(y, x, **args)
+            refs = _post_ref(y, x, w if inner else None, None, g, 0.75, 1.5, w if nxt else None,
+                             b, kind, rdt, hdt)
+            _close(r, *refs[0], f"r {kind} {inner} {nxt}")
+            if nxt:
+                _close(hn, *refs[1], f"h {kind} {inner}")
+            x2, y2 = x.clone(), y.clone()
+            r2, h2 = dw.post_norm(y2, x2, residual_out=x2, out=y2 if nxt and ydt == hdt else None,
+                                  **args)
+            assert torch.equal(r2, r) and (hn is None or torch.equal(h2, hn))
+
+
+@pytest.mark.parametrize("t,h", [(8192, 2048), (5000, 104), (1500, 5003)])
+def test_pre_norm_many_rows_same_bits(dw, t, h):
+    """An RMS norm alone has one sum a row, whose slots the next row reuses."""
+    x, w = _randn(1, t, h), _randn(2, h, mean=1.0)
+    ref, tol = _post_ref(torch.zeros_like(x), x, None, None, None, 0.0, 1.0, w, None, "rms", F32,
+                         BF)[1]
+    base = dw.pre_norm(x, w, eps=EPS)
+    _close(base, ref, tol)
+    for _ in range(20):
+        assert torch.equal(dw.pre_norm(x, w, eps=EPS), base)
+
+
 @pytest.mark.parametrize("h,pad,off", [(512, 8, 8), (512, 3, 1), (333, 5, 2), (4096, 16, 8)])
 def test_norm_strides_and_untouched_surroundings(dw, h, pad, off):
     t = 11
@@ -607,3 +685,46 @@ def test_refusals_on_the_gpu(dw):
                 lambda: dw.route_grouped_topk(x, 4, 8, 2, bias=torch.zeros(63, device="cuda"))):
         with pytest.raises(ValueError):
             bad()
+
+
+def test_a_stream_of_its_own_needs_outputs(dw):
+    """The tensors that a call allocates belong to the current stream."""
+    from dw_tpu_b200 import ops
+    x, w = _randn(1, 64, 256), _randn(2, 128, 256)
+    base, s = dw.dense_matmul(x, w), torch.cuda.Stream()
+    with pytest.raises(ValueError, match="outputs given"):
+        ops.dense_matmul_out(x, w, None, stream=s.cuda_stream)
+    with pytest.raises(ValueError, match="outputs given"):
+        ops.block_norm_out(x, weight=w[0], stream=s.cuda_stream)
+    with pytest.raises(ValueError, match="outputs given"):
+        ops.block_norm_out(x, y=x, norm_weight=w[0], stream=s.cuda_stream)
+    out = torch.empty_like(base)
+    s.wait_stream(torch.cuda.current_stream())
+    ops.dense_matmul_out(x, w, out, stream=s.cuda_stream)
+    s.synchronize()
+    assert torch.equal(out, base)
+
+
+def test_calls_on_two_streams_at_once(dw):
+    """Each stream's chain of calls overlaps its own launches; the other's run
+    between them."""
+    x, w, r = _randn(1, 1500, 1024), _randn(2, 2048, 1024, scale=0.03), _randn(3, 1500, 1024)
+    nw = _randn(4, 1024, mean=1.0)
+
+    def chain(v):
+        for _ in range(4):
+            a = dw.dense_matmul(v, w, act="swiglu")
+            v, hn = dw.post_norm(a, v, norm_weight=nw, next_weight=nw)
+            ids = dw.route_grouped_topk(hn[:, :256], 8, 8, 4)[1]
+        return v, hn, ids
+
+    base = [[t.clone() for t in chain(v)] for v in (x, r)]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], [None, None]
+    for _ in range(3):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i] = chain((x, r)[i])
+    torch.cuda.synchronize()
+    for b, g in zip(base, got):
+        assert all(torch.equal(p, q) for p, q in zip(b, g))

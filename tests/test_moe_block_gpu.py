@@ -182,3 +182,9 @@ def test_block_refusals(dw):
         dw.MoEBlock(layer, router, nw, shared_w2=block.shared_w2)
     with pytest.raises(ValueError, match="shared_w13"):
         dw.MoEBlock(layer, router, nw, shared_w13=block.shared_w2, shared_w2=block.shared_w13)
+
+
+def test_block_without_tokens(dw):
+    block, _ = _block(dw, 8)
+    r, hn = block(_randn(1, 0, H))
+    assert r.shape == hn.shape == (0, H)
