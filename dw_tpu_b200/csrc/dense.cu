@@ -1034,17 +1034,167 @@ int launch(const void* x, int64_t ldx, const void* w, int64_t ldw, int n, const 
 
 }  // namespace pair
 
+// ---------------------------------------------------------------------------
+// Few-rows kernel (a decode step of at most 16 tokens). 16 rows of w (SwiGLU: 8
+// gate rows and the 8 up rows of the same features) are operand A of
+// mma.m16n8k16, up to 8 NT rows of x operand B, both straight from global memory
+// into registers: lane t of a quad takes 8 consecutive k of a row in one 16-byte
+// load and gives its halves to two products, which add the same k in both
+// operands, in another order than they lie. A CTA's warps take every eighth of
+// 64 k, the CTAs of a cluster (when w has few rows) every so many of those; the
+// partial sums are added in warp and in CTA order.
+//
+// Bound: the stream of w, and for small w the launch and a memory latency,
+// which a kernel without TMA, mbarriers and TMEM to set up gets to sooner.
+// ---------------------------------------------------------------------------
+namespace few {
+
+constexpr int WARPS = 8, THREADS = 32 * WARPS;
+
+__device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                    uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+      "{%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// U: 64-k steps whose loads are issued together. grid (w tiles x split).
+template <int NT, int U, int EPI>
+__global__ void __launch_bounds__(THREADS, 2)
+    dense_few_kernel(const uint16_t* x, int64_t ldx, const uint16_t* w,
+                     int64_t ldw, int split, const Args a) {
+  constexpr int FEAT = EPI == GLU ? 8 : 16;  // output columns of a tile
+  constexpr int SUMS = 8 * NT * 16;          // [row of x][row of the tile]
+  __shared__ float part[WARPS][SUMS];
+  __shared__ float recv[MAX_CLUSTER][SUMS];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int gid = lane >> 2, t = lane & 3;
+  const int rank = blockIdx.x % split;
+  const int col0 = blockIdx.x / split * FEAT;
+  if (split > 1) cluster_arrive();
+  // Rows past the last repeat it; their sums are not used.
+  const int r0 = min(col0 + gid, a.n_out - 1);
+  const int r1 = EPI == GLU ? r0 + a.n_out : min(col0 + gid + 8, a.n_out - 1);
+  const uint16_t* w0 = w + r0 * ldw + t * 8;
+  const uint16_t* w1 = w + r1 * ldw + t * 8;
+  const uint16_t* xp[NT];
+#pragma unroll
+  for (int j = 0; j < NT; ++j) xp[j] = x + min(gid + 8 * j, a.m - 1) * ldx + t * 8;
+  float c[NT][4];
+#pragma unroll
+  for (int j = 0; j < NT; ++j)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c[j][e] = 0.0f;
+  overlap_wait();
+  overlap_next();
+
+  const int kt = (a.k + BK - 1) / BK, stride = split * WARPS;
+  const uint4 zero = make_uint4(0, 0, 0, 0);
+  for (int s = rank * WARPS + warp; s < kt; s += stride * U) {
+    uint4 wa[U][2], wb[U][2], xs[U][2][NT];
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int64_t at = (int64_t)(s + i * stride) * BK + h * 32;
+        const bool in = at + t * 8 < a.k;  // 8 k are all in or all out
+        wa[i][h] = in ? __ldcs(reinterpret_cast<const uint4*>(w0 + at)) : zero;
+        wb[i][h] = in ? __ldcs(reinterpret_cast<const uint4*>(w1 + at)) : zero;
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+          xs[i][h][j] = in ? *reinterpret_cast<const uint4*>(xp[j] + at) : zero;
+      }
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          const uint4 &p = wa[i][h], &q = wb[i][h], &v = xs[i][h][j];
+          mma(c[j], p.x, q.x, p.y, q.y, v.x, v.y);
+          mma(c[j], p.z, q.z, p.w, q.w, v.z, v.w);
+        }
+  }
+#pragma unroll
+  for (int j = 0; j < NT; ++j)
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      part[warp][(8 * j + 2 * t + (e & 1)) * 16 + gid + 8 * (e >> 1)] = c[j][e];
+  __syncthreads();
+  if (split > 1) cluster_wait();  // the cluster's first CTA is there
+  for (int i = threadIdx.x; i < SUMS; i += THREADS) {
+    float v = 0.0f;
+#pragma unroll
+    for (int p = 0; p < WARPS; ++p) v += part[p][i];
+    if (split > 1)
+      asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(mapa_shared(&recv[rank][i], 0)), "f"(v)
+                   : "memory");
+    else
+      recv[0][i] = v;
+  }
+  if (split > 1) {
+    cluster_arrive();
+    cluster_wait();
+    if (rank != 0) return;
+  } else {
+    __syncthreads();
+  }
+  for (int i = threadIdx.x; i < 8 * NT * FEAT; i += THREADS) {
+    const int row = i / FEAT, f = i % FEAT;
+    if (row >= a.m || col0 + f >= a.n_out) continue;
+    float z[1] = {0.0f}, u[1] = {0.0f};
+    for (int p = 0; p < split; ++p) {
+      z[0] += recv[p][row * 16 + f];
+      if (EPI == GLU) u[0] += recv[p][row * 16 + 8 + f];
+    }
+    epilogue_column<EPI, 1>(a, row, 1, col0 + f, z, u);
+  }
+}
+
+template <int EPI>
+int tiles(const Args& a) {
+  return EPI == GLU ? (a.n_out + 7) / 8 : (a.n_out + 15) / 16;
+}
+
+template <int NT, int U, int EPI>
+int launch(const void* x, int64_t ldx, const void* w, int64_t ldw, const Args& a,
+           cudaStream_t stream) {
+  // Twice the CTAs on the k axis as long as all run at once and every warp keeps
+  // two steps (4096 x 256, one row: 3.2 us unsplit, 2.4 over four; 2048 x 4096:
+  // 3.7 unsplit, 6.7 over two).
+  const int nt = tiles<EPI>(a), kt = (a.k + BK - 1) / BK;
+  int split = 1;
+  while (split < MAX_CLUSTER && nt * split <= num_sms() && kt >= 4 * split * WARPS) split *= 2;
+  return check_cuda(overlap_launch(dense_few_kernel<NT, U, EPI>,
+                                   dim3((unsigned)nt * split), dim3(THREADS), 0, split,
+                                   stream, static_cast<const uint16_t*>(x), ldx,
+                                   static_cast<const uint16_t*>(w), ldw, split, a),
+                    "dense_matmul launch");
+}
+
+}  // namespace few
+
 // The kernel and the split by what they take, in us, as fitted to times of both
 // at k = 512 .. 8192, n = 256 .. 8192, m = 1 .. 8192:
 //   split kernel  1.5 + waves * (max(0.23 * k steps of a CTA, w and x over HBM)
 //                                + 4 + (split > 1 ? 0.5 + 1.5 * rows of a tile / 128 : 0))
-//   pair kernel   6.5 + waves * max(0.27 * k steps, 4)
+//   pair kernel   6.5 + waves * max(0.27 * k steps, 4, w and x over HBM)
 // e.g. k = n = 4096, SwiGLU, m = 512: split 21.3 us, pair 26.9; m = 1024: 42.1
 // and 29.4. One CTA per SM in both: a wave is as many clusters as fit (of 8
 // CTAs fewer than 18, since a cluster stays within a GPC).
 template <int EPI>
 int run_epi(const void* x, int64_t ldx, const void* w, int64_t ldw, int n, const Args& a,
             cudaStream_t stream) {
+  const int64_t nk = (int64_t)n * a.k;
+  if (a.m <= 8 || (a.m <= 16 && nk <= 24 << 20) ||
+      (a.m <= 32 && nk <= 8 << 20 && few::tiles<EPI>(a) <= num_sms())) {
+    if (a.m <= 8) return few::launch<1, 4, EPI>(x, ldx, w, ldw, a, stream);
+    if (a.m <= 16) return few::launch<2, 2, EPI>(x, ldx, w, ldw, a, stream);
+    if (a.m <= 24) return few::launch<3, 2, EPI>(x, ldx, w, ldw, a, stream);
+    return few::launch<4, 1, EPI>(x, ldx, w, ldw, a, stream);
+  }
   const int bt = a.m <= 16 ? 16 : a.m <= 32 ? 32 : a.m <= 64 ? 64 : 128;
   const int feat = EPI == GLU ? TILE_W / 2 : TILE_W, pfeat = EPI == GLU ? 128 : 256;
   const int64_t tiles = (int64_t)((a.n_out + feat - 1) / feat) * ((a.m + bt - 1) / bt);
@@ -1066,8 +1216,9 @@ int run_epi(const void* x, int64_t ldx, const void* w, int64_t ldw, int n, const
       split = s;
     }
   }
-  const float t_pair = 6.5f + waves(ptiles, 2) * std::max(0.27f * (float)kt, 4.0f);
-  if (t_pair < best)
+  const float pv = waves(ptiles, 2);
+  const float t_pair = 6.5f + pv * std::max({0.27f * (float)kt, 4.0f, hbm / pv});
+  if (a.m > 64 && t_pair < best)
     return !a.out_vec || (a.residual && !a.res_vec)
                ? pair::launch<EPI, false, false>(x, ldx, w, ldw, n, a, stream)
            : a.residual ? pair::launch<EPI, true, true>(x, ldx, w, ldw, n, a, stream)
