@@ -1035,7 +1035,7 @@ int launch(const void* x, int64_t ldx, const void* w, int64_t ldw, int n, const 
 }  // namespace pair
 
 // ---------------------------------------------------------------------------
-// Few-rows kernel (a decode step of at most 16 tokens). 16 rows of w (SwiGLU: 8
+// Few-rows kernel (decode steps, and small products). 16 rows of w (SwiGLU: 8
 // gate rows and the 8 up rows of the same features) are operand A of
 // mma.m16n8k16, up to 8 NT rows of x operand B, both straight from global memory
 // into registers: lane t of a quad takes 8 consecutive k of a row in one 16-byte
@@ -1045,7 +1045,9 @@ int launch(const void* x, int64_t ldx, const void* w, int64_t ldw, int n, const 
 // partial sums are added in warp and in CTA order.
 //
 // Bound: the stream of w, and for small w the launch and a memory latency,
-// which a kernel without TMA, mbarriers and TMEM to set up gets to sooner.
+// which a kernel without TMA, mbarriers and TMEM to set up gets to sooner: 1 x
+// 4096 x 256 takes 2.4 us (split kernel 5.3), 1 x 4096 x 8192 13.8 (4.9 TB/s; 14.1).
+// 8 NT = 32 rows at a time were no faster than 16 (1000 x 777: 3.7 and 3.4 us for 64).
 // ---------------------------------------------------------------------------
 namespace few {
 
@@ -1060,7 +1062,12 @@ __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uin
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// U: 64-k steps whose loads are issued together. grid (w tiles x split).
+template <int EPI>
+__host__ __device__ __forceinline__ int tiles(const Args& a) {
+  return EPI == GLU ? (a.n_out + 7) / 8 : (a.n_out + 15) / 16;
+}
+
+// U: 64-k steps whose loads are issued together. grid: x tiles x w tiles x split.
 template <int NT, int U, int EPI>
 __global__ void __launch_bounds__(THREADS, 2)
     dense_few_kernel(const uint16_t* x, int64_t ldx, const uint16_t* w,
@@ -1071,8 +1078,8 @@ __global__ void __launch_bounds__(THREADS, 2)
   __shared__ float recv[MAX_CLUSTER][SUMS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int gid = lane >> 2, t = lane & 3;
-  const int rank = blockIdx.x % split;
-  const int col0 = blockIdx.x / split * FEAT;
+  const int rank = blockIdx.x % split, tile = blockIdx.x / split, nt = tiles<EPI>(a);
+  const int col0 = tile % nt * FEAT, row0 = tile / nt * (8 * NT);
   if (split > 1) cluster_arrive();
   // Rows past the last repeat it; their sums are not used.
   const int r0 = min(col0 + gid, a.n_out - 1);
@@ -1081,7 +1088,7 @@ __global__ void __launch_bounds__(THREADS, 2)
   const uint16_t* w1 = w + r1 * ldw + t * 8;
   const uint16_t* xp[NT];
 #pragma unroll
-  for (int j = 0; j < NT; ++j) xp[j] = x + min(gid + 8 * j, a.m - 1) * ldx + t * 8;
+  for (int j = 0; j < NT; ++j) xp[j] = x + min(row0 + gid + 8 * j, a.m - 1) * ldx + t * 8;
   float c[NT][4];
 #pragma unroll
   for (int j = 0; j < NT; ++j)
@@ -1143,58 +1150,67 @@ __global__ void __launch_bounds__(THREADS, 2)
   }
   for (int i = threadIdx.x; i < 8 * NT * FEAT; i += THREADS) {
     const int row = i / FEAT, f = i % FEAT;
-    if (row >= a.m || col0 + f >= a.n_out) continue;
+    if (row0 + row >= a.m || col0 + f >= a.n_out) continue;
     float z[1] = {0.0f}, u[1] = {0.0f};
     for (int p = 0; p < split; ++p) {
       z[0] += recv[p][row * 16 + f];
       if (EPI == GLU) u[0] += recv[p][row * 16 + 8 + f];
     }
-    epilogue_column<EPI, 1>(a, row, 1, col0 + f, z, u);
+    epilogue_column<EPI, 1>(a, row0 + row, 1, col0 + f, z, u);
   }
 }
 
+// How many CTAs share a tile's k, and what the kernel takes, in us.
+struct Plan {
+  int64_t ctas;
+  int split;
+  float us;
+};
 template <int EPI>
-int tiles(const Args& a) {
-  return EPI == GLU ? (a.n_out + 7) / 8 : (a.n_out + 15) / 16;
+Plan plan(const Args& a, int rows, float hbm) {
+  // Twice the CTAs on the k axis as long as all run at once and every warp keeps
+  // two steps (1 x 4096 x 256: 3.2 us unsplit, 2.4 over four; 1 x 2048 x 4096: 3.7
+  // unsplit, 6.7 over two).
+  const int64_t nb = ((int64_t)a.m + rows - 1) / rows, tiled = tiles<EPI>(a) * nb;
+  const int kt = (a.k + BK - 1) / BK, sms = num_sms();
+  Plan p{tiled, 1, 0.0f};
+  while (p.split < MAX_CLUSTER && p.ctas <= sms && kt >= 4 * p.split * WARPS) {
+    p.split *= 2;
+    p.ctas *= 2;
+  }
+  const float v = std::max(1.0f, (float)p.ctas / (float)sms);
+  p.us = 1.3f + std::max(1.4f * hbm, v * (0.6f + 0.047f * (float)kt / (float)p.split));
+  return p;
 }
 
 template <int NT, int U, int EPI>
-int launch(const void* x, int64_t ldx, const void* w, int64_t ldw, const Args& a,
+int launch(const void* x, int64_t ldx, const void* w, int64_t ldw, const Plan& p, const Args& a,
            cudaStream_t stream) {
-  // Twice the CTAs on the k axis as long as all run at once and every warp keeps
-  // two steps (4096 x 256, one row: 3.2 us unsplit, 2.4 over four; 2048 x 4096:
-  // 3.7 unsplit, 6.7 over two).
-  const int nt = tiles<EPI>(a), kt = (a.k + BK - 1) / BK;
-  int split = 1;
-  while (split < MAX_CLUSTER && nt * split <= num_sms() && kt >= 4 * split * WARPS) split *= 2;
-  return check_cuda(overlap_launch(dense_few_kernel<NT, U, EPI>,
-                                   dim3((unsigned)nt * split), dim3(THREADS), 0, split,
-                                   stream, static_cast<const uint16_t*>(x), ldx,
-                                   static_cast<const uint16_t*>(w), ldw, split, a),
+  return check_cuda(overlap_launch(dense_few_kernel<NT, U, EPI>, dim3((unsigned)p.ctas),
+                                   dim3(THREADS), 0, p.split, stream,
+                                   static_cast<const uint16_t*>(x), ldx,
+                                   static_cast<const uint16_t*>(w), ldw, p.split, a),
                     "dense_matmul launch");
 }
 
 }  // namespace few
 
-// The kernel and the split by what they take, in us, as fitted to times of both
-// at k = 512 .. 8192, n = 256 .. 8192, m = 1 .. 8192:
-//   split kernel  1.5 + waves * (max(0.23 * k steps of a CTA, w and x over HBM)
-//                                + 4 + (split > 1 ? 0.5 + 1.5 * rows of a tile / 128 : 0))
-//   pair kernel   6.5 + waves * max(0.27 * k steps, 4, w and x over HBM)
-// e.g. k = n = 4096, SwiGLU, m = 512: split 21.3 us, pair 26.9; m = 1024: 42.1
-// and 29.4. One CTA per SM in both: a wave is as many clusters as fit (of 8
-// CTAs fewer than 18, since a cluster stays within a GPC).
+// The kernel, and how k is split, by what they take, in us. Fitted to times of
+// all three (each split of the second) at 200 shapes, k = 64 .. 8192, n = 16 ..
+// 16384, m = 9 .. 4096, one launch after another; w and x over HBM at 6.5 TB/s:
+//   few    1.3 + max(1.4 * HBM, CTAs an SM * (0.6 + 0.047 * k steps of a CTA))
+//   split  -0.6 + waves * (max(0.22 * k steps of a CTA, 1.05 * HBM / waves)
+//                          + 2.75 + 2.5 * b (+ 0.85 + 0.8 * b with k split))
+//   pair   5 + waves * max(0.35 * k steps, 1.33 * HBM / waves)
+// b: rows of x in a tile / 128. The choice is the fastest one or within 5% of it
+// at all but 4 of the shapes (12%). One CTA per SM in the last two: a wave is as
+// many clusters as fit (of 8 CTAs fewer than 18, since a cluster stays within a
+// GPC). E.g. k = 1000, n = 777: few 2.5 us at m = 33, split 5.0; 8.7 and 8.0 at
+// m = 256. k = 2048, n = 4096: split 10.5, pair 15.4 at m = 256; 25.3 and 17.8 at
+// 1024.
 template <int EPI>
 int run_epi(const void* x, int64_t ldx, const void* w, int64_t ldw, int n, const Args& a,
             cudaStream_t stream) {
-  const int64_t nk = (int64_t)n * a.k;
-  if (a.m <= 8 || (a.m <= 16 && nk <= 24 << 20) ||
-      (a.m <= 32 && nk <= 8 << 20 && few::tiles<EPI>(a) <= num_sms())) {
-    if (a.m <= 8) return few::launch<1, 4, EPI>(x, ldx, w, ldw, a, stream);
-    if (a.m <= 16) return few::launch<2, 2, EPI>(x, ldx, w, ldw, a, stream);
-    if (a.m <= 24) return few::launch<3, 2, EPI>(x, ldx, w, ldw, a, stream);
-    return few::launch<4, 1, EPI>(x, ldx, w, ldw, a, stream);
-  }
   const int bt = a.m <= 16 ? 16 : a.m <= 32 ? 32 : a.m <= 64 ? 64 : 128;
   const int feat = EPI == GLU ? TILE_W / 2 : TILE_W, pfeat = EPI == GLU ? 128 : 256;
   const int64_t tiles = (int64_t)((a.n_out + feat - 1) / feat) * ((a.m + bt - 1) / bt);
@@ -1205,19 +1221,25 @@ int run_epi(const void* x, int64_t ldx, const void* w, int64_t ldw, int n, const
     return (float)((tiles + c - 1) / c);
   };
   const float hbm = 2.0f * (float)a.k * ((float)a.m + (float)n) / 6.5e6f;
+  const float b = (float)bt / 128.0f;
   int split = 1;
   float best = 0.0f;
   for (int s = 1; s <= MAX_CLUSTER && (s == 1 || kt >= 2 * s); s *= 2) {
     const float v = waves(tiles, s);
-    const float t = 1.5f + v * (std::max(0.23f * (float)((kt + s - 1) / s), hbm / v) + 4.0f +
-                                (s > 1 ? 0.5f + 1.5f * (float)bt / 128.0f : 0.0f));
+    const float t = v * (std::max(0.22f * (float)((kt + s - 1) / s), 1.05f * hbm / v) + 2.75f +
+                         2.5f * b + (s > 1 ? 0.85f + 0.8f * b : 0.0f)) -
+                    0.6f;
     if (s == 1 || t < best) {
       best = t;
       split = s;
     }
   }
   const float pv = waves(ptiles, 2);
-  const float t_pair = 6.5f + pv * std::max({0.27f * (float)kt, 4.0f, hbm / pv});
+  const float t_pair = 5.0f + pv * std::max(0.35f * (float)kt, 1.33f * hbm / pv);
+  const few::Plan p = few::plan<EPI>(a, a.m <= 8 ? 8 : 16, hbm);
+  if (a.m <= 8) return few::launch<1, 4, EPI>(x, ldx, w, ldw, p, a, stream);
+  if (p.us < best && (a.m <= 64 || p.us < t_pair) && p.ctas <= INT32_MAX)
+    return few::launch<2, 2, EPI>(x, ldx, w, ldw, p, a, stream);
   if (a.m > 64 && t_pair < best)
     return !a.out_vec || (a.residual && !a.res_vec)
                ? pair::launch<EPI, false, false>(x, ldx, w, ldw, n, a, stream)
