@@ -208,8 +208,13 @@ __device__ __forceinline__ float seg_sum(float v, int lpt) {
   for (int o = lpt / 2; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
-template <class T>
-__device__ __forceinline__ T seg_max(T v, int lpt) {
+template <bool WARP>
+__device__ __forceinline__ uint32_t seg_max(uint32_t v, int lpt) {
+  if (WARP) return __reduce_max_sync(0xffffffffu, v);
+  for (int o = lpt / 2; o; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+__device__ __forceinline__ float seg_max(float v, int lpt) {
   for (int o = lpt / 2; o; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
   return v;
 }
@@ -232,15 +237,28 @@ __device__ __forceinline__ void largest(const uint32_t (&key)[KPL], uint32_t lim
   }
 }
 
-// KPL: places in a lane's run; WHOLE: every group's lanes use them all.
-template <int LD, int KPL, bool WHOLE>
+// Element s of an array in registers.
+template <class T, int N>
+__device__ __forceinline__ T of_slot(const T (&v)[N], int s) {
+  T r = v[0];
+#pragma unroll
+  for (int j = 1; j < N; ++j)
+    if (s == j) r = v[j];
+  return r;
+}
+
+// KPL: places in a lane's run; WHOLE: every group's lanes use them all; WARP: 32
+// lanes a token.
+template <int LD, int KPL, bool WHOLE, bool WARP>
 __global__ void __launch_bounds__(32 * WARPS) route_grouped_kernel(const Args a) {
   using P = Packed<KPL>;
   constexpr uint32_t PLACES = P::PLACES;
+  constexpr int NS = WARP ? 1 : 4;  // picks a lane holds (top_k is at most 32)
   extern __shared__ uint64_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint64_t* buf = smem + warp * a.e;
-  const int lpt = 1 << a.lpt_log, sl = lane & (lpt - 1), seg = lane & ~(lpt - 1);
+  const int lpt_log = WARP ? 5 : a.lpt_log, lpt = 1 << lpt_log;
+  const int sl = lane & (lpt - 1), seg = lane & ~(lpt - 1);
   const uint32_t seg_mask = (lpt == 32 ? 0xFFFFFFFFu : (1u << lpt) - 1u) << seg;
   const int g = sl >> a.lg_log, part = sl & ((1 << a.lg_log) - 1);
   const bool in_group = g < a.groups;
@@ -250,12 +268,12 @@ __global__ void __launch_bounds__(32 * WARPS) route_grouped_kernel(const Args a)
   const int first = count > 0 ? g * a.per + start : 0;
   auto has = [&](int i) { return WHOLE ? true : i < count; };
   const bool biased = a.bias != nullptr;
-  const int tpw = 32 >> a.lpt_log;  // tokens a warp
+  const int tpw = 32 >> lpt_log;  // tokens a warp
   const int64_t stride = (int64_t)gridDim.x * WARPS * tpw;
   overlap_wait();
   overlap_next();
   for (int64_t base = ((int64_t)blockIdx.x * WARPS + warp) * tpw; base < a.t; base += stride) {
-    const int64_t tok = base + (lane >> a.lpt_log);
+    const int64_t tok = base + (lane >> lpt_log);
     const bool live = tok < a.t;
     const bool real = live && (a.num_valid < 0 || tok < a.num_valid);
     const int64_t row = (live ? tok : base) * a.ld;
@@ -386,8 +404,8 @@ __global__ void __launch_bounds__(32 * WARPS) route_grouped_kernel(const Args a)
     // does not need it.
     const bool settles = !(biased && a.scoring == DWM_SCORE_SOFTMAX);
     if (a.keep < a.groups && (biased || a.top2)) {
-      const float in = value32(~seg_max(open ? ~gkey : 0u, lpt));  // the least of the open
-      const float out = value32(seg_max(in_group && !open ? gkey : 0u, lpt));
+      const float in = value32(~seg_max<WARP>(open ? ~gkey : 0u, lpt));  // the least of the open
+      const float out = value32(seg_max<WARP>(in_group && !open ? gkey : 0u, lpt));
       // (Without a bias a sum of two scores is off relative to itself, unless it
       // is next to the f32 underflow.)
       const bool close = biased ? !(in - out > 2.0f * MARGIN * size)
@@ -430,15 +448,15 @@ __global__ void __launch_bounds__(32 * WARPS) route_grouped_kernel(const Args a)
     int left = open ? count : 0;  // in l or below it
     const int n_open = a.keep * a.per;
     uint32_t top = 0;  // the last pick's packed value
-    int last_id = 0, slot_id[4] = {0, 0, 0, 0};
+    int last_id = 0, slot_id[NS] = {};
     auto pick = [&](int k) {
-      top = seg_max(l[0] & ~PLACES, lpt);
+      top = seg_max<WARP>(l[0] & ~PLACES, lpt);
       // Of equal ones the lowest lane's, whose experts come first.
       const uint32_t who = __ballot_sync(0xffffffffu, (l[0] & ~PLACES) == top) & seg_mask;
       const int winner = __ffs(who) - 1;
       last_id = __shfl_sync(0xffffffffu, expert(l[0]), winner);
 #pragma unroll
-      for (int s = 0; s < 4; ++s)
+      for (int s = 0; s < NS; ++s)
         if (k == s * lpt + sl) slot_id[s] = last_id;
       uint32_t taken = 0;
       if (lane == winner) {
@@ -480,50 +498,43 @@ __global__ void __launch_bounds__(32 * WARPS) route_grouped_kernel(const Args a)
     if (__any_sync(0xffffffffu, close && real)) {
       // Up to three picks more, then all of them in the order of their 64-bit
       // values; what was not picked has to be below the last that is chosen.
-      const int all = min(min(a.top_k + 4, n_open), 4 * lpt);
+      const int all = min(min(a.top_k + 4, n_open), NS * lpt);
       for (int k = rounds; k < all; ++k) pick(k);
-      double c[4];
-      int place[4] = {0, 0, 0, 0}, id[4];
+      double c[NS];
+      int place[NS] = {}, id[NS];
 #pragma unroll
-      for (int s = 0; s < 4; ++s) c[s] = s * lpt + sl < all ? choice64(slot_id[s]) : 0.0;
+      for (int s = 0; s < NS; ++s) c[s] = s * lpt + sl < all ? choice64(slot_id[s]) : 0.0;
       double least = 0.0;  // the value at the place top_k - 1
       for (int k = 0; k < all; ++k) {
-        const int of = seg + (k & (lpt - 1)), s = k >> a.lpt_log;
-        const double v =
-            __shfl_sync(0xffffffffu, s == 0 ? c[0] : s == 1 ? c[1] : s == 2 ? c[2] : c[3], of);
-        const int e = __shfl_sync(
-            0xffffffffu,
-            s == 0 ? slot_id[0] : s == 1 ? slot_id[1] : s == 2 ? slot_id[2] : slot_id[3], of);
+        const int of = seg + (k & (lpt - 1)), s = k >> lpt_log;
+        const double v = __shfl_sync(0xffffffffu, of_slot(c, s), of);
+        const int e = __shfl_sync(0xffffffffu, of_slot(slot_id, s), of);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) place[j] += v > c[j] || (v == c[j] && e < slot_id[j]);
+        for (int j = 0; j < NS; ++j) place[j] += v > c[j] || (v == c[j] && e < slot_id[j]);
       }
 #pragma unroll
-      for (int j = 0; j < 4; ++j) id[j] = slot_id[j];
+      for (int j = 0; j < NS; ++j) id[j] = slot_id[j];
       for (int k = 0; k < all; ++k) {
-        const int of = seg + (k & (lpt - 1)), s = k >> a.lpt_log;
-        const int to = __shfl_sync(
-            0xffffffffu, s == 0 ? place[0] : s == 1 ? place[1] : s == 2 ? place[2] : place[3], of);
-        const int e = __shfl_sync(
-            0xffffffffu,
-            s == 0 ? slot_id[0] : s == 1 ? slot_id[1] : s == 2 ? slot_id[2] : slot_id[3], of);
-        const double v =
-            __shfl_sync(0xffffffffu, s == 0 ? c[0] : s == 1 ? c[1] : s == 2 ? c[2] : c[3], of);
+        const int of = seg + (k & (lpt - 1)), s = k >> lpt_log;
+        const int to = __shfl_sync(0xffffffffu, of_slot(place, s), of);
+        const int e = __shfl_sync(0xffffffffu, of_slot(slot_id, s), of);
+        const double v = __shfl_sync(0xffffffffu, of_slot(c, s), of);
         if (to == a.top_k - 1) least = v;
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < NS; ++j)
           if (to == j * lpt + sl) id[j] = e;
       }
       if (close) {
         unsure |= !settles || (all < n_open && !(least > bound(top)));
 #pragma unroll
-        for (int j = 0; j < 4; ++j) slot_id[j] = id[j];
+        for (int j = 0; j < NS; ++j) slot_id[j] = id[j];
       }
     }
 
     // Weights: slot s of lane sl is the pick s * lpt + sl.
-    float w[4], total = 0.0f;
+    float w[NS], total = 0.0f;
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {
+    for (int s = 0; s < NS; ++s) {
       w[s] = 0.0f;
       if (s * lpt + sl < a.top_k)
         w[s] = score32<true>(load_logit<LD>(a.logits, row + slot_id[s]), a.scoring, mx, inv_sum);
@@ -535,7 +546,7 @@ __global__ void __launch_bounds__(32 * WARPS) route_grouped_kernel(const Args a)
     if (live && !(doubts & seg_mask)) {
       const float scale = !a.renorm ? a.scale : total == 0.0f ? 0.0f : a.scale;
 #pragma unroll
-      for (int s = 0; s < 4; ++s) {
+      for (int s = 0; s < NS; ++s) {
         const int k = s * lpt + sl;
         if (k < a.top_k) {
           const float x = (a.renorm && total != 0.0f ? w[s] / total : w[s]) * scale;
@@ -547,8 +558,8 @@ __global__ void __launch_bounds__(32 * WARPS) route_grouped_kernel(const Args a)
       }
     }
     for (uint32_t again = doubts; again;) {
-      const int of = (__ffs(again) - 1) >> a.lpt_log;
-      again &= ~((lpt == 32 ? 0xFFFFFFFFu : (1u << lpt) - 1u) << (of << a.lpt_log));
+      const int of = (__ffs(again) - 1) >> lpt_log;
+      again &= ~((lpt == 32 ? 0xFFFFFFFFu : (1u << lpt) - 1u) << (of << lpt_log));
       const Pick p = route_row64<LD>(a, base + of, buf, lane);
       if (lane < a.top_k) {
         const int64_t at = (base + of) * a.top_k + lane;
@@ -567,8 +578,11 @@ int launch(const Args& a, cudaStream_t s) {
   const unsigned grid =
       (unsigned)std::min<int64_t>((a.t + tokens - 1) / tokens, (int64_t)num_sms() * 64);
   const size_t smem = (size_t)WARPS * a.e * sizeof(uint64_t);  // at most 32 KB
-  auto fn = a.run == KPL && a.per % a.run == 0 ? route_grouped_kernel<LD, KPL, true>
-                                               : route_grouped_kernel<LD, KPL, false>;
+  const bool whole = a.run == KPL && a.per % a.run == 0;
+  auto fn = a.lpt_log == 5 ? whole ? route_grouped_kernel<LD, KPL, true, true>
+                                   : route_grouped_kernel<LD, KPL, false, true>
+            : whole        ? route_grouped_kernel<LD, KPL, true, false>
+                           : route_grouped_kernel<LD, KPL, false, false>;
   return check_cuda(overlap_launch(fn, dim3(grid), dim3(32 * WARPS), smem, 1, s, a),
                     "route_grouped_topk launch");
 }
@@ -648,14 +662,16 @@ extern "C" int dwm_route_grouped_topk(const void* logits, int logits_dtype, int6
   a.w32 = topk_weights_f32;
   a.w16 = static_cast<uint16_t*>(topk_weights_bf16);
   // Lanes: a power of two of groups, each of as many lanes as leave at most 32
-  // experts a lane (64 where the warp has no more lanes), 8 a token at least. (All
-  // 32 lanes a token for small batches were no faster: the shorter runs save what
-  // the longer reductions cost.)
+  // experts a lane (64 where the warp has no more lanes); 8 a token at least, and
+  // up to eight tokens an SM the whole warp, for its shorter runs and its one
+  // instruction for a maximum (256 experts with a bias: one token 4.9 us against
+  // 6.6 with 8 lanes, 256 tokens 5.3 and 7.5, 4096 tokens 16.9 and 14.3).
+  const int lanes_log = t <= 8 * (int64_t)num_sms() ? 5 : 3;
   int groups_log = 0;
   while ((1 << groups_log) < num_groups) ++groups_log;
   a.lg_log = 0;
   while (groups_log + a.lg_log < 5 &&
-         ((a.per + (1 << a.lg_log) - 1) >> a.lg_log > 32 || groups_log + a.lg_log < 3))
+         ((a.per + (1 << a.lg_log) - 1) >> a.lg_log > 32 || groups_log + a.lg_log < lanes_log))
     ++a.lg_log;
   a.lpt_log = groups_log + a.lg_log;
   a.run = (a.per + (1 << a.lg_log) - 1) >> a.lg_log;
