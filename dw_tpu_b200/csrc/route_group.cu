@@ -16,8 +16,8 @@
 // the groups or the picks in question are compared in 64 bits; a token that
 // this does not settle is done again in 64 bits by the whole warp (8-12 us, which
 // one token of 1024 would make the time of all). Bound: instruction issue; a
-// single token takes 6.3 us of dependent instructions, 32771 tokens of 160
-// experts 21 us where their bytes take 3.4 (in 64 bits throughout: 83).
+// single token takes 3.9 us of dependent instructions, 32771 tokens of 160
+// experts 20 us where their bytes take 3.4 (in 64 bits throughout: 83).
 #include <algorithm>
 
 #include "common.cuh"
@@ -204,18 +204,23 @@ struct Packed {
 constexpr int DEEP = 6;  // a lane's largest that are kept sorted
 
 // Sum or maximum over a token's lanes.
-__device__ __forceinline__ float seg_sum(float v, int lpt) {
-  for (int o = lpt / 2; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+template <int LPT>
+__device__ __forceinline__ float seg_sum(float v) {
+#pragma unroll
+  for (int o = LPT / 2; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
-template <bool WARP>
-__device__ __forceinline__ uint32_t seg_max(uint32_t v, int lpt) {
-  if (WARP) return __reduce_max_sync(0xffffffffu, v);
-  for (int o = lpt / 2; o; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
+template <int LPT>
+__device__ __forceinline__ uint32_t seg_max(uint32_t v) {
+  if (LPT == 32) return __reduce_max_sync(0xffffffffu, v);
+#pragma unroll
+  for (int o = LPT / 2; o; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
   return v;
 }
-__device__ __forceinline__ float seg_max(float v, int lpt) {
-  for (int o = lpt / 2; o; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
+template <int LPT>
+__device__ __forceinline__ float seg_max(float v) {
+#pragma unroll
+  for (int o = LPT / 2; o; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
   return v;
 }
 
@@ -247,17 +252,17 @@ __device__ __forceinline__ T of_slot(const T (&v)[N], int s) {
   return r;
 }
 
-// KPL: places in a lane's run; WHOLE: every group's lanes use them all; WARP: 32
-// lanes a token.
-template <int LD, int KPL, bool WHOLE, bool WARP>
+// KPL: places in a lane's run; WHOLE: every group's lanes use them all;
+// 2^LPT_LOG lanes a token.
+template <int LD, int KPL, bool WHOLE, int LPT_LOG>
 __global__ void __launch_bounds__(32 * WARPS) route_grouped_kernel(const Args a) {
   using P = Packed<KPL>;
   constexpr uint32_t PLACES = P::PLACES;
-  constexpr int NS = WARP ? 1 : 4;  // picks a lane holds (top_k is at most 32)
+  constexpr int NS = 32 >> LPT_LOG;  // picks a lane holds (top_k is at most 32)
   extern __shared__ uint64_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint64_t* buf = smem + warp * a.e;
-  const int lpt_log = WARP ? 5 : a.lpt_log, lpt = 1 << lpt_log;
+  constexpr int lpt_log = LPT_LOG, lpt = 1 << lpt_log;
   const int sl = lane & (lpt - 1), seg = lane & ~(lpt - 1);
   const uint32_t seg_mask = (lpt == 32 ? 0xFFFFFFFFu : (1u << lpt) - 1u) << seg;
   const int g = sl >> a.lg_log, part = sl & ((1 << a.lg_log) - 1);
@@ -314,7 +319,7 @@ __global__ void __launch_bounds__(32 * WARPS) route_grouped_kernel(const Args a)
       mx = -INFINITY;
 #pragma unroll
       for (int i = 0; i < KPL; ++i) mx = fmaxf(mx, v[i]);  // (an absent one repeats the first)
-      mx = seg_max(count > 0 ? mx : -INFINITY, lpt);
+      mx = seg_max<lpt>(count > 0 ? mx : -INFINITY);
       if (mx == -INFINITY) mx = 0.0f;
       if (biased || !a.renorm) {
         float sum = 0.0f;
@@ -323,7 +328,7 @@ __global__ void __launch_bounds__(32 * WARPS) route_grouped_kernel(const Args a)
           const float s = score32<true>(v[i], DWM_SCORE_SOFTMAX, mx, 1.0f);
           if (has(i)) sum += s;
         }
-        sum = seg_sum(count > 0 ? sum : 0.0f, lpt);
+        sum = seg_sum<lpt>(count > 0 ? sum : 0.0f);
         inv_sum = sum > 0.0f ? 1.0f / sum : 1.0f;
       }
     }
@@ -344,7 +349,7 @@ __global__ void __launch_bounds__(32 * WARPS) route_grouped_kernel(const Args a)
         choices(DWM_SCORE_SIGMOID);
       else
         choices(DWM_SCORE_SQRTSOFTPLUS);
-      size = seg_max(size, lpt);
+      size = seg_max<lpt>(size);
     }
     uint32_t key[KPL];
 #pragma unroll
@@ -404,8 +409,8 @@ __global__ void __launch_bounds__(32 * WARPS) route_grouped_kernel(const Args a)
     // does not need it.
     const bool settles = !(biased && a.scoring == DWM_SCORE_SOFTMAX);
     if (a.keep < a.groups && (biased || a.top2)) {
-      const float in = value32(~seg_max<WARP>(open ? ~gkey : 0u, lpt));  // the least of the open
-      const float out = value32(seg_max<WARP>(in_group && !open ? gkey : 0u, lpt));
+      const float in = value32(~seg_max<lpt>(open ? ~gkey : 0u));  // the least of the open
+      const float out = value32(seg_max<lpt>(in_group && !open ? gkey : 0u));
       // (Without a bias a sum of two scores is off relative to itself, unless it
       // is next to the f32 underflow.)
       const bool close = biased ? !(in - out > 2.0f * MARGIN * size)
@@ -450,7 +455,7 @@ __global__ void __launch_bounds__(32 * WARPS) route_grouped_kernel(const Args a)
     uint32_t top = 0;  // the last pick's packed value
     int last_id = 0, slot_id[NS] = {};
     auto pick = [&](int k) {
-      top = seg_max<WARP>(l[0] & ~PLACES, lpt);
+      top = seg_max<lpt>(l[0] & ~PLACES);
       // Of equal ones the lowest lane's, whose experts come first.
       const uint32_t who = __ballot_sync(0xffffffffu, (l[0] & ~PLACES) == top) & seg_mask;
       const int winner = __ffs(who) - 1;
@@ -540,7 +545,7 @@ __global__ void __launch_bounds__(32 * WARPS) route_grouped_kernel(const Args a)
         w[s] = score32<true>(load_logit<LD>(a.logits, row + slot_id[s]), a.scoring, mx, inv_sum);
       total += w[s];
     }
-    if (a.renorm) total = seg_sum(total, lpt);
+    if (a.renorm) total = seg_sum<lpt>(total);
     // What one lane of a token is unsure of, all are.
     const uint32_t doubts = __ballot_sync(0xffffffffu, unsure && real && in_group);
     if (live && !(doubts & seg_mask)) {
@@ -572,30 +577,35 @@ __global__ void __launch_bounds__(32 * WARPS) route_grouped_kernel(const Args a)
   }
 }
 
-template <int LD, int KPL>
+template <int LD, int KPL, int LPT_LOG>
 int launch(const Args& a, cudaStream_t s) {
-  const int64_t tokens = (int64_t)WARPS * (32 >> a.lpt_log);  // a CTA's
+  const int64_t tokens = (int64_t)WARPS * (32 >> LPT_LOG);  // a CTA's
   const unsigned grid =
       (unsigned)std::min<int64_t>((a.t + tokens - 1) / tokens, (int64_t)num_sms() * 64);
   const size_t smem = (size_t)WARPS * a.e * sizeof(uint64_t);  // at most 32 KB
-  const bool whole = a.run == KPL && a.per % a.run == 0;
-  auto fn = a.lpt_log == 5 ? whole ? route_grouped_kernel<LD, KPL, true, true>
-                                   : route_grouped_kernel<LD, KPL, false, true>
-            : whole        ? route_grouped_kernel<LD, KPL, true, false>
-                           : route_grouped_kernel<LD, KPL, false, false>;
+  auto fn = a.run == KPL && a.per % a.run == 0 ? route_grouped_kernel<LD, KPL, true, LPT_LOG>
+                                               : route_grouped_kernel<LD, KPL, false, LPT_LOG>;
   return check_cuda(overlap_launch(fn, dim3(grid), dim3(32 * WARPS), smem, 1, s, a),
                     "route_grouped_topk launch");
 }
 
+template <int LD, int LPT_LOG>
+int by_run(const Args& a, cudaStream_t s) {
+  if (a.run <= 4) return launch<LD, 4, LPT_LOG>(a, s);
+  if (a.run <= 8) return launch<LD, 8, LPT_LOG>(a, s);
+  if (a.run <= 16) return launch<LD, 16, LPT_LOG>(a, s);
+  if (a.run <= 20) return launch<LD, 20, LPT_LOG>(a, s);
+  if (a.run <= 24) return launch<LD, 24, LPT_LOG>(a, s);
+  if (a.run <= 32) return launch<LD, 32, LPT_LOG>(a, s);
+  if constexpr (LPT_LOG == 5) return launch<LD, 64, LPT_LOG>(a, s);
+  return set_error(DWM_ERR_UNSUPPORTED, "run=%d", a.run);  // (more lanes have fewer)
+}
+
 template <int LD>
 int run(const Args& a, cudaStream_t s) {
-  if (a.run <= 4) return launch<LD, 4>(a, s);
-  if (a.run <= 8) return launch<LD, 8>(a, s);
-  if (a.run <= 16) return launch<LD, 16>(a, s);
-  if (a.run <= 20) return launch<LD, 20>(a, s);
-  if (a.run <= 24) return launch<LD, 24>(a, s);
-  if (a.run <= 32) return launch<LD, 32>(a, s);
-  return launch<LD, 64>(a, s);
+  return a.lpt_log == 3   ? by_run<LD, 3>(a, s)
+         : a.lpt_log == 4 ? by_run<LD, 4>(a, s)
+                          : by_run<LD, 5>(a, s);
 }
 
 }  // namespace route_group
@@ -663,10 +673,11 @@ extern "C" int dwm_route_grouped_topk(const void* logits, int logits_dtype, int6
   a.w16 = static_cast<uint16_t*>(topk_weights_bf16);
   // Lanes: a power of two of groups, each of as many lanes as leave at most 32
   // experts a lane (64 where the warp has no more lanes); 8 a token at least, and
-  // up to eight tokens an SM the whole warp, for its shorter runs and its one
-  // instruction for a maximum (256 experts with a bias: one token 4.9 us against
-  // 6.6 with 8 lanes, 256 tokens 5.3 and 7.5, 4096 tokens 16.9 and 14.3).
-  const int lanes_log = t <= 8 * (int64_t)num_sms() ? 5 : 3;
+  // up to twelve tokens an SM the whole warp, for its shorter runs and its one
+  // instruction for a maximum (256 experts with a bias: one token 4.1 us against
+  // 6.0 with 8 lanes, 1024 tokens 5.1 and 6.8; 32768 tokens 45.8 and 41.5, of 160
+  // experts 49 and 24).
+  const int lanes_log = t <= 12 * (int64_t)num_sms() ? 5 : 3;
   int groups_log = 0;
   while ((1 << groups_log) < num_groups) ++groups_log;
   a.lg_log = 0;
