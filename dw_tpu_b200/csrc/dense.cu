@@ -1047,7 +1047,8 @@ int launch(const void* x, int64_t ldx, const void* w, int64_t ldw, int n, const 
 // Bound: the stream of w, and for small w the launch and a memory latency,
 // which a kernel without TMA, mbarriers and TMEM to set up gets to sooner: 1 x
 // 4096 x 256 takes 2.4 us (split kernel 5.3), 1 x 4096 x 8192 13.8 (4.9 TB/s; 14.1).
-// 8 NT = 32 rows at a time were no faster than 16 (1000 x 777: 3.7 and 3.4 us for 64).
+// Tiles of 32 x 32 read half as much for a product: 333 x 1000 x 776 takes 5.4 us
+// with them, 9.5 with 16 x 16, 8.5 with the split kernel.
 // ---------------------------------------------------------------------------
 namespace few {
 
@@ -1063,52 +1064,65 @@ __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uin
 }
 
 template <int EPI>
-__host__ __device__ __forceinline__ int tiles(const Args& a) {
-  return EPI == GLU ? (a.n_out + 7) / 8 : (a.n_out + 15) / 16;
+__host__ __device__ __forceinline__ int tiles(int n_out, int mt) {
+  const int feat = (EPI == GLU ? 8 : 16) * mt;
+  return (n_out + feat - 1) / feat;
 }
 
-// U: 64-k steps whose loads are issued together. grid: x tiles x w tiles x split.
-template <int NT, int U, int EPI>
+// A tile: MT groups of 16 rows of w by NT groups of 8 rows of x. U: 64-k steps
+// whose loads are issued together. MAX_SPLIT: the most CTAs on one tile's k. grid:
+// x tiles x w tiles x split.
+template <int MT, int NT, int U, int MAX_SPLIT, int EPI>
 __global__ void __launch_bounds__(THREADS, 2)
     dense_few_kernel(const uint16_t* x, int64_t ldx, const uint16_t* w,
                      int64_t ldw, int split, const Args a) {
-  constexpr int FEAT = EPI == GLU ? 8 : 16;  // output columns of a tile
-  constexpr int SUMS = 8 * NT * 16;          // [row of x][row of the tile]
+  constexpr int GROUP = EPI == GLU ? 8 : 16;  // output columns of 16 rows of w
+  constexpr int FEAT = MT * GROUP;
+  constexpr int ROWS = MT * 16 + 4;    // (4: apart, the quads' sums are in banks of their own)
+  constexpr int SUMS = 8 * NT * ROWS;  // [row of x][row of the tile]
   __shared__ float part[WARPS][SUMS];
-  __shared__ float recv[MAX_CLUSTER][SUMS];
+  __shared__ float recv[MAX_SPLIT][SUMS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int gid = lane >> 2, t = lane & 3;
-  const int rank = blockIdx.x % split, tile = blockIdx.x / split, nt = tiles<EPI>(a);
+  const int rank = blockIdx.x % split, tile = blockIdx.x / split, nt = tiles<EPI>(a.n_out, MT);
   const int col0 = tile % nt * FEAT, row0 = tile / nt * (8 * NT);
   if (split > 1) cluster_arrive();
   // Rows past the last repeat it; their sums are not used.
-  const int r0 = min(col0 + gid, a.n_out - 1);
-  const int r1 = EPI == GLU ? r0 + a.n_out : min(col0 + gid + 8, a.n_out - 1);
-  const uint16_t* w0 = w + r0 * ldw + t * 8;
-  const uint16_t* w1 = w + r1 * ldw + t * 8;
-  const uint16_t* xp[NT];
+  const uint16_t *wp[MT][2], *xp[NT];
+#pragma unroll
+  for (int g = 0; g < MT; ++g) {
+    const int r0 = min(col0 + g * GROUP + gid, a.n_out - 1);
+    const int r1 = EPI == GLU ? r0 + a.n_out : min(col0 + g * GROUP + gid + 8, a.n_out - 1);
+    wp[g][0] = w + r0 * ldw + t * 8;
+    wp[g][1] = w + r1 * ldw + t * 8;
+  }
 #pragma unroll
   for (int j = 0; j < NT; ++j) xp[j] = x + min(row0 + gid + 8 * j, a.m - 1) * ldx + t * 8;
-  float c[NT][4];
+  float c[MT][NT][4];
 #pragma unroll
-  for (int j = 0; j < NT; ++j)
+  for (int g = 0; g < MT; ++g)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) c[j][e] = 0.0f;
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) c[g][j][e] = 0.0f;
   overlap_wait();
   overlap_next();
 
   const int kt = (a.k + BK - 1) / BK, stride = split * WARPS;
   const uint4 zero = make_uint4(0, 0, 0, 0);
   for (int s = rank * WARPS + warp; s < kt; s += stride * U) {
-    uint4 wa[U][2], wb[U][2], xs[U][2][NT];
+    uint4 ws[U][2][MT][2], xs[U][2][NT];
 #pragma unroll
     for (int i = 0; i < U; ++i)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int64_t at = (int64_t)(s + i * stride) * BK + h * 32;
         const bool in = at + t * 8 < a.k;  // 8 k are all in or all out
-        wa[i][h] = in ? __ldcs(reinterpret_cast<const uint4*>(w0 + at)) : zero;
-        wb[i][h] = in ? __ldcs(reinterpret_cast<const uint4*>(w1 + at)) : zero;
+#pragma unroll
+        for (int g = 0; g < MT; ++g)
+#pragma unroll
+          for (int r = 0; r < 2; ++r)
+            ws[i][h][g][r] = in ? __ldcs(reinterpret_cast<const uint4*>(wp[g][r] + at)) : zero;
 #pragma unroll
         for (int j = 0; j < NT; ++j)
           xs[i][h][j] = in ? *reinterpret_cast<const uint4*>(xp[j] + at) : zero;
@@ -1118,43 +1132,51 @@ __global__ void __launch_bounds__(THREADS, 2)
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          const uint4 &p = wa[i][h], &q = wb[i][h], &v = xs[i][h][j];
-          mma(c[j], p.x, q.x, p.y, q.y, v.x, v.y);
-          mma(c[j], p.z, q.z, p.w, q.w, v.z, v.w);
-        }
+        for (int g = 0; g < MT; ++g)
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+            const uint4 &p = ws[i][h][g][0], &q = ws[i][h][g][1], &v = xs[i][h][j];
+            mma(c[g][j], p.x, q.x, p.y, q.y, v.x, v.y);
+            mma(c[g][j], p.z, q.z, p.w, q.w, v.z, v.w);
+          }
   }
 #pragma unroll
-  for (int j = 0; j < NT; ++j)
+  for (int g = 0; g < MT; ++g)
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      part[warp][(8 * j + 2 * t + (e & 1)) * 16 + gid + 8 * (e >> 1)] = c[j][e];
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        part[warp][(8 * j + 2 * t + (e & 1)) * ROWS + g * 16 + gid + 8 * (e >> 1)] = c[g][j][e];
   __syncthreads();
-  if (split > 1) cluster_wait();  // the cluster's first CTA is there
-  for (int i = threadIdx.x; i < SUMS; i += THREADS) {
-    float v = 0.0f;
+  if (split > 1) {
+    cluster_wait();  // the cluster's first CTA is there
+    for (int i = threadIdx.x; i < SUMS; i += THREADS) {
+      float v = 0.0f;
 #pragma unroll
-    for (int p = 0; p < WARPS; ++p) v += part[p][i];
-    if (split > 1)
+      for (int p = 0; p < WARPS; ++p) v += part[p][i];
       asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(mapa_shared(&recv[rank][i], 0)), "f"(v)
                    : "memory");
-    else
-      recv[0][i] = v;
-  }
-  if (split > 1) {
+    }
     cluster_arrive();
     cluster_wait();
     if (rank != 0) return;
-  } else {
-    __syncthreads();
   }
   for (int i = threadIdx.x; i < 8 * NT * FEAT; i += THREADS) {
     const int row = i / FEAT, f = i % FEAT;
     if (row0 + row >= a.m || col0 + f >= a.n_out) continue;
+    const int at = row * ROWS + f / GROUP * 16 + f % GROUP;
     float z[1] = {0.0f}, u[1] = {0.0f};
-    for (int p = 0; p < split; ++p) {
-      z[0] += recv[p][row * 16 + f];
-      if (EPI == GLU) u[0] += recv[p][row * 16 + 8 + f];
+    if (split == 1) {
+#pragma unroll
+      for (int p = 0; p < WARPS; ++p) {
+        z[0] += part[p][at];
+        if (EPI == GLU) u[0] += part[p][at + 8];
+      }
+    } else {
+      for (int p = 0; p < split; ++p) {
+        z[0] += recv[p][at];
+        if (EPI == GLU) u[0] += recv[p][at + 8];
+      }
     }
     epilogue_column<EPI, 1>(a, row0 + row, 1, col0 + f, z, u);
   }
@@ -1167,27 +1189,29 @@ struct Plan {
   float us;
 };
 template <int EPI>
-Plan plan(const Args& a, int rows, float hbm) {
+Plan plan(const Args& a, int mt, int nt, int max_split, float hbm) {
   // Twice the CTAs on the k axis as long as all run at once and every warp keeps
   // two steps (1 x 4096 x 256: 3.2 us unsplit, 2.4 over four; 1 x 2048 x 4096: 3.7
   // unsplit, 6.7 over two).
-  const int64_t nb = ((int64_t)a.m + rows - 1) / rows, tiled = tiles<EPI>(a) * nb;
+  const int64_t nb = ((int64_t)a.m + 8 * nt - 1) / (8 * nt);
   const int kt = (a.k + BK - 1) / BK, sms = num_sms();
-  Plan p{tiled, 1, 0.0f};
-  while (p.split < MAX_CLUSTER && p.ctas <= sms && kt >= 4 * p.split * WARPS) {
+  Plan p{tiles<EPI>(a.n_out, mt) * nb, 1, 0.0f};
+  while (p.split < max_split && p.ctas <= sms && kt >= 4 * p.split * WARPS) {
     p.split *= 2;
     p.ctas *= 2;
   }
-  const float v = std::max(1.0f, (float)p.ctas / (float)sms);
-  p.us = 1.3f + std::max(1.4f * hbm, v * (0.6f + 0.047f * (float)kt / (float)p.split));
+  const float v = std::max(1.0f, (float)p.ctas / (float)sms), steps = (float)kt / (float)p.split;
+  const float waves = (float)((p.ctas + 2 * sms - 1) / (2 * sms));
+  p.us = 1.15f + (mt == 1 ? std::max(1.45f * hbm, waves * 0.042f * steps + v * (0.46f + 0.024f * steps))
+                          : std::max(2.0f * hbm, waves * 0.09f * steps + v * (0.8f + 0.045f * steps)));
   return p;
 }
 
-template <int NT, int U, int EPI>
+template <int MT, int NT, int U, int MAX_SPLIT, int EPI>
 int launch(const void* x, int64_t ldx, const void* w, int64_t ldw, const Plan& p, const Args& a,
            cudaStream_t stream) {
-  return check_cuda(overlap_launch(dense_few_kernel<NT, U, EPI>, dim3((unsigned)p.ctas),
-                                   dim3(THREADS), 0, p.split, stream,
+  return check_cuda(overlap_launch(dense_few_kernel<MT, NT, U, MAX_SPLIT, EPI>,
+                                   dim3((unsigned)p.ctas), dim3(THREADS), 0, p.split, stream,
                                    static_cast<const uint16_t*>(x), ldx,
                                    static_cast<const uint16_t*>(w), ldw, p.split, a),
                     "dense_matmul launch");
@@ -1196,18 +1220,21 @@ int launch(const void* x, int64_t ldx, const void* w, int64_t ldw, const Plan& p
 }  // namespace few
 
 // The kernel, and how k is split, by what they take, in us. Fitted to times of
-// all three (each split of the second) at 200 shapes, k = 64 .. 8192, n = 16 ..
-// 16384, m = 9 .. 4096, one launch after another; w and x over HBM at 6.5 TB/s:
-//   few    1.3 + max(1.4 * HBM, CTAs an SM * (0.6 + 0.047 * k steps of a CTA))
-//   split  -0.6 + waves * (max(0.22 * k steps of a CTA, 1.05 * HBM / waves)
-//                          + 2.75 + 2.5 * b (+ 0.85 + 0.8 * b with k split))
-//   pair   5 + waves * max(0.35 * k steps, 1.33 * HBM / waves)
-// b: rows of x in a tile / 128. The choice is the fastest one or within 5% of it
-// at all but 4 of the shapes (12%). One CTA per SM in the last two: a wave is as
-// many clusters as fit (of 8 CTAs fewer than 18, since a cluster stays within a
-// GPC). E.g. k = 1000, n = 777: few 2.5 us at m = 33, split 5.0; 8.7 and 8.0 at
-// m = 256. k = 2048, n = 4096: split 10.5, pair 15.4 at m = 256; 25.3 and 17.8 at
-// 1024.
+// every kernel and split at 170 shapes, k = 64 .. 8192, n = 16 .. 8192, m = 16 ..
+// 2048, one launch after another; HBM: w and x at 6.5 TB/s:
+//   few, tiles of 16 x 16   1.15 + max(1.45 * HBM, waves * 0.042 * k steps of a CTA
+//                                      + CTAs an SM * (0.46 + 0.024 * k steps))
+//        tiles of 32 x 32   1.15 + max(2 * HBM, waves * 0.09 * k steps
+//                                      + CTAs an SM * (0.8 + 0.045 * k steps))
+//   split                  -0.6 + waves * (max(0.22 * k steps, 1.05 * HBM / waves)
+//                                          + 2.75 + 2.5 * b (+ 0.85 + 0.8 * b split))
+//   pair                    5 + waves * max(0.35 * k steps, 1.33 * HBM / waves)
+// b: rows of x in a tile / 128. A wave: two CTAs per SM in the first, one CTA in the
+// others: as many clusters as fit (of 8 CTAs fewer than 18, since a cluster stays
+// within a GPC). The choice takes 0.5% more than the fastest on average, 25% at
+// most. E.g. k = 1000, n = 776: few 2.7 us at m = 48, split 5.4; 5.4 (large tiles)
+// and 8.5 at m = 333, 9.5 and 8.6 at 512. k = 2048, n = 4096: split 10.5, pair 15.4
+// at m = 256; 25.3 and 17.8 at 1024.
 template <int EPI>
 int run_epi(const void* x, int64_t ldx, const void* w, int64_t ldw, int n, const Args& a,
             cudaStream_t stream) {
@@ -1236,11 +1263,15 @@ int run_epi(const void* x, int64_t ldx, const void* w, int64_t ldw, int n, const
   }
   const float pv = waves(ptiles, 2);
   const float t_pair = 5.0f + pv * std::max(0.35f * (float)kt, 1.33f * hbm / pv);
-  const few::Plan p = few::plan<EPI>(a, a.m <= 8 ? 8 : 16, hbm);
-  if (a.m <= 8) return few::launch<1, 4, EPI>(x, ldx, w, ldw, p, a, stream);
-  if (p.us < best && (a.m <= 64 || p.us < t_pair) && p.ctas <= INT32_MAX)
-    return few::launch<2, 2, EPI>(x, ldx, w, ldw, p, a, stream);
-  if (a.m > 64 && t_pair < best)
+  const few::Plan small = few::plan<EPI>(a, 1, a.m <= 8 ? 1 : 2, 8, hbm);
+  const few::Plan large = few::plan<EPI>(a, 2, 4, 2, hbm);
+  if (a.m <= 8) return few::launch<1, 1, 4, 8, EPI>(x, ldx, w, ldw, small, a, stream);
+  if (a.m > 64) best = std::min(best, t_pair);
+  const few::Plan& least = small.us < large.us ? small : large;
+  if (least.us < best && least.ctas <= INT32_MAX)
+    return &least == &small ? few::launch<1, 2, 2, 8, EPI>(x, ldx, w, ldw, small, a, stream)
+                            : few::launch<2, 4, 1, 2, EPI>(x, ldx, w, ldw, large, a, stream);
+  if (a.m > 64 && t_pair == best)
     return !a.out_vec || (a.residual && !a.res_vec)
                ? pair::launch<EPI, false, false>(x, ldx, w, ldw, n, a, stream)
            : a.residual ? pair::launch<EPI, true, true>(x, ldx, w, ldw, n, a, stream)
