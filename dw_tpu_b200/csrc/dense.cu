@@ -1105,8 +1105,18 @@ __global__ void __launch_bounds__(THREADS, 2)
     for (int j = 0; j < NT; ++j)
 #pragma unroll
       for (int e = 0; e < 4; ++e) c[g][j][e] = 0.0f;
+  // The outputs of a thread: column f of `mine` rows of the tile from `row`.
+  constexpr int OUTS = 8 * NT * FEAT > THREADS ? 8 * NT * FEAT / THREADS : 1;
+  const int row = threadIdx.x / FEAT * OUTS, f = threadIdx.x % FEAT;
+  const int mine = col0 + f < a.n_out ? min(OUTS, min(8 * NT, a.m - row0) - row) : 0;
   overlap_wait();
   overlap_next();
+  if (a.residual && rank == 0)
+    for (int q = 0; q < mine; ++q) {
+      const int64_t at = (row0 + row + q) * a.ldr + col0 + f;
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const uint8_t*>(a.residual) +
+                                                    at * (a.res_f32 ? 4 : 2)));
+    }
 
   const int kt = (a.k + BK - 1) / BK, stride = split * WARPS;
   const uint4 zero = make_uint4(0, 0, 0, 0);
@@ -1161,25 +1171,26 @@ __global__ void __launch_bounds__(THREADS, 2)
     cluster_wait();
     if (rank != 0) return;
   }
-  for (int i = threadIdx.x; i < 8 * NT * FEAT; i += THREADS) {
-    const int row = i / FEAT, f = i % FEAT;
-    if (row0 + row >= a.m || col0 + f >= a.n_out) continue;
-    const int at = row * ROWS + f / GROUP * 16 + f % GROUP;
-    float z[1] = {0.0f}, u[1] = {0.0f};
+  if (mine <= 0) return;
+  float z[OUTS], u[OUTS];
+#pragma unroll
+  for (int q = 0; q < OUTS; ++q) {
+    const int at = (row + q) * ROWS + f / GROUP * 16 + f % GROUP;
+    z[q] = u[q] = 0.0f;
     if (split == 1) {
 #pragma unroll
       for (int p = 0; p < WARPS; ++p) {
-        z[0] += part[p][at];
-        if (EPI == GLU) u[0] += part[p][at + 8];
+        z[q] += part[p][at];
+        if (EPI == GLU) u[q] += part[p][at + 8];
       }
     } else {
       for (int p = 0; p < split; ++p) {
-        z[0] += recv[p][at];
-        if (EPI == GLU) u[0] += recv[p][at + 8];
+        z[q] += recv[p][at];
+        if (EPI == GLU) u[q] += recv[p][at + 8];
       }
     }
-    epilogue_column<EPI, 1>(a, row0 + row, 1, col0 + f, z, u);
   }
+  epilogue_column<EPI, OUTS>(a, row0 + row, mine, col0 + f, z, u);
 }
 
 // How many CTAs share a tile's k, and what the kernel takes, in us.
