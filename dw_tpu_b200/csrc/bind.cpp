@@ -3,8 +3,8 @@
 // allocate what is not given and call the C ABI on the current stream of the
 // tensors' device. A decode step makes these calls for kernels of 2-10 us, where
 // ~40 attribute lookups and a ctypes call cost more than the kernel: host time of
-// post_norm with most arguments 24.6 us that way, 6.2 us here; pre_norm 17.4 and
-// 5.0, dense_matmul 16.0 and 5.4.
+// post_norm with most arguments 24.6 us that way, 5.4 us here; pre_norm 17.4 and
+// 4.3, dense_matmul 16.0 and 5.4.
 //
 // The C ABI stays the one implementation: its functions are looked up in
 // libdw_moe.so (init), and what they refuse raises ValueError with their

@@ -10,9 +10,17 @@
 // and h is formed from the f32 r, not from its rounding, so that the fused
 // call is no less exact than f32 arithmetic throughout.
 //
-// Bound: memory. A row of each tensor is read once and written once, and
-// stays in registers between the two norms. One CTA takes one row (a warp,
-// rows of up to 1024 elements), each thread up to 32 of its elements.
+// Few rows (block_norm_kernel): one CTA takes one row (a warp, rows of up to 1024
+// elements), every load of it issued before the first sum. Bound: the launch and
+// one memory latency (4096 elements: 1 row 1.8 us, 64 rows with everything 2.7).
+//
+// Many rows (block_norm_stream_kernel): one CTA per SM, its groups of threads take
+// rows in turn from a ring of bulk copies, the rows' vectors in shared memory.
+// Bound: memory, a row of each tensor read and written once and kept in registers
+// between the two norms: 8192 x 4096 bf16 with both norms and a gate by channel
+// 45.8 us (5.9 TB/s; 74 with a CTA a row). Rows that do not start on 16 bytes take
+// an element a load, and are bound by instruction issue: 1023 x 5003, layer norms,
+// f32 residual, full gate 27.1 us (2.6 TB/s).
 #include <algorithm>
 
 #include "common.cuh"
@@ -220,22 +228,24 @@ __device__ __forceinline__ void store(uint8_t* row, bool f32, const Cols<VEC, CP
   }
 }
 
-// The threads that share a row: `threads` of them (whole warps), this one the
+// The threads that share a row: threads() of them (T if not 0) (whole warps), this one the
 // `i`-th, barrier `bar` theirs alone. part: one slot a warp for each of a
 // row's (at most four) sums, so one barrier a sum is enough; 16-byte aligned,
 // the slots of absent warps zero.
+template <int T>
 struct Group {
-  int i, threads, bar;
+  int i, run_threads, bar;
   float (*part)[32];
 
+  __device__ __forceinline__ int threads() const { return T ? T : run_threads; }
   __device__ __forceinline__ void sync() const {
-    if (threads == 32)
+    if (threads() == 32)
       __syncwarp();
     else
-      asm volatile("bar.sync %0, %1;" ::"r"(bar), "r"(threads) : "memory");
+      asm volatile("bar.sync %0, %1;" ::"r"(bar), "r"(threads()) : "memory");
   }
   __device__ __forceinline__ void clear_parts() const {
-    for (int j = i; j < 128; j += threads) part[j / 32][j % 32] = 0.0f;
+    for (int j = i; j < 128; j += threads()) part[j / 32][j % 32] = 0.0f;
   }
   // Sum over the row's threads, in a fixed order: the same bits in all of
   // them. between() runs after the barrier (with one warp a row: none).
@@ -243,7 +253,7 @@ struct Group {
   __device__ __forceinline__ float sum(float v, int slot, const F& between) const {
 #pragma unroll
     for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    if (threads == 32) {
+    if (threads() == 32) {
       between();
       return v;
     }
@@ -251,7 +261,8 @@ struct Group {
     sync();
     between();
     float s = 0.0f;
-    for (int w = 0; w < threads; w += 128) {
+#pragma unroll
+    for (int w = 0; w < threads(); w += 128) {
       const float4 p = *reinterpret_cast<const float4*>(&part[slot][w / 32]);
       s += (p.x + p.y) + (p.z + p.w);
     }
@@ -263,7 +274,7 @@ struct Group {
 // row has all of its elements of u.
 template <int VEC, int CPT, int T, int WD, class Vec, class Done>
 __device__ __forceinline__ void normalise(F2 (&u)[pairs(VEC, CPT)], const Cols<VEC, CPT, T>& cols,
-                                          const Args& a, const Group& g, int slot, float inv_h,
+                                          const Args& a, const Group<T>& g, int slot, float inv_h,
                                           const Vec& vec, int weight, int bias,
                                           const Done& read_done) {
   constexpr int NP = pairs(VEC, CPT);
@@ -313,7 +324,7 @@ __device__ __forceinline__ void normalise(F2 (&u)[pairs(VEC, CPT)], const Cols<V
 // runs once every thread has the row's elements.
 template <int VEC, int CPT, int T, int YD, int RD, int WD, class Y, class Res, class Gate,
           class Vec, class Done>
-__device__ __forceinline__ void do_row(const Args& a, const Group& g, int slot, uint8_t* r_out,
+__device__ __forceinline__ void do_row(const Args& a, const Group<T>& g, int slot, uint8_t* r_out,
                                        uint8_t* h_out, float inv_h,
                                        const Cols<VEC, CPT, T>& cols, float gate_tok, const Y& y,
                                        const Res& res, const Gate& gate, const Vec& vec,
@@ -372,12 +383,12 @@ constexpr int max_threads(bool stream) {
 template <int VEC, int CPT, int T, int YD, int RD, int WD>
 __global__ void __launch_bounds__(max_threads<VEC, CPT>(false)) block_norm_kernel(const Args a) {
   __shared__ __align__(16) float part[4][32];
-  const Group g{(int)threadIdx.x, (int)blockDim.x, 0, part};
+  const Group<T> g{(int)threadIdx.x, (int)blockDim.x, 0, part};
   const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
   overlap_wait();
   overlap_next();
   if (row >= a.t) return;  // a whole warp of a CTA with a warp a row
-  const Cols<VEC, CPT, T> cols(a.h, g.i, g.threads);
+  const Cols<VEC, CPT, T> cols(a.h, g.i, g.threads());
   const int ye = bytes_of<YD>(a.y_f32), re = bytes_of<RD>(a.res_f32);
   const uint8_t* pg = row_ptr(a.gate, a.gate_mode == DWM_GATE_FULL ? row : 0, a.ldg, ye);
   // Up to 16 elements a thread everything is loaded ahead; the gate and the
@@ -394,7 +405,7 @@ __global__ void __launch_bounds__(max_threads<VEC, CPT>(false)) block_norm_kerne
     if (a.h_out) w1.load(a.vec[W1], cols, a.w_f32);
   }
   const float tok = token_gate<YD>(a, row);
-  if (g.threads > 32) {
+  if (g.threads() > 32) {
     g.clear_parts();
     g.sync();
   }
@@ -449,7 +460,7 @@ __global__ void __launch_bounds__(max_threads<VEC, CPT>(true), 1)
   extern __shared__ __align__(16) uint8_t ring[];
   volatile int* abort_flag = &abort_word;
   const int gi = threadIdx.y, groups = blockDim.y;
-  const Group g{(int)threadIdx.x, (int)blockDim.x, gi, part[gi]};
+  const Group<T> g{(int)threadIdx.x, (int)blockDim.x, gi, part[gi]};
   const uint32_t vectors = smem_u32(ring);
   const uint32_t stages =
       vectors + (uint32_t)(5 * a.vec_bytes + gi * a.stages * a.stage_bytes);
@@ -462,7 +473,7 @@ __global__ void __launch_bounds__(max_threads<VEC, CPT>(true), 1)
   __syncthreads();
   overlap_wait();
   overlap_next();
-  const Cols<VEC, CPT, T> cols(a.h, g.i, g.threads);
+  const Cols<VEC, CPT, T> cols(a.h, g.i, g.threads());
   const float inv_h = 1.0f / (float)a.h;
   const int64_t first = (int64_t)blockIdx.x * groups + gi, step = (int64_t)gridDim.x * groups;
   const bool full_gate = a.gate_mode == DWM_GATE_FULL;
@@ -492,7 +503,7 @@ __global__ void __launch_bounds__(max_threads<VEC, CPT>(true), 1)
       const int es = j < 4 ? bytes_of<WD>(a.w_f32) : ye;
       if (!p) continue;
       uint8_t* dst = ring + j * a.vec_bytes;
-      const int tid = gi * g.threads + g.i, threads = groups * g.threads;
+      const int tid = gi * g.threads() + g.i, threads = groups * g.threads();
       if (VEC == 8) {
         for (int i = tid; i < a.h * es / 16; i += threads)
           reinterpret_cast<uint4*>(dst)[i] = static_cast<const uint4*>(p)[i];
@@ -634,6 +645,7 @@ int by_width(const Args& a, cudaStream_t s) {
 constexpr int MAX_H = 16384;
 
 int run(const Args& a, bool vec, cudaStream_t s) {
+  // (Types known when the kernel is compiled gained rows without VEC 1%.)
   if (!vec) return by_width<1, ANY, ANY, ANY>(a, s);
 #define DWM_NORM(YD, RD, WD)                                                               \
   if ((a.y_f32 != 0) == (YD == FP) && (a.res_f32 != 0) == (RD == FP) &&                    \
