@@ -3,13 +3,14 @@
 // products around the expert layer that are not FP4: the router's logits, the
 // shared expert's projections.
 //
-// Three kernels; run_epi chooses. Split kernel (a decode batch). The product is computed transposed: 128 rows of w are UMMA
-// operand A, up to 128 rows of x are operand B, so a decode batch pays for its
-// own tokens (N = 16 and up) and not for 128. The k axis is split over a
-// cluster of 1, 2, 4 or 8 CTAs, which fills the GPU when w has few rows. Each
-// CTA owns some of the tile's rows of x; all send it their f32 partials of those
-// rows (bulk copies between the CTAs' shared memories), and it adds them in CTA
-// order, so the result depends on the shapes alone: no atomics, no workspace.
+// Three kernels; run_epi chooses. Split kernel (a decode batch): the product is
+// computed transposed, 128 rows of w as UMMA operand A, up to 128 rows of x as
+// operand B, so a decode batch pays for its own tokens (N = 16 and up) and not for
+// 128. The k axis is split over a cluster of 1, 2, 4 or 8 CTAs, which fills the GPU
+// when w has few rows. Each CTA owns some of the tile's rows of x; all send it their
+// f32 partials of those rows (bulk copies between the CTAs' shared memories), and it
+// adds them in CTA order, so the result depends on the shapes alone: no atomics, no
+// workspace.
 //
 // With SwiGLU a tile is 64 gate rows and the 64 up rows of the same features,
 // which meet in the partial tile.
@@ -565,7 +566,8 @@ int launch_split(const void* x, int64_t ldx, const void* w, int64_t ldw, int n, 
                  const Args& a, cudaStream_t stream) {
   using L = Layout<BT>;
   constexpr int FEAT = EPI == GLU ? TILE_W / 2 : TILE_W;
-  DWM_CHECK_ARG((a.m + (int64_t)BT - 1) / BT <= 65535 && (a.n_out + (int64_t)FEAT - 1) / FEAT <= 65535,
+  DWM_CHECK_ARG((a.m + (int64_t)BT - 1) / BT <= 65535 &&
+                    (a.n_out + (int64_t)FEAT - 1) / FEAT <= 65535,
                 "m=%d rows by %d columns exceed the grid", a.m, a.n_out);
   CUtensorMap tm_w, tm_x;
   int rc = encode_tmap_2d(&tm_w, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, w, (uint64_t)a.k, (uint64_t)n,
@@ -1217,8 +1219,10 @@ Plan plan(const Args& a, int mt, int nt, int max_split, float hbm) {
   }
   const float v = std::max(1.0f, (float)p.ctas / (float)sms), steps = (float)kt / (float)p.split;
   const float waves = (float)((p.ctas + 2 * sms - 1) / (2 * sms));
-  p.us = 1.15f + (mt == 1 ? std::max(1.45f * hbm, waves * 0.042f * steps + v * (0.46f + 0.024f * steps))
-                          : std::max(2.0f * hbm, waves * 0.09f * steps + v * (0.8f + 0.045f * steps)));
+  p.us = 1.15f + (mt == 1 ? std::max(1.45f * hbm, waves * 0.042f * steps +
+                                                      v * (0.46f + 0.024f * steps))
+                          : std::max(2.0f * hbm, waves * 0.09f * steps +
+                                                     v * (0.8f + 0.045f * steps)));
   return p;
 }
 

@@ -439,13 +439,13 @@ def route_grouped_topk_out(logits, top_k, num_groups, topk_groups, ids_out, w32_
         w32_out, w16_out, stream)
 
 
-def route_grouped_topk_new(logits, top_k, num_groups, topk_groups, dtype, scoring_fn, group_score,
-                           renormalize, routed_scale, bias, num_valid_tokens):
-    """The same into new tensors: (weights of ``dtype``, bf16 or f32, and ids)."""
+def route_grouped_topk_new(logits, top_k, num_groups, topk_groups, dtype_code, scoring_fn,
+                           group_score, renormalize, routed_scale, bias, num_valid_tokens):
+    """The same into new tensors: (weights, bf16 or f32 by their code, and ids)."""
     return L.bind().route_grouped_topk(
         logits, top_k, num_groups, topk_groups, code_of(_SCORING, scoring_fn, "scoring_fn"),
-        code_of(_GROUP_SCORES, group_score, "group_score"), int(bool(renormalize)), routed_scale,
-        bias, -1 if num_valid_tokens is None else max(0, num_valid_tokens), L.FLOATS[dtype], None,
+        code_of(_GROUP_SCORES, group_score, "group_score"), 1 if renormalize else 0, routed_scale,
+        bias, -1 if num_valid_tokens is None else max(0, num_valid_tokens), dtype_code, None,
         None, None, None)
 
 

@@ -5,6 +5,7 @@ from __future__ import annotations
 
 import torch
 
+from . import _lib as L
 from . import ops
 
 
@@ -47,16 +48,13 @@ def route_grouped_topk(gating_output: torch.Tensor, top_k: int, num_groups: int,
     best ("top2"). The weights are the scores, divided by their sum if
     ``renormalize``, times ``routed_scale``. Selection is that of 64-bit scores
     whatever the logits' dtype. Inference only: no gradient."""
-    logits = gating_output
-    if logits.dtype not in (torch.bfloat16, torch.float32):
-        logits = logits.float()
-    if bias is not None and (bias.dtype != torch.float32 or not bias.is_contiguous()):
+    logits = gating_output if gating_output.dtype in L.FLOATS else gating_output.float()
+    if bias is not None and (bias.dtype is not torch.float32 or not bias.is_contiguous()):
         bias = bias.float().contiguous()
-    w, ids = ops.route_grouped_topk_new(
-        logits, top_k, num_groups, topk_groups,
-        torch.bfloat16 if dtype == torch.bfloat16 else torch.float32, scoring_fn, group_score,
-        renormalize, routed_scale, bias, num_valid_tokens)
-    return (w if w.dtype == dtype else w.to(dtype)), ids
+    w_ids = ops.route_grouped_topk_new(logits, top_k, num_groups, topk_groups,
+                                       L.FLOATS.get(dtype, L.F32), scoring_fn, group_score,
+                                       renormalize, routed_scale, bias, num_valid_tokens)
+    return w_ids if dtype in L.FLOATS else (w_ids[0].to(dtype), w_ids[1])
 
 
 def route_hash(gating_output: torch.Tensor, hash_ids: torch.Tensor, renormalize: bool = True,
