@@ -174,6 +174,41 @@ def test_dense_rows_are_their_own(dw, m):
     assert bool(got[0].isinf().all()) and bool(got[m + 1].isinf().all())
 
 
+@pytest.mark.parametrize("m", [1, 8, 9, 33, 70])
+@pytest.mark.parametrize("k", [2056, 4096, 8192])
+@pytest.mark.parametrize("n", [2, 66, 256])
+def test_dense_long_k(dw, m, k, n):
+    """Few columns of w: their k is shared by several CTAs, and ends inside a step."""
+    _dense_case(dw, m, k, n, bias=F32, res=BF, out_dtype=F32, seed=m + k + n)
+    _dense_case(dw, m, k, n, act="swiglu", bias=BF, res=F32, out_dtype=BF, seed=m * k + n)
+
+
+@pytest.mark.parametrize("m", [2, 13, 100, 333])
+@pytest.mark.parametrize("k,n", [(8, 4000), (520, 1032), (1000, 776)])
+@pytest.mark.parametrize("act", ["gelu", "swiglu"])
+def test_dense_few_hundred_rows(dw, m, k, n, act):
+    """In place, in rows that start anywhere, with a row of NaN."""
+    x, w = _randn(1, m, k), _randn(2, n, k, scale=k ** -0.5)
+    cols = n // 2 if act == "swiglu" else n
+    ref, tol = None, None
+    for pad, off in ((0, 0), (7, 3)):
+        buf = torch.full((m, cols + pad), -7.0, dtype=BF, device="cuda")
+        r = buf[:, off:off + cols]
+        r.copy_(_randn(3, m, cols))
+        if ref is None:
+            ref, tol = _dense_ref(x, w, None, act, r, 0.5, BF)
+            base = dw.dense_matmul(x, w, act=act, residual=r, residual_scale=0.5)
+            _close(base, ref, tol)
+        dw.dense_matmul(x, w, act=act, residual=r, residual_scale=0.5, out=r)
+        assert torch.equal(r, base)
+        r.fill_(-7.0)
+        assert bool((buf == -7.0).all())
+    x[m // 2, 3] = math.nan
+    got = dw.dense_matmul(x, w, act=act, residual=_randn(3, m, cols), residual_scale=0.5)
+    keep = [i for i in range(m) if i != m // 2]
+    assert torch.equal(got[keep], base[keep]) and bool(got[m // 2].isnan().all())
+
+
 @pytest.mark.parametrize("n,pad,off", [(1544, 0, 0), (1544, 24, 8), (1546, 0, 0), (1544, 3, 1)])
 @pytest.mark.parametrize("res,out_dtype", [(None, BF), (BF, BF), (F32, BF), (BF, F32), (F32, F32)])
 def test_dense_many_rows(dw, n, pad, off, res, out_dtype):
