@@ -438,6 +438,78 @@ def test_route_masked_and_non_finite(dw):
     assert ids[10].tolist()[0] == 39
 
 
+# From some tokens an SM on, several tokens share a warp.
+MANY = 2001
+
+
+@pytest.mark.parametrize("e,groups,keep,k", [
+    (1, 1, 1, 1), (8, 8, 8, 8), (31, 31, 7, 7), (32, 32, 32, 32), (33, 1, 1, 32), (34, 17, 16, 32),
+    (64, 2, 1, 32), (100, 5, 5, 3), (160, 8, 3, 6), (256, 8, 4, 8), (250, 5, 2, 8), (513, 27, 26, 17),
+    (1024, 32, 1, 32), (1024, 4, 3, 32), (992, 31, 30, 32)])
+def test_route_many_tokens(dw, e, groups, keep, k):
+    for dtype in (F32, BF):
+        x = _randn(e + k, MANY, e, scale=2.0, dtype=dtype)
+        b = _randn(9, e, scale=0.2, dtype=F32)
+        _route_case(dw, x, k, groups, keep, bias=b)
+        _route_case(dw, x, k, groups, keep, False, "softmax", "max")
+        _route_case(dw, x, k, groups, keep, scoring="sqrtsoftplus")
+        _route_case(dw, x, k, groups, keep, scoring="softmax", bias=b)
+
+
+def _undecided(x, groups, keep, scoring, bias):
+    """Rows whose order of groups 64-bit arithmetic leaves open. The sum of two
+    experts of ranks p and q of logits one f32 step d apart is 2 s + (p + q) s' d up
+    to s'' d^2 (p^2 + q^2) / 2 <= 2^-50 (d = 2^-24, p, q < 128, s'' < 0.3), so that
+    groups of the same p + q differ by a few of the last steps of 64 bits: as much
+    as two correct evaluations. exp, log1p (a step each, the sum's and the bias's
+    half, the root's half of half of them) put a score within 2^-51 of itself, the
+    sum of two, at most 4 here, within 2^-49; two sums closer than 2^-48 may come in
+    either order."""
+    x = x.double().cpu()
+    s = {"softmax": lambda v: v.softmax(1), "sigmoid": torch.sigmoid,
+         "sqrtsoftplus": lambda v: (v.clamp(min=0) + torch.log1p(torch.exp(-v.abs()))).sqrt()}
+    s = s[scoring](x)
+    c = s if bias is None else s + bias.double().cpu()
+    v = c.reshape(len(x), groups, -1).topk(2, dim=2)[0].sum(2).sort(dim=1, descending=True)[0]
+    return v[:, keep - 1] - v[:, keep] < 2.0 ** -48
+
+
+def test_route_many_tokens_ties_and_masks(dw):
+    """Ties, values one f32 step apart, masked experts and NaN, between ordinary
+    tokens of the same warp."""
+    g = torch.Generator().manual_seed(4)
+    e = 128
+    near = (torch.tensor(0.7).view(torch.int32) + torch.arange(e, dtype=torch.int32)).view(F32)
+    x = torch.randn((MANY, e), generator=g) * 1.5
+    x[::5] = torch.randint(-1, 2, x[::5].shape, generator=g).float()
+    x[1::7] = torch.stack([near[torch.randperm(e, generator=g)] for _ in range(len(x[1::7]))])
+    x[2::11, 16:112] = -math.inf
+    x[3::97] = -math.inf
+    x = x.cuda()
+    b = (torch.randint(0, 2, (e,), generator=g).float() * 0.5).cuda()
+    steps = torch.zeros(MANY, dtype=torch.bool)
+    steps[1::7] = True
+    steps[2::11] = steps[3::97] = False
+    for scoring in ("softmax", "sigmoid", "sqrtsoftplus"):
+        for bias in (None, b):
+            _route_case(dw, x, 8, 8, 3, scoring=scoring, group_score="max", bias=bias)
+            w, ids = dw.route_grouped_topk(x, 8, 8, 3, True, scoring, "top2", 2.5, F32, bias)
+            rw, ri = _route_ref(x, 8, 8, 3, True, scoring, "top2", 2.5, bias)
+            sure = ~(steps & _undecided(x, 8, 3, scoring, bias))
+            assert int((~sure).sum()) < MANY // 20
+            assert torch.equal(ids.cpu()[sure], ri[sure])
+            # (The others' weights are as close as their logits: 128 steps of 2^-24.)
+            _close(w.cpu(), rw, 2.0 ** -19 * rw.abs() + 1e-37 + 2.0 ** -16 * ~sure[:, None])
+    y = x.clone()
+    y[10, 1:] = math.nan
+    w, ids = dw.route_grouped_topk(y, 8, 8, 3, dtype=F32, num_valid_tokens=MANY - 3)
+    rw, ri = dw.route_grouped_topk(x, 8, 8, 3, dtype=F32)
+    rest = [i for i in range(MANY - 3) if i != 10]
+    assert torch.equal(ids[rest], ri[rest]) and torch.equal(w[rest], rw[rest])
+    assert ids[10, 0] == 0 and len(set(ids[10].tolist())) == 8
+    assert not bool(ids[MANY - 3:].any()) and not bool(w[MANY - 3:].any())
+
+
 @pytest.mark.parametrize("valid", [0, 1, 7, 100])
 def test_route_padding_strides_stream(dw, valid):
     buf = torch.full((12, 70), math.nan, device="cuda")
