@@ -298,9 +298,9 @@ int dwm_dense_matmul(const void* x, int64_t ldx, const void* w, int64_t ldw, int
  * (DWM_NORM_RMS) or m = mean(v) (DWM_NORM_LAYER); statistics, products and
  * sums in f32, h from the f32 r, each output rounded once. y [t, h] (bf16 or
  * f32) is the block's output, gate (DWM_GATE_*) has its dtype, residual [t, h]
- * and r_out share one dtype, h_out is bf16 or f32, w1 / b1 / w2 / b2 [h] share one; b1 and b2 may be NULL.
- * inner = 0: n2 is the identity. h_out = NULL: no n1 (w1 unused). y = NULL:
- * only h = n1(residual) (r_out NULL, no gate, inner = 0). ld*: row strides in
+ * and r_out share one dtype, h_out is bf16 or f32, w1 / b1 / w2 / b2 [h] share
+ * one; b1 and b2 may be NULL. inner = 0: n2 is the identity. h_out = NULL: no
+ * n1 (w1 unused). y = NULL: only h = n1(residual) (r_out NULL, no gate, inner = 0). ld*: row strides in
  * elements, any; 16-byte loads are used where every row of every tensor starts
  * on 16 bytes. An output may be one of y, residual and a full gate itself (same
  * pointer, stride and element size); any other overlap is refused.

@@ -457,21 +457,21 @@ def test_route_many_tokens(dw, e, groups, keep, k):
 
 
 def _undecided(x, groups, keep, scoring, bias):
-    """Rows whose order of groups 64-bit arithmetic leaves open. The sum of two
-    experts of ranks p and q of logits one f32 step d apart is 2 s + (p + q) s' d up
-    to s'' d^2 (p^2 + q^2) / 2 <= 2^-50 (d = 2^-24, p, q < 128, s'' < 0.3), so that
-    groups of the same p + q differ by a few of the last steps of 64 bits: as much
-    as two correct evaluations. exp, log1p (a step each, the sum's and the bias's
-    half, the root's half of half of them) put a score within 2^-51 of itself, the
-    sum of two, at most 4 here, within 2^-49; two sums closer than 2^-48 may come in
-    either order."""
+    """Rows whose order of groups 64-bit arithmetic leaves open. The sum of the
+    scores of logits p and q steps of d = 2^-24 above another is 2 s + (p + q) s' d
+    + (p^2 + q^2) s'' d^2 / 2, so two groups of the same p + q may differ by as little
+    as s'' d^2 = 2^-50. A score (at most 2) has errors of half a step of 2^-52 or a
+    step of a value below 1 from exp, log1p, their sum and the root, 2^-51 together;
+    with the bias and the sum of two (at most 4) that makes 2^-49 at most. Where two
+    sums computed here are 2^-47 or less apart, they may truly be 2^-48 apart in
+    either order, or 2^-48 the other way in the kernel's own arithmetic."""
     x = x.double().cpu()
     s = {"softmax": lambda v: v.softmax(1), "sigmoid": torch.sigmoid,
          "sqrtsoftplus": lambda v: (v.clamp(min=0) + torch.log1p(torch.exp(-v.abs()))).sqrt()}
     s = s[scoring](x)
     c = s if bias is None else s + bias.double().cpu()
     v = c.reshape(len(x), groups, -1).topk(2, dim=2)[0].sum(2).sort(dim=1, descending=True)[0]
-    return v[:, keep - 1] - v[:, keep] < 2.0 ** -48
+    return v[:, keep - 1] - v[:, keep] <= 2.0 ** -47
 
 
 def test_route_many_tokens_ties_and_masks(dw):
