@@ -1284,7 +1284,12 @@ int run_epi(const void* x, int64_t ldx, const void* w, int64_t ldw, int n, const
   const float t_pair = 5.0f + pv * std::max(0.35f * (float)kt, 1.33f * hbm / pv);
   const few::Plan small = few::plan<EPI>(a, 1, a.m <= 8 ? 1 : 2, 8, hbm);
   const few::Plan large = few::plan<EPI>(a, 2, 4, 2, hbm);
-  if (a.m <= 8) return few::launch<1, 1, 4, 8, EPI>(x, ldx, w, ldw, small, a, stream);
+  // Up to 8 rows always, of w's rows 16 at a time unless a warp has but one step of
+  // many tiles (1 x 512 x 8192: 3.7 us, 2.9 with 32; 1 x 4096 x 4096: 7.1 and 11).
+  if (a.m <= 8)
+    return kt <= few::WARPS && large.us < small.us
+               ? few::launch<2, 4, 1, 2, EPI>(x, ldx, w, ldw, large, a, stream)
+               : few::launch<1, 1, 4, 8, EPI>(x, ldx, w, ldw, small, a, stream);
   if (a.m > 64) best = std::min(best, t_pair);
   const few::Plan& least = small.us < large.us ? small : large;
   if (least.us < best && least.ctas <= INT32_MAX)
