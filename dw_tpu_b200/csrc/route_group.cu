@@ -252,8 +252,8 @@ __device__ __forceinline__ T of_slot(const T (&v)[N], int s) {
   return r;
 }
 
-// KPL: places in a lane's run; WHOLE: every group's lanes use them all;
-// 2^LPT_LOG lanes a token.
+// KPL: places in a lane's run; WHOLE: a lane that has experts uses them all (28
+// experts in runs of 4 leave one lane of eight without any); 2^LPT_LOG lanes a token.
 template <int LD, int KPL, bool WHOLE, int LPT_LOG>
 __global__ void __launch_bounds__(32 * WARPS) route_grouped_kernel(const Args a) {
   using P = Packed<KPL>;
@@ -361,6 +361,10 @@ __global__ void __launch_bounds__(32 * WARPS) route_grouped_kernel(const Args a)
     bool unsure = nan;  // not decided in f32
     uint32_t l[DEEP];
     largest<false>(key, 0u, l);
+    if (count == 0) {
+#pragma unroll
+      for (int j = 0; j < DEEP; ++j) l[j] = 0;
+    }
     auto expert = [&](uint32_t k) { return first + (int)(PLACES - (k & PLACES)); };
 
     // bf16 logits without a bias fit the keys whole; otherwise the values are
@@ -381,8 +385,8 @@ __global__ void __launch_bounds__(32 * WARPS) route_grouped_kernel(const Args a)
                          : (double)P::HIDDEN * fabs(x));
     };
     auto value = [&](uint32_t k) { return exact ? P::value(k & ~PLACES) : choice(expert(k)); };
-    uint32_t m1 = count > 0 ? key32(value(l[0])) : 0u;
-    uint32_t m2 = a.top2 && count > 0 && l[1] ? key32(value(l[1])) : 0u;
+    uint32_t m1 = l[0] ? key32(value(l[0])) : 0u;
+    uint32_t m2 = a.top2 && l[1] ? key32(value(l[1])) : 0u;
     for (int o = (1 << a.lg_log) / 2; o; o >>= 1) {
       const uint32_t n1 = __shfl_xor_sync(0xffffffffu, m1, o),
                      n2 = __shfl_xor_sync(0xffffffffu, m2, o);
@@ -449,7 +453,7 @@ __global__ void __launch_bounds__(32 * WARPS) route_grouped_kernel(const Args a)
     }
 
     // The top k, the largest of the lanes' largest each time.
-    if (!open || count == 0) l[0] = 0;
+    if (!open) l[0] = 0;
     int left = open ? count : 0;  // in l or below it
     const int n_open = a.keep * a.per;
     uint32_t top = 0;  // the last pick's packed value

@@ -1,0 +1,129 @@
+"""route_grouped_topk where choices lie close together, against the order of
+64-bit values: groups that tie exactly, a few near experts among far ones, sums
+of a group that differ by less than f32 holds, scores that f32 cannot hold."""
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+BF, F32, F64 = torch.bfloat16, torch.float32, torch.float64
+SCORINGS = ["softmax", "sigmoid", "sqrtsoftplus"]
+
+
+@pytest.fixture(scope="module")
+def dw():
+    import dw_tpu_b200
+    return dw_tpu_b200
+
+
+@pytest.fixture(autouse=True)
+def _no_device_error():
+    yield
+    from dw_tpu_b200 import _lib
+    _lib.raise_on_device_error()
+
+
+def _scores(x, scoring):
+    if scoring == "softmax":
+        return torch.softmax(x, 1)
+    if scoring == "sigmoid":
+        return 1 / (1 + torch.exp(-x))
+    return (x.clamp(min=0) + torch.log1p(torch.exp(-x.abs()))).sqrt()
+
+
+def _ref(x, k, groups, keep, renorm, scoring, group_score, scale, bias):
+    """(weights, ids, undecided rows) in 64 bits: values descending, ties to the
+    lower index, without a bias by the logits. Undecided: two groups at the border,
+    of different pairs of experts, whose sums lie within 2^-44 of the row's largest
+    |score| + |bias|. A score is off by a few steps of 2^-53 of itself, under softmax
+    by those of a sum of 1024 (some 2^-47), here and in the kernel; the difference of
+    two sums of two such values, twice, by less than 2^-44."""
+    x = x.double().cpu()
+    t, e = x.shape
+    per = e // groups
+    s = _scores(x, scoring)
+    b = torch.zeros(e, dtype=F64) if bias is None else bias.double().cpu()
+    c = x if bias is None else s + b
+    cg = c.reshape(t, groups, per)
+    at = cg.sort(dim=2, descending=True, stable=True)[1][:, :, :1 if group_score == "max" else 2]
+    pairs = x.reshape(t, groups, per).gather(2, at)
+    if group_score == "max":
+        v = cg.amax(2)
+    else:
+        v = (s + b if bias is not None else s).reshape(t, groups, per).gather(2, at).sum(2)
+    by = v.sort(dim=1, descending=True, stable=True)[1]
+    undecided = torch.zeros(t, dtype=torch.bool)
+    if keep < groups and group_score == "top2":
+        rows = torch.arange(t)
+        inside, outside = by[:, keep - 1], by[:, keep]
+        size = (s + b.abs()).amax(1)
+        near = v[rows, inside] - v[rows, outside] <= 2.0 ** -44 * size
+        of = b.expand(t, e).reshape(t, groups, per).gather(2, at)
+        same = ((pairs[rows, inside] == pairs[rows, outside]) &
+                (of[rows, inside] == of[rows, outside])).all(1)
+        undecided = near & ~same
+    open_ = torch.zeros((t, groups), dtype=torch.bool).scatter_(1, by[:, :keep], True)
+    order = c.sort(dim=1, descending=True, stable=True)[1]
+    is_open = open_.repeat_interleave(per, 1).gather(1, order)
+    ids = order.gather(1, (~is_open).to(torch.int8).sort(dim=1, stable=True)[1])[:, :k]
+    w = s.gather(1, ids)
+    if renorm:
+        total = w.sum(1, keepdim=True)
+        w = torch.where(total == 0, torch.zeros_like(w), w / total)
+    return w * scale, ids.int(), undecided
+
+
+def _check(dw, x, k, groups, keep, scoring="sigmoid", group_score="top2", bias=None, renorm=True,
+           scale=2.5):
+    w, ids = dw.route_grouped_topk(x, k, groups, keep, renorm, scoring, group_score, scale, F32,
+                                   bias)
+    rw, ri, undecided = _ref(x, k, groups, keep, renorm, scoring, group_score, scale, bias)
+    assert int(undecided.sum()) <= len(x) // 20
+    sure = ~undecided
+    wrong = (ids.cpu() != ri).any(1) & sure
+    assert not wrong.any(), (
+        f"{int(wrong.sum())} of {len(x)} tokens, first {int(wrong.nonzero()[0])}: "
+        f"{ids[wrong.nonzero()[0]].tolist()} for {ri[wrong.nonzero()[0]].tolist()}")
+    # Steps of f32 (2^-24) of a weight: 4 of expf, 1 each of 1 + e, the division, the
+    # renormalisation and the scale; of a total of at most 32 such weights as many and 8
+    # more; of a softmax's sum 4 of expf, the mean size of its exponents (ln 256 at
+    # most) and some 10 additions. Below 2^5.
+    err = (w.cpu().double() - rw).abs()[sure]
+    assert bool((err <= 2.0 ** -19 * rw[sure].abs() + 1e-37).all()), float(err.max())
+    return w, ids
+
+
+def _steps(value, n):
+    """The f32 numbers 0, 1, .. n - 1 steps above ``value``."""
+    return (torch.tensor(value).view(torch.int32) + torch.arange(n, dtype=torch.int32)).view(F32)
+
+
+@pytest.mark.parametrize("e,groups", [(112, 4), (84, 3), (104, 2), (112, 2), (120, 2), (240, 2),
+                                      (56, 2), (28, 1)])
+@pytest.mark.parametrize("scoring", SCORINGS)
+def test_groups_that_tie_where_lanes_are_left_over(dw, e, groups, scoring):
+    """Groups that the lanes of a warp do not share out evenly, logits of four values:
+    most tokens have two groups of one value."""
+    g = torch.Generator().manual_seed(e + groups)
+    level = torch.tensor([0.0, 0.0, 0.0, 0.5, 0.75, 1.0])
+    for t in (1, 200):
+        x = level[torch.randint(0, 6, (t, e), generator=g)] * (torch.rand((t, e), generator=g) < 0.2)
+        x = x.cuda()
+        for bias in (None, torch.full((e,), 0.25, device="cuda"),
+                     (torch.randint(0, 2, (e,), generator=g) * 0.5).cuda()):
+            for gs in ("max", "top2"):
+                if gs == "top2" and bias is not None and bias.unique().numel() > 1:
+                    continue  # (sums of unlike scores and biases tie by rounding)
+                for keep in range(1, groups + 1):
+                    for k in (1, 4):
+                        _check(dw, x, k, groups, keep, scoring, gs, bias)
+
+
+def test_empty_lanes_add_no_expert_to_a_group(dw):
+    x = torch.zeros((1, 112))
+    x[0, 0], x[0, 1] = 1.0, 0.5
+    x[0, 28] = x[0, 56] = 1.0
+    x[0, 29] = x[0, 57] = 0.75
+    _, ids = _check(dw, x.cuda(), 1, 4, 1)
+    assert ids.item() == 28
