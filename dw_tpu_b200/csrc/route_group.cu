@@ -19,6 +19,7 @@
 // single token takes 3.9 us of dependent instructions, 32771 tokens of 160
 // experts 20 us where their bytes take 3.4 (in 64 bits throughout: 83).
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
 
@@ -194,6 +195,7 @@ __device__ __forceinline__ float score32(float x, int scoring, float mx, float i
 // to 2^bits steps off the value.
 template <int KPL>
 struct Packed {
+  using Set = std::conditional_t<KPL <= 32, uint32_t, uint64_t>;  // of places
   static constexpr uint32_t PLACES = KPL <= 32 ? 31 : 63;
   // The difference of two values that packing may hide, of the larger.
   static constexpr float HIDDEN = (KPL <= 32 ? 2.0f : 4.0f) / 262144.0f;
@@ -455,6 +457,7 @@ __global__ void __launch_bounds__(32 * WARPS) route_grouped_kernel(const Args a)
     // The top k, the largest of the lanes' largest each time.
     if (!open) l[0] = 0;
     int left = open ? count : 0;  // in l or below it
+    typename P::Set gone = 0;     // the places that are picked
     const int n_open = a.keep * a.per;
     uint32_t top = 0;  // the last pick's packed value
     int last_id = 0, slot_id[NS] = {};
@@ -470,6 +473,7 @@ __global__ void __launch_bounds__(32 * WARPS) route_grouped_kernel(const Args a)
       uint32_t taken = 0;
       if (lane == winner) {
         taken = l[0];
+        gone |= (typename P::Set)1 << (PLACES - (taken & PLACES));
 #pragma unroll
         for (int j = 0; j + 1 < DEEP; ++j) l[j] = l[j + 1];
         l[DEEP - 1] = 0;
@@ -481,34 +485,49 @@ __global__ void __launch_bounds__(32 * WARPS) route_grouped_kernel(const Args a)
         if (empty) largest<true>(key, taken, l);
       }
     };
-    const int rounds = a.top_k + (!exact && a.top_k < n_open);
+    // Packed values x <= last whose order packing or f32 may hide.
+    auto near = [&](float last, float x) {
+      return !(last - x > (biased ? (2.0f * MARGIN + P::HIDDEN) * size
+                                  : P::HIDDEN * fmaxf(fabsf(x), fabsf(last))));
+    };
+    // Whether the choice of expert e certainly comes before that of f, which has
+    // the higher index if they tie.
+    auto ahead = [&](int e, int f) {
+      const float p = choice(e), q = choice(f);
+      if (biased ? p - q > 2.0f * MARGIN * size : p > q) return true;
+      // Equal logits and biases are a tie in 64 bits too.
+      return load_logit<LD>(a.logits, row + e) == load_logit<LD>(a.logits, row + f) &&
+             (!biased || a.bias[e] == a.bias[f]);
+    };
     bool close = false;
     float last = 0.0f;
-    for (int k = 0; k < rounds; ++k) {
+    for (int k = 0; k < a.top_k; ++k) {
       const int before = last_id;
       pick(k);
       if (!exact) {
         const float x = P::value(top);
-        const float far = biased ? (2.0f * MARGIN + P::HIDDEN) * size
-                                 : P::HIDDEN * fmaxf(fabsf(x), fabsf(last));
-        if (k > 0 && !(last - x > far)) {
-          const float p = choice(before), q = choice(last_id);
-          bool sure = biased ? p - q > 2.0f * MARGIN * size : p > q;
-          // Equal logits and biases are a tie in 64 bits too.
-          if (!sure)
-            sure = load_logit<LD>(a.logits, row + before) ==
-                       load_logit<LD>(a.logits, row + last_id) &&
-                   (!biased || a.bias[before] == a.bias[last_id]);
-          close |= !sure;
-        }
+        if (k > 0 && near(last, x)) close |= !ahead(before, last_id);
         last = x;
+      }
+    }
+    // What is left comes after the last pick: its largest packed value clearly, or
+    // each expert by itself (of one packed value the largest need not be the first).
+    if (!exact && a.top_k < n_open) {
+      const bool cut = near(last, P::value(seg_max<lpt>(l[0] & ~PLACES)));
+      if (__any_sync(0xffffffffu, cut && real)) {
+        bool sure = true;
+        if (cut && l[0] && near(last, P::value(l[0])))
+          for (int i = 0; i < count; ++i)
+            if (!(gone >> i & 1)) sure = sure && ahead(last_id, first + i);
+        close |= (__ballot_sync(0xffffffffu, !sure) & seg_mask) != 0;
       }
     }
     if (__any_sync(0xffffffffu, close && real)) {
       // Up to three picks more, then all of them in the order of their 64-bit
       // values; what was not picked has to be below the last that is chosen.
       const int all = min(min(a.top_k + 4, n_open), NS * lpt);
-      for (int k = rounds; k < all; ++k) pick(k);
+      for (int k = a.top_k; k < all; ++k) pick(k);
+      const uint32_t rest = all < n_open ? seg_max<lpt>(l[0] & ~PLACES) : 0u;
       double c[NS];
       int place[NS] = {}, id[NS];
 #pragma unroll
@@ -534,7 +553,7 @@ __global__ void __launch_bounds__(32 * WARPS) route_grouped_kernel(const Args a)
           if (to == j * lpt + sl) id[j] = e;
       }
       if (close) {
-        unsure |= !settles || (all < n_open && !(least > bound(top)));
+        unsure |= !settles || (rest && !(least > bound(rest)));
 #pragma unroll
         for (int j = 0; j < NS; ++j) slot_id[j] = id[j];
       }

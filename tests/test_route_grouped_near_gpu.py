@@ -127,3 +127,63 @@ def test_empty_lanes_add_no_expert_to_a_group(dw):
     x[0, 29] = x[0, 57] = 0.75
     _, ids = _check(dw, x.cuda(), 1, 4, 1)
     assert ids.item() == 28
+
+
+@pytest.mark.parametrize("steps", [(2, 1, 3), (1, 1, 2), (3, 1, 5), (0, 0, 1, 4), (4, 0, 2, 7)])
+@pytest.mark.parametrize("e,groups", [(32, 1), (256, 8), (512, 1), (1024, 4)])
+def test_experts_of_one_lane_steps_apart(dw, steps, e, groups):
+    """The experts left after the last pick decide too, not the first of them alone."""
+    near = _steps(1.0, 8)
+    for at in (0, 5, e // groups - 4):
+        x = torch.full((1, e), 0.5)
+        for j, s in enumerate(steps):
+            x[0, at + j] = near[s]
+        for t in (1, 2001):
+            y = x.expand(t, e).cuda()
+            for k in (1, 2, 3):
+                for scoring in SCORINGS:
+                    _check(dw, y.contiguous(), k, groups, groups, scoring, "max")
+    zero = torch.zeros(e, device="cuda")
+    x = torch.full((1, e), -1.0, dtype=BF)
+    x[0, :3] = torch.tensor([11.0, 11.0, 11.0625])  # sigmoids 1.0e-6 apart
+    for k in (1, 2, 3):
+        _check(dw, x.cuda(), k, groups, groups, bias=zero)
+
+
+def _near_among_far(seed, t, e, top_k, run=None):
+    """Tokens of far logits with 2 to 4 within 7 steps of 1 across the cut at top_k, within
+    ``run`` neighbours or anywhere, and the larger ones well above."""
+    g = torch.Generator().manual_seed(seed)
+    x = -2 * torch.rand((t, e), generator=g)
+    near = _steps(1.0, 8)
+    for i in range(t):
+        n = int(torch.randint(2, 5, (1,), generator=g))
+        below = int(torch.randint(1, min(top_k, n - 1) + 1, (1,), generator=g))
+        places = torch.randperm(e, generator=g)
+        if run:
+            first = int(torch.randint(0, e // run, (1,), generator=g)) * run
+            inside = first + torch.randperm(run, generator=g)[:n]
+            rest = places[(places < first) | (places >= first + run)]
+            places = torch.cat([inside, rest])
+        x[i, places[:n]] = near[torch.randint(0, 8, (n,), generator=g)]
+        larger = top_k - below
+        x[i, places[n:n + larger]] = 2 + torch.randperm(32, generator=g)[:larger] / 8
+    return x
+
+
+@pytest.mark.parametrize("top_k", [1, 2, 8])
+@pytest.mark.parametrize("t", [1, 200, 2001])
+@pytest.mark.parametrize("e,groups,run", [(256, 8, 8), (256, 8, None), (128, 1, 16), (160, 8, 20),
+                                          (64, 4, None)])
+def test_near_experts_among_far_ones(dw, top_k, t, e, groups, run):
+    x = _near_among_far(top_k + t + e, max(t, 60), e, top_k, run)
+    flat = torch.full((e,), 0.25)
+    one = torch.zeros(e)
+    one[::3] = 2.0 ** -20
+    tokens = [x.cuda()] if t > 1 else [row[None].cuda() for row in x]
+    for y in tokens:
+        for scoring in SCORINGS:
+            for gs in ("max", "top2"):
+                _check(dw, y, top_k, groups, groups, scoring, gs)
+                _check(dw, y, top_k, groups, groups, scoring, gs, flat.cuda())
+        _check(dw, y, top_k, groups, groups, bias=one.cuda())
