@@ -353,12 +353,15 @@ __global__ void __launch_bounds__(32 * WARPS) route_grouped_kernel(const Args a)
         choices(DWM_SCORE_SQRTSOFTPLUS);
       size = seg_max<lpt>(size);
     }
-    uint32_t key[KPL];
+    // A lane's two largest, exact; its keys.
+    uint32_t key[KPL], m1 = 0, m2 = 0;
 #pragma unroll
     for (int i = 0; i < KPL; ++i) {
       nan |= isnan(v[i]);
-      const uint32_t k = (key32(v[i]) & ~PLACES) | (PLACES - (uint32_t)i);
-      key[i] = has(i) ? k : 0u;
+      const uint32_t k = has(i) ? key32(v[i]) : 0u;
+      m2 = max(m2, min(m1, k));
+      m1 = max(m1, k);
+      key[i] = has(i) ? (k & ~PLACES) | (PLACES - (uint32_t)i) : 0u;
     }
     bool unsure = nan;  // not decided in f32
     uint32_t l[DEEP];
@@ -366,6 +369,7 @@ __global__ void __launch_bounds__(32 * WARPS) route_grouped_kernel(const Args a)
     if (count == 0) {
 #pragma unroll
       for (int j = 0; j < DEEP; ++j) l[j] = 0;
+      m1 = m2 = 0;
     }
     auto expert = [&](uint32_t k) { return first + (int)(PLACES - (k & PLACES)); };
 
@@ -386,9 +390,6 @@ __global__ void __launch_bounds__(32 * WARPS) route_grouped_kernel(const Args a)
       return x + (biased ? (double)(2.0f * MARGIN + P::HIDDEN) * size
                          : (double)P::HIDDEN * fabs(x));
     };
-    auto value = [&](uint32_t k) { return exact ? P::value(k & ~PLACES) : choice(expert(k)); };
-    uint32_t m1 = l[0] ? key32(value(l[0])) : 0u;
-    uint32_t m2 = a.top2 && l[1] ? key32(value(l[1])) : 0u;
     for (int o = (1 << a.lg_log) / 2; o; o >>= 1) {
       const uint32_t n1 = __shfl_xor_sync(0xffffffffu, m1, o),
                      n2 = __shfl_xor_sync(0xffffffffu, m2, o);

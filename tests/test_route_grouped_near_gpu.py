@@ -187,3 +187,63 @@ def test_near_experts_among_far_ones(dw, top_k, t, e, groups, run):
                 _check(dw, y, top_k, groups, groups, scoring, gs)
                 _check(dw, y, top_k, groups, groups, scoring, gs, flat.cuda())
         _check(dw, y, top_k, groups, groups, bias=one.cuda())
+
+
+@pytest.mark.parametrize("e,groups,keep", [(256, 8, 8), (256, 8, 4), (160, 8, 3), (256, 1, 1)])
+@pytest.mark.parametrize("offset", [50.0, -50.0, 1000.0])
+def test_a_common_offset_of_the_logits(dw, e, groups, keep, offset):
+    """Softmax scores are those without the offset; the logits' steps are 4e-6 to 6e-5."""
+    g = torch.Generator().manual_seed(int(offset) + e)
+    x = (torch.randn((1500, e), generator=g) * 1e-3 + offset).cuda()
+    spread = (torch.randn((1500, e), generator=g) * 1.5 + offset).cuda()
+    b = (torch.randn(e, generator=g) * 0.01).cuda()
+    for y in (x, spread):
+        for k in (1, 2, 4, 8):
+            _check(dw, y, k, groups, keep, "softmax", "max")
+        _check(dw, y, 8, groups, keep, "softmax", "top2")
+        _check(dw, y, 8, groups, keep, "softmax", "top2", b, scale=1.0)
+
+
+def _near_groups(seed, t, e, groups):
+    """Groups whose largest lie 0 to 6 steps apart, each with a second one as near."""
+    g = torch.Generator().manual_seed(seed)
+    per = e // groups
+    x = -1 - torch.rand((t, groups, per), generator=g)
+    near = _steps(1.0, 7)
+    for i in range(t):
+        for q in range(groups):
+            if torch.rand((), generator=g) < 0.6:
+                n = min(per, int(torch.randint(1, 4, (1,), generator=g)))
+                first = int(torch.randint(0, per - n + 1, (1,), generator=g))
+                x[i, q, first:first + n] = near[torch.randint(0, 7, (n,), generator=g)]
+    return x.reshape(t, e)
+
+
+@pytest.mark.parametrize("e,groups,keep,k", [(160, 8, 1, 1), (256, 8, 4, 8), (256, 8, 1, 2),
+                                             (64, 16, 5, 4), (1024, 4, 2, 8), (96, 3, 1, 1)])
+@pytest.mark.parametrize("t", [100, 2001])
+def test_groups_whose_best_are_steps_apart(dw, e, groups, keep, k, t):
+    x = _near_groups(e + keep, t, e, groups).cuda()
+    b = torch.full((e,), 0.25, device="cuda")
+    for scoring in SCORINGS:
+        _check(dw, x, k, groups, keep, scoring, "max")
+        _check(dw, x, k, groups, keep, scoring, "max", b)
+
+
+@pytest.mark.parametrize("top_k", [1, 2, 8])
+@pytest.mark.parametrize("e,groups", [(256, 8), (160, 8), (96, 3)])
+def test_near_experts_with_a_group_closed(dw, top_k, e, groups):
+    x = _near_among_far(top_k + e, 2001, e, top_k).cuda()
+    for scoring in SCORINGS:
+        for keep in (groups - 1, max(1, groups // 2)):
+            _check(dw, x, top_k, groups, keep, scoring, "max")
+            _check(dw, x[:200], top_k, groups, keep, scoring, "max")
+
+
+def test_the_largest_of_a_group_and_not_its_first(dw):
+    near = _steps(1.0, 8)
+    for t in (1, 2001):
+        x = torch.full((t, 160), 0.5)
+        x[:, 0], x[:, 1], x[:, 20] = near[0], near[5], near[3]
+        _, ids = _check(dw, x.cuda(), 1, 8, 1, group_score="max")
+        assert bool((ids == 1).all())
