@@ -254,10 +254,17 @@ __device__ __forceinline__ T of_slot(const T (&v)[N], int s) {
   return r;
 }
 
+// CTAs an SM whose registers fit at once: many tokens are bound by instruction issue
+// and gain from more warps (72 registers for runs of up to 24: 32771 tokens of 160
+// experts 20.1 us, with 96 22.3; 96 for longer ones: 32768 of 256 27.4 us, with 128
+// 29.9), few tokens by latency alone.
+constexpr int resident(int kpl, int lpt_log) { return lpt_log != 3 ? 1 : kpl <= 24 ? 14 : 10; }
+
 // KPL: places in a lane's run; WHOLE: a lane that has experts uses them all (28
 // experts in runs of 4 leave one lane of eight without any); 2^LPT_LOG lanes a token.
 template <int LD, int KPL, bool WHOLE, int LPT_LOG>
-__global__ void __launch_bounds__(32 * WARPS) route_grouped_kernel(const Args a) {
+__global__ void __launch_bounds__(32 * WARPS, resident(KPL, LPT_LOG))
+    route_grouped_kernel(const Args a) {
   using P = Packed<KPL>;
   constexpr uint32_t PLACES = P::PLACES;
   constexpr int NS = 32 >> LPT_LOG;  // picks a lane holds (top_k is at most 32)
@@ -366,11 +373,7 @@ __global__ void __launch_bounds__(32 * WARPS) route_grouped_kernel(const Args a)
     bool unsure = nan;  // not decided in f32
     uint32_t l[DEEP];
     largest<false>(key, 0u, l);
-    if (count == 0) {
-#pragma unroll
-      for (int j = 0; j < DEEP; ++j) l[j] = 0;
-      m1 = m2 = 0;
-    }
+    if (count == 0) m1 = m2 = 0;
     auto expert = [&](uint32_t k) { return first + (int)(PLACES - (k & PLACES)); };
 
     // bf16 logits without a bias fit the keys whole; otherwise the values are
@@ -427,12 +430,12 @@ __global__ void __launch_bounds__(32 * WARPS) route_grouped_kernel(const Args a)
         double c[4], d1 = -INFINITY, d2 = -INFINITY;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          c[j] = l[j] ? choice64(expert(l[j])) : -INFINITY;
+          c[j] = count > 0 && l[j] ? choice64(expert(l[j])) : -INFINITY;
           d2 = fmax(d2, fmin(d1, c[j]));
           d1 = fmax(d1, c[j]);
         }
         // A fifth that may be one of the two largest: not settled.
-        bool sure = settles && (!l[4] || (a.top2 ? d2 : d1) > bound(l[4]));
+        bool sure = settles && (count == 0 || !l[4] || (a.top2 ? d2 : d1) > bound(l[4]));
         for (int o = (1 << a.lg_log) / 2; o; o >>= 1) {
           const double n1 = __shfl_xor_sync(0xffffffffu, d1, o),
                        n2 = __shfl_xor_sync(0xffffffffu, d2, o);
@@ -456,7 +459,7 @@ __global__ void __launch_bounds__(32 * WARPS) route_grouped_kernel(const Args a)
     }
 
     // The top k, the largest of the lanes' largest each time.
-    if (!open) l[0] = 0;
+    if (!open || count == 0) l[0] = 0;
     int left = open ? count : 0;  // in l or below it
     typename P::Set gone = 0;     // the places that are picked
     const int n_open = a.keep * a.per;
@@ -502,33 +505,44 @@ __global__ void __launch_bounds__(32 * WARPS) route_grouped_kernel(const Args a)
     };
     bool close = false;
     float last = 0.0f;
-    for (int k = 0; k < a.top_k; ++k) {
-      const int before = last_id;
-      pick(k);
-      if (!exact) {
-        const float x = P::value(top);
-        if (k > 0 && near(last, x)) close |= !ahead(before, last_id);
-        last = x;
+    int picks = a.top_k, k = 0;
+    uint32_t rest = 0;  // the largest packed value that is left
+    bool settling = false;
+    while (true) {
+      for (; k < picks; ++k) {
+        const int before = last_id;
+        pick(k);
+        if (!exact) {
+          const float x = P::value(top);
+          if (k > 0 && near(last, x)) close |= k < a.top_k && !ahead(before, last_id);
+          last = x;
+        }
       }
-    }
-    // What is left comes after the last pick: its largest packed value clearly, or
-    // each expert by itself (of one packed value the largest need not be the first).
-    if (!exact && a.top_k < n_open) {
-      const bool cut = near(last, P::value(seg_max<lpt>(l[0] & ~PLACES)));
+      if (exact) break;
+      rest = picks < n_open ? seg_max<lpt>(l[0] & ~PLACES) : 0u;
+      if (settling) break;
+      // What is left comes after the last pick: its largest packed value clearly, or
+      // each expert by itself (of one packed value the largest need not be the first).
+      const bool cut = rest && near(last, P::value(rest));
       if (__any_sync(0xffffffffu, cut && real)) {
         bool sure = true;
-        if (cut && l[0] && near(last, P::value(l[0])))
-          for (int i = 0; i < count; ++i)
-            if (!(gone >> i & 1)) sure = sure && ahead(last_id, first + i);
+        if (cut && l[0] && near(last, P::value(l[0]))) {
+          sure = ahead(last_id, expert(l[0]));
+          // (What is near and not in the list comes after what is.)
+          if (sure && left > 1 && (!l[1] || near(last, P::value(l[1]))))
+            for (int i = 0; i < count; ++i)
+              if (!(gone >> i & 1)) sure = sure && ahead(last_id, first + i);
+        }
         close |= (__ballot_sync(0xffffffffu, !sure) & seg_mask) != 0;
       }
+      settling = __any_sync(0xffffffffu, close && real);
+      if (!settling) break;
+      picks = min(min(a.top_k + 4, n_open), NS * lpt);
     }
-    if (__any_sync(0xffffffffu, close && real)) {
-      // Up to three picks more, then all of them in the order of their 64-bit
+    if (settling) {
+      // Up to four picks more, then all of them in the order of their 64-bit
       // values; what was not picked has to be below the last that is chosen.
-      const int all = min(min(a.top_k + 4, n_open), NS * lpt);
-      for (int k = a.top_k; k < all; ++k) pick(k);
-      const uint32_t rest = all < n_open ? seg_max<lpt>(l[0] & ~PLACES) : 0u;
+      const int all = picks;
       double c[NS];
       int place[NS] = {}, id[NS];
 #pragma unroll
@@ -562,13 +576,21 @@ __global__ void __launch_bounds__(32 * WARPS) route_grouped_kernel(const Args a)
 
     // Weights: slot s of lane sl is the pick s * lpt + sl.
     float w[NS], total = 0.0f;
+    auto weights = [&](int scoring) {
 #pragma unroll
-    for (int s = 0; s < NS; ++s) {
-      w[s] = 0.0f;
-      if (s * lpt + sl < a.top_k)
-        w[s] = score32<true>(load_logit<LD>(a.logits, row + slot_id[s]), a.scoring, mx, inv_sum);
-      total += w[s];
-    }
+      for (int s = 0; s < NS; ++s) {
+        w[s] = 0.0f;
+        if (s * lpt + sl < a.top_k)
+          w[s] = score32<true>(load_logit<LD>(a.logits, row + slot_id[s]), scoring, mx, inv_sum);
+        total += w[s];
+      }
+    };
+    if (a.scoring == DWM_SCORE_SOFTMAX)
+      weights(DWM_SCORE_SOFTMAX);
+    else if (a.scoring == DWM_SCORE_SIGMOID)
+      weights(DWM_SCORE_SIGMOID);
+    else
+      weights(DWM_SCORE_SQRTSOFTPLUS);
     if (a.renorm) total = seg_sum<lpt>(total);
     // What one lane of a token is unsure of, all are.
     const uint32_t doubts = __ballot_sync(0xffffffffu, unsure && real && in_group);
