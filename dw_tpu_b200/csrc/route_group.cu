@@ -175,20 +175,41 @@ __device__ __forceinline__ float value32(uint32_t key) {
   return __uint_as_float(key >> 31 ? key ^ 0x80000000u : ~key);
 }
 
-// The f32 score, for the weights (FULL) to a few steps of itself. For the order
-// it and its sum with a bias are off by less than MARGIN / 2 of the largest
-// |score| + |bias|: expf and division by a few steps (2^-24 each), the exponent's
-// own rounding by 2^-24 |x| where the score's slope is at most 1 / (4 |x|), and
-// for softmax the sum over the experts by 2^-21.
-constexpr float MARGIN = 1e-6f;
+// The f32 score; FULL: for the weights, else for the choices, with the division of
+// two steps.
 template <bool FULL>
 __device__ __forceinline__ float score32(float x, int scoring, float mx, float inv_sum) {
   // (mx is 0 where every logit is -inf.)
   if (scoring == DWM_SCORE_SOFTMAX) return expf(x == mx ? 0.0f : x - mx) * inv_sum;
   if (scoring == DWM_SCORE_SIGMOID)
-    return FULL ? 1.0f / (1.0f + expf(-x)) : sigmoid_fast(x);
+    return FULL ? 1.0f / (1.0f + expf(-x)) : __fdividef(1.0f, 1.0f + expf(-x));
   return sqrtf(fmaxf(x, 0.0f) + log1pf(expf(-fabsf(x))));
 }
+
+// How far apart two choices, or two sums of two, have to be for their f32 order to
+// be that of 64 bits, in units u = 2^-24 of the token's largest |score| + |bias|.
+// A choice is off by
+//   sigmoid       10: expf 4 (2 ulp), 1 + e 1, __fdividef 4, the bias 1
+//   sqrtsoftplus   7: half of (expf 4, log1pf 4, their sum 1), the root 1, the bias 1
+//   softmax        7: expf 4, the exponent |d| e^-|d| < 1, the product 1, the bias 1;
+//                     and all of a token's alike, by the sum over the experts, expf 4,
+//                     the exponents ln 1024 (their mean size is below that), the
+//                     additions in sequence and the reciprocal 1
+// Two sums of two of them differ by four such errors (the common one twice), and by 4
+// for the additions. Scores below FLOOR are not measured by themselves: of a
+// sqrtsoftplus down there f32 holds no more than 4e-23.
+constexpr float UNIT = 1.0f / 16777216.0f;
+constexpr float FLOOR = 1e-15f;
+template <int KPL, int LPT_LOG>
+__device__ __forceinline__ float margin_of(int scoring) {
+  constexpr int ADDS = KPL + LPT_LOG;  // of a lane's and of the lanes'
+  return scoring == DWM_SCORE_SOFTMAX ? (4 * 7 + 2 * (4 + 7 + ADDS + 1) + 4) * UNIT
+                                      : (4 * 10 + 4 + 2) * UNIT;
+}
+// Without a bias a sum of two scores is off relative to itself, in the same units by
+// 6, of a softmax by 5 and the size of its exponent, which above FLOOR is at most 35;
+// of two of them twice that, with room.
+constexpr float RELATIVE = 128 * UNIT;
 
 // Within a lane the keys are made unique: their low bits, as many as KPL places
 // take, are the place in the run, the lowest place the largest. That takes up
@@ -341,7 +362,8 @@ __global__ void __launch_bounds__(32 * WARPS, resident(KPL, LPT_LOG))
         inv_sum = sum > 0.0f ? 1.0f / sum : 1.0f;
       }
     }
-    float size = 0.0f;  // the largest |score| + |bias|
+    float size = FLOOR;  // the largest |score| + |bias|
+    auto margin = [&] { return margin_of<KPL, LPT_LOG>(a.scoring) * size; };
     if (biased) {
       auto choices = [&](int scoring) {
 #pragma unroll
@@ -390,7 +412,7 @@ __global__ void __launch_bounds__(32 * WARPS, resident(KPL, LPT_LOG))
     // What the values of a lane's packed keys up to k are below, in 64 bits.
     auto bound = [&](uint32_t k) {
       const double x = P::value(k & ~PLACES);
-      return x + (biased ? (double)(2.0f * MARGIN + P::HIDDEN) * size
+      return x + (biased ? (double)margin() + (double)P::HIDDEN * size
                          : (double)P::HIDDEN * fabs(x));
     };
     for (int o = (1 << a.lg_log) / 2; o; o >>= 1) {
@@ -421,10 +443,8 @@ __global__ void __launch_bounds__(32 * WARPS, resident(KPL, LPT_LOG))
     if (a.keep < a.groups && (biased || a.top2)) {
       const float in = value32(~seg_max<lpt>(open ? ~gkey : 0u));  // the least of the open
       const float out = value32(seg_max<lpt>(in_group && !open ? gkey : 0u));
-      // (Without a bias a sum of two scores is off relative to itself, unless it
-      // is next to the f32 underflow.)
-      const bool close = biased ? !(in - out > 2.0f * MARGIN * size)
-                                : !(in > 1e-30f && in - out > 16.0f * MARGIN * in);
+      const bool close = biased ? !(in - out > margin())
+                                : !(in > FLOOR && in - out > RELATIVE * in);
       if (__any_sync(0xffffffffu, close && real)) {
         // The groups' values in 64 bits, from each lane's first four.
         double c[4], d1 = -INFINITY, d2 = -INFINITY;
@@ -491,14 +511,14 @@ __global__ void __launch_bounds__(32 * WARPS, resident(KPL, LPT_LOG))
     };
     // Packed values x <= last whose order packing or f32 may hide.
     auto near = [&](float last, float x) {
-      return !(last - x > (biased ? (2.0f * MARGIN + P::HIDDEN) * size
+      return !(last - x > (biased ? margin() + P::HIDDEN * size
                                   : P::HIDDEN * fmaxf(fabsf(x), fabsf(last))));
     };
     // Whether the choice of expert e certainly comes before that of f, which has
     // the higher index if they tie.
     auto ahead = [&](int e, int f) {
       const float p = choice(e), q = choice(f);
-      if (biased ? p - q > 2.0f * MARGIN * size : p > q) return true;
+      if (biased ? p - q > margin() : p > q) return true;
       // Equal logits and biases are a tie in 64 bits too.
       return load_logit<LD>(a.logits, row + e) == load_logit<LD>(a.logits, row + f) &&
              (!biased || a.bias[e] == a.bias[f]);

@@ -2,6 +2,8 @@
 64-bit values: groups that tie exactly, a few near experts among far ones, sums
 of a group that differ by less than f32 holds, scores that f32 cannot hold."""
 
+import math
+
 import pytest
 import torch
 
@@ -247,3 +249,57 @@ def test_the_largest_of_a_group_and_not_its_first(dw):
         x[:, 0], x[:, 1], x[:, 20] = near[0], near[5], near[3]
         _, ids = _check(dw, x.cuda(), 1, 8, 1, group_score="max")
         assert bool((ids == 1).all())
+
+
+@pytest.mark.parametrize("e,groups,keep", [(256, 8, 4), (160, 8, 3), (1024, 1, 1)])
+@pytest.mark.parametrize("low", [-12.0, -30.0, -60.0, -95.0])
+def test_biases_as_small_as_the_scores(dw, e, groups, keep, low):
+    """Strongly negative logits: the scores are e^low, and so are the biases, so that the
+    error of the exponential counts whole."""
+    g = torch.Generator().manual_seed(int(-low) + e)
+    x = (low + torch.rand((4000, e), generator=g) * 0.5).cuda()
+    for scoring in ("sigmoid", "sqrtsoftplus"):
+        size = math.exp(low if scoring == "sigmoid" else low / 2)
+        b = (torch.rand(e, generator=g, dtype=F64) * size).to(F32).cuda()
+        for gs in ("max", "top2"):
+            _check(dw, x, 8, groups, keep, scoring, gs, b)
+
+
+def _two_choices(seed, t, e, low, scoring):
+    """(logits, biases): two experts of each token whose choices differ by less than a step
+    of the larger logit, by way of biases a thousandth of the scores; the others far below."""
+    g = torch.Generator().manual_seed(seed)
+    score = (lambda v: 1 / (1 + torch.exp(-v))) if scoring == "sigmoid" else (
+        lambda v: torch.log1p(torch.exp(v)).sqrt())
+    per = 1 if scoring == "sigmoid" else 2  # log score is about the logit / per
+    b = (torch.rand(e, generator=g, dtype=F64) * float(score(torch.tensor(low, dtype=F64))) *
+         1e-3).to(F32)
+    x = torch.full((t, e), low - 3, dtype=F32)
+    i, j = torch.rand((t, e), generator=g).topk(2, dim=1)[1].unbind(1)
+    rows = torch.arange(t)
+    x[rows, i] = low + torch.rand(t, generator=g) * 0.01
+    want = score(x[rows, i].double()) + b[i].double() - b[j].double()
+    v = x[rows, i].double()
+    for _ in range(8):
+        v = v + per * torch.log(want / score(v))
+    x[rows, j] = v.to(F32)
+    return x, b
+
+
+@pytest.mark.parametrize("low", [-6.0, -20.0, -40.0, -60.0, -80.0])
+@pytest.mark.parametrize("scoring", ["sigmoid", "sqrtsoftplus"])
+def test_two_near_choices_of_tiny_scores(dw, scoring, low):
+    x, b = _two_choices(int(-low), 4000, 256, low, scoring)
+    for groups, keep in ((1, 1), (8, 8), (8, 1)):
+        _check(dw, x.cuda(), 1, groups, keep, scoring, "max", b.cuda())
+        _check(dw, x[:500].cuda(), 1, groups, keep, scoring, "max", b.cuda())
+
+
+def test_many_experts_under_a_biased_softmax(dw):
+    """The sum over all the experts is in every choice."""
+    g = torch.Generator().manual_seed(5)
+    for e, groups, keep in ((1024, 1, 1), (1024, 8, 4), (256, 8, 4)):
+        x = (torch.randn((4000, e), generator=g) * 2).cuda()
+        b = (torch.randn(e, generator=g) / e).cuda()
+        for gs in ("max", "top2"):
+            _check(dw, x, 8, groups, keep, "softmax", gs, b)
