@@ -14,8 +14,9 @@
 // f32 and note how far apart the values are where a choice was made. Where two
 // are closer than the f32 error (a few tokens in a hundred for random logits),
 // the groups or the picks in question are compared in 64 bits; a token that
-// this does not settle is done again in 64 bits by the whole warp (8-12 us, which
-// one token of 1024 would make the time of all). Bound: instruction issue; a
+// this does not settle, or one of whose weights f32 does not hold, is done again
+// in 64 bits by the whole warp (8-12 us, which one token of 1024 would make the
+// time of all). Bound: instruction issue; a
 // single token takes 3.9 us of dependent instructions, 32771 tokens of 160
 // experts 20 us where their bytes take 3.4 (in 64 bits throughout: 83).
 #include <algorithm>
@@ -184,6 +185,21 @@ __device__ __forceinline__ float score32(float x, int scoring, float mx, float i
   if (scoring == DWM_SCORE_SIGMOID)
     return FULL ? 1.0f / (1.0f + expf(-x)) : __fdividef(1.0f, 1.0f + expf(-x));
   return sqrtf(fmaxf(x, 0.0f) + log1pf(expf(-fabsf(x))));
+}
+
+// The weight: score32 with the rounding of a softmax's exponent made good (it is as
+// many units as the exponent is large).
+__device__ __forceinline__ float weight32(float x, int scoring, float mx, float inv_sum) {
+  const float s = score32<true>(x, scoring, mx, inv_sum);
+  if (scoring != DWM_SCORE_SOFTMAX) return s;
+  const float d = x - mx, t = d - x, off = (x - (d - t)) - (mx + t);  // x - mx = d + off
+  return fabsf(d) < INFINITY ? fmaf(s, off, s) : s;
+}
+// Logits (under a softmax, to its maximum) whose scores f32 does not hold to its full
+// precision, and 64 bits do.
+__device__ __forceinline__ bool faint(float x, int scoring, float mx) {
+  const float d = scoring == DWM_SCORE_SOFTMAX ? x - mx : x;
+  return d < -80.0f && d > -1500.0f;
 }
 
 // How far apart two choices, or two sums of two, have to be for their f32 order to
@@ -596,12 +612,16 @@ __global__ void __launch_bounds__(32 * WARPS, resident(KPL, LPT_LOG))
 
     // Weights: slot s of lane sl is the pick s * lpt + sl.
     float w[NS], total = 0.0f;
+    bool weak = false;  // a weight that takes 64 bits
     auto weights = [&](int scoring) {
 #pragma unroll
       for (int s = 0; s < NS; ++s) {
         w[s] = 0.0f;
-        if (s * lpt + sl < a.top_k)
-          w[s] = score32<true>(load_logit<LD>(a.logits, row + slot_id[s]), scoring, mx, inv_sum);
+        if (s * lpt + sl < a.top_k) {
+          const float x = load_logit<LD>(a.logits, row + slot_id[s]);
+          w[s] = weight32(x, scoring, mx, inv_sum);
+          weak |= faint(x, scoring, mx);
+        }
         total += w[s];
       }
     };
@@ -613,7 +633,7 @@ __global__ void __launch_bounds__(32 * WARPS, resident(KPL, LPT_LOG))
       weights(DWM_SCORE_SQRTSOFTPLUS);
     if (a.renorm) total = seg_sum<lpt>(total);
     // What one lane of a token is unsure of, all are.
-    const uint32_t doubts = __ballot_sync(0xffffffffu, unsure && real && in_group);
+    const uint32_t doubts = __ballot_sync(0xffffffffu, ((unsure && in_group) || weak) && real);
     if (live && !(doubts & seg_mask)) {
       const float scale = !a.renorm ? a.scale : total == 0.0f ? 0.0f : a.scale;
 #pragma unroll

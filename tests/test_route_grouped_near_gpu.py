@@ -303,3 +303,28 @@ def test_many_experts_under_a_biased_softmax(dw):
         b = (torch.randn(e, generator=g) / e).cuda()
         for gs in ("max", "top2"):
             _check(dw, x, 8, groups, keep, "softmax", gs, b)
+
+
+@pytest.mark.parametrize("scoring", SCORINGS)
+@pytest.mark.parametrize("low", [-82.0, -89.0, -95.0, -105.0, -200.0])
+@pytest.mark.parametrize("t", [1, 300])
+def test_weights_of_scores_below_f32(dw, scoring, low, t):
+    """Scores that f32 does not hold still have ratios; a few ordinary tokens among them,
+    masked ones, and chosen experts far below a closed group's."""
+    g = torch.Generator().manual_seed(int(-low))
+    x = low + torch.rand((t, 64), generator=g) * 4
+    if t > 1:
+        x[::7] = torch.randn((len(x[::7]), 64), generator=g)
+        x[3, 5:] = -math.inf
+        x[10, 3:] = -3.0e38
+    for renorm in (True, False):
+        for groups, keep in ((1, 1), (8, 3)):
+            _check(dw, x.cuda(), 8, groups, keep, scoring, renorm=renorm)
+    if scoring != "softmax":
+        return
+    b = torch.zeros(64)
+    b[32:] = 10 + torch.arange(32) / 8
+    x = low + torch.rand((t, 64), generator=g) * 4
+    x[:, :32] += -low
+    for renorm in (True, False):
+        _check(dw, x.cuda(), 8, 8, 3, scoring, bias=b.cuda(), renorm=renorm)
