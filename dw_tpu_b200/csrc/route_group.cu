@@ -211,16 +211,19 @@ __device__ __forceinline__ bool faint(float x, int scoring, float mx) {
 //                     and all of a token's alike, by the sum over the experts, expf 4,
 //                     the exponents ln 1024 (their mean size is below that), the
 //                     additions in sequence and the reciprocal 1
-// Two sums of two of them differ by four such errors (the common one twice), and by 4
-// for the additions. Scores below FLOOR are not measured by themselves: of a
-// sqrtsoftplus down there f32 holds no more than 4e-23.
+// So two choices differ by twice the one and the other once (their difference is at
+// most the larger), two sums of two by twice that and 4 for the additions. Scores
+// below FLOOR are not measured by themselves: of a sqrtsoftplus down there f32 holds
+// no more than 4e-23.
 constexpr float UNIT = 1.0f / 16777216.0f;
 constexpr float FLOOR = 1e-15f;
 template <int KPL, int LPT_LOG>
-__device__ __forceinline__ float margin_of(int scoring) {
+__device__ __forceinline__ float margin_of(int scoring, bool sums) {
   constexpr int ADDS = KPL + LPT_LOG;  // of a lane's and of the lanes'
-  return scoring == DWM_SCORE_SOFTMAX ? (4 * 7 + 2 * (4 + 7 + ADDS + 1) + 4) * UNIT
-                                      : (4 * 10 + 4 + 2) * UNIT;
+  constexpr int SOFTMAX = 2 * 7 + 4 + 7 + ADDS + 1, OTHER = 2 * 10;
+  // (1 and 2 for the differences and margins themselves.)
+  return scoring == DWM_SCORE_SOFTMAX ? (sums ? 2 * SOFTMAX + 6 : SOFTMAX + 1) * UNIT
+                                      : (sums ? 2 * OTHER + 6 : OTHER + 1) * UNIT;
 }
 // Without a bias a sum of two scores is off relative to itself, in the same units by
 // 6, of a softmax by 5 and the size of its exponent, which above FLOOR is at most 35;
@@ -379,7 +382,7 @@ __global__ void __launch_bounds__(32 * WARPS, resident(KPL, LPT_LOG))
       }
     }
     float size = FLOOR;  // the largest |score| + |bias|
-    auto margin = [&] { return margin_of<KPL, LPT_LOG>(a.scoring) * size; };
+    auto margin = [&](bool sums) { return margin_of<KPL, LPT_LOG>(a.scoring, sums) * size; };
     if (biased) {
       auto choices = [&](int scoring) {
 #pragma unroll
@@ -428,7 +431,7 @@ __global__ void __launch_bounds__(32 * WARPS, resident(KPL, LPT_LOG))
     // What the values of a lane's packed keys up to k are below, in 64 bits.
     auto bound = [&](uint32_t k) {
       const double x = P::value(k & ~PLACES);
-      return x + (biased ? (double)margin() + (double)P::HIDDEN * size
+      return x + (biased ? (double)margin(false) + (double)P::HIDDEN * size
                          : (double)P::HIDDEN * fabs(x));
     };
     for (int o = (1 << a.lg_log) / 2; o; o >>= 1) {
@@ -459,7 +462,7 @@ __global__ void __launch_bounds__(32 * WARPS, resident(KPL, LPT_LOG))
     if (a.keep < a.groups && (biased || a.top2)) {
       const float in = value32(~seg_max<lpt>(open ? ~gkey : 0u));  // the least of the open
       const float out = value32(seg_max<lpt>(in_group && !open ? gkey : 0u));
-      const bool close = biased ? !(in - out > margin())
+      const bool close = biased ? !(in - out > margin(a.top2))
                                 : !(in > FLOOR && in - out > RELATIVE * in);
       if (__any_sync(0xffffffffu, close && real)) {
         // The groups' values in 64 bits, from each lane's first four.
@@ -527,14 +530,14 @@ __global__ void __launch_bounds__(32 * WARPS, resident(KPL, LPT_LOG))
     };
     // Packed values x <= last whose order packing or f32 may hide.
     auto near = [&](float last, float x) {
-      return !(last - x > (biased ? margin() + P::HIDDEN * size
+      return !(last - x > (biased ? margin(false) + P::HIDDEN * size
                                   : P::HIDDEN * fmaxf(fabsf(x), fabsf(last))));
     };
     // Whether the choice of expert e certainly comes before that of f, which has
     // the higher index if they tie.
     auto ahead = [&](int e, int f) {
       const float p = choice(e), q = choice(f);
-      if (biased ? p - q > margin() : p > q) return true;
+      if (biased ? p - q > margin(false) : p > q) return true;
       // Equal logits and biases are a tie in 64 bits too.
       return load_logit<LD>(a.logits, row + e) == load_logit<LD>(a.logits, row + f) &&
              (!biased || a.bias[e] == a.bias[f]);
