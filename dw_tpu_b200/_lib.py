@@ -29,6 +29,7 @@ DEV_OVERFLOW = 4
 BF16 = 0
 F32 = 1
 U8 = 2
+F64 = 3
 ACT_NONE = 0
 ACT_SWIGLU = 1
 ACT_SWIGLU_CLAMP = 2

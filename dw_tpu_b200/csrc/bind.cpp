@@ -199,7 +199,7 @@ PyObject* route_grouped_topk(PyObject*, PyObject* const* v, Py_ssize_t n_args) {
   const int64_t ld = rows(logits, "logits");
   const int t = size32(logits.size(0), "t"), e = size32(logits.size(1), "e");
   const int top_k = int32(v[1], "top_k");
-  const int dt = dtype_of(logits, "logits");
+  const int dt = logits.scalar_type() == at::kDouble ? DWM_F64 : dtype_of(logits, "logits");
   if (bias) {
     same_device(dev, *bias, "bias");
     TORCH_CHECK_VALUE(bias->scalar_type() == at::kFloat, "bias must be f32");

@@ -67,11 +67,13 @@ __device__ __forceinline__ double score(double x, int scoring, double mx, double
 }
 
 template <int LD>
-__device__ __forceinline__ float load_logit(const void* logits, int64_t i) {
+__device__ __forceinline__ auto load_logit(const void* logits, int64_t i) {
   if constexpr (LD == DWM_BF16)
     return bf16_bits_to_f32(static_cast<const uint16_t*>(logits)[i]);
-  else
+  else if constexpr (LD == DWM_F32)
     return static_cast<const float*>(logits)[i];
+  else
+    return static_cast<const double*>(logits)[i];
 }
 
 // The warp's largest key and, of the lanes that hold it, the lowest index.
@@ -165,6 +167,30 @@ __device__ __noinline__ Pick route_row64(const Args& a, int64_t tok, uint64_t* b
     s = total == 0.0 ? 0.0 : s / total;
   }
   return {id, (float)(s * (double)a.scale)};
+}
+
+__device__ __forceinline__ void store_pick(const Args& a, int64_t tok, int k, int id,
+                                           float weight) {
+  const int64_t at = tok * a.top_k + k;
+  a.ids[at] = id;
+  if (a.w32) a.w32[at] = weight;
+  if (a.w16) a.w16[at] = (uint16_t)f32_to_bf16_bits(weight);
+}
+
+// Logits of 64 bits, whose order f32 does not hold: every token as above, a warp
+// each (32768 x 256 with a bias: 157 us).
+__global__ void __launch_bounds__(32 * WARPS) route_grouped64_kernel(const Args a) {
+  extern __shared__ uint64_t smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  overlap_wait();
+  overlap_next();
+  for (int64_t tok = (int64_t)blockIdx.x * WARPS + warp; tok < a.t;
+       tok += (int64_t)gridDim.x * WARPS) {
+    Pick p{0, 0.0f};
+    if (a.num_valid < 0 || tok < a.num_valid)
+      p = route_row64<DWM_F64>(a, tok, smem + warp * a.e, lane);
+    if (lane < a.top_k) store_pick(a, tok, lane, p.id, p.weight);
+  }
 }
 
 // 32-bit keys of numbers (not NaN), ordered as the 64-bit ones.
@@ -644,10 +670,7 @@ __global__ void __launch_bounds__(32 * WARPS, resident(KPL, LPT_LOG))
         const int k = s * lpt + sl;
         if (k < a.top_k) {
           const float x = (a.renorm && total != 0.0f ? w[s] / total : w[s]) * scale;
-          const int64_t at = tok * a.top_k + k;
-          a.ids[at] = real ? slot_id[s] : 0;
-          if (a.w32) a.w32[at] = real ? x : 0.0f;
-          if (a.w16) a.w16[at] = real ? (uint16_t)f32_to_bf16_bits(x) : (uint16_t)0;
+          store_pick(a, tok, k, real ? slot_id[s] : 0, real ? x : 0.0f);
         }
       }
     }
@@ -655,15 +678,18 @@ __global__ void __launch_bounds__(32 * WARPS, resident(KPL, LPT_LOG))
       const int of = (__ffs(again) - 1) >> lpt_log;
       again &= ~((lpt == 32 ? 0xFFFFFFFFu : (1u << lpt) - 1u) << (of << lpt_log));
       const Pick p = route_row64<LD>(a, base + of, buf, lane);
-      if (lane < a.top_k) {
-        const int64_t at = (base + of) * a.top_k + lane;
-        a.ids[at] = p.id;
-        if (a.w32) a.w32[at] = p.weight;
-        if (a.w16) a.w16[at] = (uint16_t)f32_to_bf16_bits(p.weight);
-      }
+      if (lane < a.top_k) store_pick(a, base + of, lane, p.id, p.weight);
       __syncwarp();
     }
   }
+}
+
+int launch64(const Args& a, cudaStream_t s) {
+  const unsigned grid =
+      (unsigned)std::min<int64_t>(((int64_t)a.t + WARPS - 1) / WARPS, (int64_t)num_sms() * 64);
+  return check_cuda(overlap_launch(route_grouped64_kernel, dim3(grid), dim3(32 * WARPS),
+                                   (size_t)WARPS * a.e * sizeof(uint64_t), 1, s, a),
+                    "route_grouped_topk launch");
 }
 
 template <int LD, int KPL, int LPT_LOG>
@@ -709,8 +735,8 @@ extern "C" int dwm_route_grouped_topk(const void* logits, int logits_dtype, int6
                                       int num_valid_tokens, int32_t* topk_ids,
                                       float* topk_weights_f32, void* topk_weights_bf16,
                                       void* stream) {
-  DWM_CHECK_ARG(logits_dtype == DWM_BF16 || logits_dtype == DWM_F32,
-                "logits dtype must be bf16 or f32");
+  DWM_CHECK_ARG(logits_dtype == DWM_BF16 || logits_dtype == DWM_F32 || logits_dtype == DWM_F64,
+                "logits dtype must be bf16, f32 or f64");
   DWM_CHECK_ARG(t >= 0 && e >= 1 && e <= 1024, "bad shape t=%d e=%d (e in [1, 1024])", t, e);
   DWM_CHECK_ARG(num_groups >= 1 && num_groups <= 32 && e % num_groups == 0,
                 "num_groups=%d must be in [1, 32] and divide e=%d", num_groups, e);
@@ -727,7 +753,7 @@ extern "C" int dwm_route_grouped_topk(const void* logits, int logits_dtype, int6
   DWM_CHECK_ARG(t <= 1 || ld_logits >= e, "ld_logits is shorter than a row");
   DWM_CHECK_ARG(t == 0 || (logits && topk_ids), "NULL pointer");
   if (t == 0) return DWM_OK;
-  const int es = logits_dtype == DWM_F32 ? 4 : 2;
+  const int es = logits_dtype == DWM_F64 ? 8 : logits_dtype == DWM_F32 ? 4 : 2;
   auto misaligned = [](const void* p, int size) { return reinterpret_cast<uintptr_t>(p) % size; };
   DWM_CHECK_ARG(!misaligned(logits, es) && !misaligned(bias, 4) && !misaligned(topk_ids, 4) &&
                     !misaligned(topk_weights_f32, 4) && !misaligned(topk_weights_bf16, 2),
@@ -760,6 +786,8 @@ extern "C" int dwm_route_grouped_topk(const void* logits, int logits_dtype, int6
   a.ids = topk_ids;
   a.w32 = topk_weights_f32;
   a.w16 = static_cast<uint16_t*>(topk_weights_bf16);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (logits_dtype == DWM_F64) return route_group::launch64(a, s);
   // Lanes: a power of two of groups, each of as many lanes as leave at most 32
   // experts a lane (64 where the warp has no more lanes); 8 a token at least, and
   // up to twelve tokens an SM the whole warp, for its shorter runs and its one
@@ -777,7 +805,6 @@ extern "C" int dwm_route_grouped_topk(const void* logits, int logits_dtype, int6
   a.run = (a.per + (1 << a.lg_log) - 1) >> a.lg_log;
   a.vec = a.per % a.run == 0 && a.run * es % 16 == 0 && (t == 1 || ld_logits * es % 16 == 0) &&
           (reinterpret_cast<uintptr_t>(logits) & 15) == 0;
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
   return logits_dtype == DWM_BF16 ? route_group::run<DWM_BF16>(a, s)
                                   : route_group::run<DWM_F32>(a, s);
 }

@@ -427,9 +427,9 @@ def route_grouped_topk_out(logits, top_k, num_groups, topk_groups, ids_out, w32_
                            w16_out=None, *, scoring_fn="sigmoid", group_score="top2",
                            renormalize=True, routed_scale=1.0, bias=None, num_valid_tokens=None,
                            stream=None):
-    """Group-limited routing of logits [t, e] (dwm_route_grouped_topk): ids_out
-    int32 [t, top_k], w32_out f32 and / or w16_out bf16 of the same shape.
-    Logits rows may be strided."""
+    """Group-limited routing of logits [t, e], bf16, f32 or f64
+    (dwm_route_grouped_topk): ids_out int32 [t, top_k], w32_out f32 and / or
+    w16_out bf16 of the same shape. Logits rows may be strided."""
     if ids_out is None:
         raise ValueError("ids_out is required")
     L.bind().route_grouped_topk(

@@ -47,8 +47,12 @@ def route_grouped_topk(gating_output: torch.Tensor, top_k: int, num_groups: int,
     group's the best choice in it (``group_score="max"``) or the sum of its two
     best ("top2"). The weights are the scores, divided by their sum if
     ``renormalize``, times ``routed_scale``. Selection is that of 64-bit scores
-    whatever the logits' dtype. Inference only: no gradient."""
-    logits = gating_output if gating_output.dtype in L.FLOATS else gating_output.float()
+    whatever the logits' dtype (f64 logits take several times as long). Inference
+    only: no gradient."""
+    logits = gating_output
+    if logits.dtype not in L.FLOATS and logits.dtype is not torch.float64:
+        # f32 holds the 16- and 8-bit floats whole, f64 the integers.
+        logits = logits.float() if logits.is_floating_point() else logits.double()
     if bias is not None and (bias.dtype is not torch.float32 or not bias.is_contiguous()):
         bias = bias.float().contiguous()
     w_ids = ops.route_grouped_topk_new(logits, top_k, num_groups, topk_groups,

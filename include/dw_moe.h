@@ -45,6 +45,7 @@ extern "C" {
 #define DWM_BF16 0
 #define DWM_F32 1
 #define DWM_U8 2 /* E8M0 exponent codes (scales only) */
+#define DWM_F64 3 /* logits of dwm_route_grouped_topk only */
 
 #define DWM_ACT_NONE 0
 #define DWM_ACT_SWIGLU 1       /* silu(gate) * up on [gate | up] halves */
@@ -226,7 +227,7 @@ int dwm_dedupe_topk(float* topk_weights_f32, int32_t* topk_ids, int t, int top_k
  * how f32 rounds nearly equal scores. A NaN choice ranks below every number;
  * -inf logits have score 0. Rows >= num_valid_tokens (if >= 0) get expert 0
  * with weight 0. e <= 1024, top_k <= min(32, topk_groups * e / num_groups).
- * logits rows are ld_logits elements apart. The outputs are contiguous as in
+ * logits (bf16, f32 or f64) rows are ld_logits elements apart. The outputs are contiguous as in
  * dwm_route_topk and must not overlap the inputs. */
 int dwm_route_grouped_topk(const void* logits, int logits_dtype, int64_t ld_logits, int t, int e,
                            int top_k, int num_groups, int topk_groups, int scoring,

@@ -328,3 +328,43 @@ def test_weights_of_scores_below_f32(dw, scoring, low, t):
     x[:, :32] += -low
     for renorm in (True, False):
         _check(dw, x.cuda(), 8, 8, 3, scoring, bias=b.cuda(), renorm=renorm)
+
+
+@pytest.mark.parametrize("e,groups,keep,k", [(1, 1, 1, 1), (64, 8, 3, 4), (250, 5, 2, 8),
+                                             (1024, 32, 1, 32), (33, 1, 1, 32)])
+@pytest.mark.parametrize("t", [0, 1, 5, 1500])
+def test_logits_of_64_bits(dw, e, groups, keep, k, t):
+    """Logits that f32 rounds to one number keep their order."""
+    g = torch.Generator().manual_seed(e + t)
+    x = torch.randn((t, e), generator=g, dtype=F64).cuda()
+    close = 1 + torch.randperm(t * e, generator=g).reshape(t, e).to(F64) * 2.0 ** -45
+    b = (torch.randint(0, 3, (e,), generator=g) * 0.25).cuda()
+    for scoring in SCORINGS:
+        for gs in ("max", "top2"):
+            _check(dw, x, k, groups, keep, scoring, gs)
+            _check(dw, x, k, groups, keep, scoring, gs, b, renorm=False)
+        _check(dw, close.cuda(), k, groups, keep, scoring, "max")
+
+
+def test_64_bit_logits_padding_strides_and_types(dw):
+    g = torch.Generator().manual_seed(3)
+    wide = torch.full((9, 70), math.nan, dtype=F64)
+    wide[:, 3:67] = torch.randn((9, 64), generator=g, dtype=F64)
+    x = wide.cuda()[:, 3:67]
+    w, ids = dw.route_grouped_topk(x, 4, 8, 2, dtype=F32, num_valid_tokens=7)
+    rw, ri, _ = _ref(x, 4, 8, 2, True, "sigmoid", "top2", 1.0, None)
+    rw[7:], ri[7:] = 0, 0
+    assert torch.equal(ids.cpu(), ri)
+    assert bool(((w.cpu().double() - rw).abs() <= 2.0 ** -24 * rw).all())  # one rounding
+    y = x.clone()
+    y[2, 5], y[3] = math.nan, -math.inf
+    w2, ids2 = dw.route_grouped_topk(y, 4, 8, 2, dtype=F32, num_valid_tokens=7)
+    rest = [0, 1, 4, 5, 6]
+    assert torch.equal(w2[rest], w[rest]) and torch.equal(ids2[rest], ids[rest])
+    assert 5 not in ids2[2].tolist() and not bool(w2[3].any())
+    # Whole numbers past 2^24, and half precision, as they are.
+    n = (2 ** 24 + torch.randperm(64, generator=g))[None].cuda()
+    assert dw.route_grouped_topk(n, 4, 1, 1, group_score="max")[1].tolist() == \
+        n.argsort(1, descending=True)[:, :4].tolist()
+    h = torch.randn((20, 64), generator=g).half().cuda()
+    _check(dw, h, 4, 8, 2)
