@@ -132,13 +132,13 @@ class DeviceError(RuntimeError):
     """A kernel reported a device-side fault through the status word."""
 
 
+_BUILD = "build it with `python __graft_entry__.py` (nvcc, sm_100a)"
+
+
 def require_built() -> None:
-    """Raise ImportError if libdw_moe.so or its binding has not been built
-    (without mapping them)."""
-    for path in (LIB_PATH, os.path.join(_HERE, "_bind.so")):
-        if not os.path.exists(path):
-            raise ImportError(
-                f"{path} not found: build it with `python __graft_entry__.py` (nvcc, sm_100a)")
+    """Raise ImportError if libdw_moe.so has not been built (without mapping it)."""
+    if not os.path.exists(LIB_PATH):
+        raise ImportError(f"{LIB_PATH} not found: {_BUILD}")
 
 
 def load():
@@ -169,14 +169,18 @@ _bind = None
 
 
 def bind():
-    """The native binding (csrc/bind.cpp) of the calls that take torch tensors,
-    wired to libdw_moe.so; raise ImportError if it is absent."""
+    """The native binding (csrc/bind.cpp) of the operators around the expert
+    layer, wired to libdw_moe.so; raise ImportError if it is absent. (Their first
+    call needs it; the package and its other ops do not.)"""
     global _bind
     if _bind is None:
         load()
         with _lock:
             if _bind is None:
-                from . import _bind as mod
+                try:
+                    from . import _bind as mod
+                except ImportError as e:
+                    raise ImportError(f"dw_tpu_b200._bind does not load: {_BUILD}") from e
                 mod.init(LIB_PATH)
                 _bind = mod
     return _bind

@@ -1,0 +1,44 @@
+"""How the calls of the operators around the expert layer are reached: the
+binding's absence and its build, without a GPU."""
+
+import os
+import subprocess
+import sys
+
+import pytest
+import torch
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+@pytest.fixture
+def bare(tmp_path):
+    """A folder with the package as it is, but for the binding."""
+    package = tmp_path / "dw_tpu_b200"
+    package.mkdir()
+    for name in os.listdir(os.path.join(ROOT, "dw_tpu_b200")):
+        if not name.startswith(("_bind", "__pycache__")):
+            (package / name).symlink_to(os.path.join(ROOT, "dw_tpu_b200", name))
+    return tmp_path
+
+
+def _run(code, cwd):
+    r = subprocess.run([sys.executable, "-c", code], cwd=cwd, capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr[-2000:]
+
+
+def test_the_expert_layer_needs_no_binding(bare):
+    """The package imports, and the ops that the binding has no part in reach the
+    library; its own calls say what is missing."""
+    _run("import os, torch, dw_tpu_b200 as dw\n"
+         "assert os.path.dirname(dw.__file__) == os.path.join(os.getcwd(), 'dw_tpu_b200')\n"
+         "x = torch.zeros((4, 64), dtype=torch.bfloat16)\n"
+         "for call in (lambda: dw.route_topk(x, 2), lambda: dw.dispatch_gather(x, x[0].int())):\n"
+         "    try: call()\n"
+         "    except ValueError as e: assert 'CUDA' in str(e), e\n"
+         "    else: raise SystemExit('no refusal')\n"
+         "for call in (lambda: dw.dense_matmul(x, x), lambda: dw.pre_norm(x, x[0]),\n"
+         "             lambda: dw.route_grouped_topk(x, 4, 8, 4)):\n"
+         "    try: call()\n"
+         "    except ImportError as e: assert 'build it' in str(e), e\n"
+         "    else: raise SystemExit('no refusal')\n", bare)
