@@ -170,8 +170,9 @@ _bind = None
 
 def bind():
     """The native binding (csrc/bind.cpp) of the operators around the expert
-    layer, wired to libdw_moe.so; raise ImportError if it is absent. (Their first
-    call needs it; the package and its other ops do not.)"""
+    layer, wired to libdw_moe.so; raise ImportError if it is absent or built for
+    another torch. (Their first call needs it; the package and its other ops do
+    not.)"""
     global _bind
     if _bind is None:
         load()
@@ -181,6 +182,10 @@ def bind():
                     from . import _bind as mod
                 except ImportError as e:
                     raise ImportError(f"dw_tpu_b200._bind does not load: {_BUILD}") from e
+                built_for = getattr(mod, "torch_version", "another version")
+                if built_for != str(torch.__version__):
+                    raise ImportError(f"{mod.__file__} is built for torch {built_for}, this is "
+                                      f"{torch.__version__}: {_BUILD}")
                 mod.init(LIB_PATH)
                 _bind = mod
     return _bind

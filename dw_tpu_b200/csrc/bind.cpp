@@ -361,4 +361,9 @@ PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_bind", nullptr, -1, kMethods};
 
 }  // namespace
 
-extern "C" PyMODINIT_FUNC PyInit__bind() { return PyModule_Create(&kModule); }
+extern "C" PyMODINIT_FUNC PyInit__bind() {
+  PyObject* m = PyModule_Create(&kModule);
+  // The torch whose internals it is compiled against.
+  if (m && PyModule_AddStringConstant(m, "torch_version", DWM_TORCH_VERSION) != 0) Py_CLEAR(m);
+  return m;
+}

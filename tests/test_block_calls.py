@@ -4,6 +4,7 @@ binding's absence and its build, without a GPU."""
 import os
 import subprocess
 import sys
+import sysconfig
 
 import pytest
 import torch
@@ -42,3 +43,25 @@ def test_the_expert_layer_needs_no_binding(bare):
          "    try: call()\n"
          "    except ImportError as e: assert 'build it' in str(e), e\n"
          "    else: raise SystemExit('no refusal')\n", bare)
+
+
+def test_a_binding_of_another_torch_is_refused(monkeypatch):
+    from dw_tpu_b200 import _lib
+    monkeypatch.setattr(_lib, "_bind", None)
+    monkeypatch.setattr(torch, "__version__", "2.0.1+other")
+    with pytest.raises(ImportError, match="built for torch .* this is 2.0.1.other: build it"):
+        _lib.bind()
+    monkeypatch.undo()
+    mod = _lib.bind()
+    assert mod.torch_version == str(torch.__version__)
+    assert mod.__file__.endswith(sysconfig.get_config_var("EXT_SUFFIX"))
+
+
+def test_a_binding_of_an_older_build_is_refused(bare):
+    """One without its torch's version, under the plain name."""
+    (bare / "dw_tpu_b200" / "_bind.py").write_text("")
+    _run("import torch, dw_tpu_b200 as dw\n"
+         "x = torch.zeros((4, 64), dtype=torch.bfloat16)\n"
+         "try: dw.dense_matmul(x, x)\n"
+         "except ImportError as e: assert 'built for torch another version' in str(e), e\n"
+         "else: raise SystemExit('no refusal')\n", bare)
