@@ -16,6 +16,7 @@
 
 #include <ATen/core/Tensor.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -85,9 +86,12 @@ c10::Device cuda_device(const Tensor& t) {
   TORCH_CHECK_VALUE(t.is_cuda(), "dw_tpu_b200 ops take CUDA tensors (no CPU path)");
   return t.device();
 }
-// Inputs that autograd would expect a gradient for are refused: these ops are
-// for inference and record none.
+// Inputs that autograd would expect a gradient for, or that carry a forward-mode
+// tangent, are refused: these ops are for inference and record none.
 void no_grad(const Tensor& t) {
+  TORCH_CHECK_VALUE(!(t._fw_grad(/*level=*/0).defined() &&
+                      c10::AutogradState::get_tls_state().get_fw_grad_mode()),
+                    "inference only: an input has a forward-mode tangent");
   TORCH_CHECK_VALUE(!(t.requires_grad() && c10::GradMode::is_enabled()),
                     "inference only: an input requires a gradient (call under torch.no_grad() or "
                     "detach it)");
@@ -149,6 +153,7 @@ PyObject* dense_matmul(PyObject*, PyObject* const* v, Py_ssize_t n_args) {
   no_grad(w);
   no_grad(bias);
   no_grad(res);
+  no_grad(out);
   const c10::Device dev = cuda_device(x);
   same_device(dev, w, "w");
   TORCH_CHECK_VALUE(x.scalar_type() == at::kBFloat16 && w.scalar_type() == at::kBFloat16,
@@ -169,7 +174,6 @@ PyObject* dense_matmul(PyObject*, PyObject* const* v, Py_ssize_t n_args) {
   const c10::cuda::OptionalCUDAGuard guard(dev);
   if (out) {
     same_device(dev, *out, "out");
-    no_grad(out);
   } else {
     out = fresh(m, n_out, int32(v[8], "out_dtype"), dev, v[9]);
   }
@@ -195,6 +199,8 @@ PyObject* route_grouped_topk(PyObject*, PyObject* const* v, Py_ssize_t n_args) {
       w16 = optional_tensor(v[13], "w16_out");
   no_grad(logits);
   no_grad(bias);
+  no_grad(w32);
+  no_grad(w16);
   const c10::Device dev = cuda_device(logits);
   const int64_t ld = rows(logits, "logits");
   const int t = size32(logits.size(0), "t"), e = size32(logits.size(1), "e");
@@ -253,6 +259,8 @@ PyObject* block_norm(PyObject*, PyObject* const* v, Py_ssize_t n_args) {
   no_grad(y);
   no_grad(gate);
   for (const Opt& x : vec) no_grad(x);
+  no_grad(r_out);
+  no_grad(h_out);
   const c10::Device dev = cuda_device(res);
   const int64_t ldres = rows(res, "residual");
   const int t = size32(res.size(0), "t"), h = size32(res.size(1), "h");
@@ -295,7 +303,6 @@ PyObject* block_norm(PyObject*, PyObject* const* v, Py_ssize_t n_args) {
   if (y) {
     if (r_out) {
       same_device(dev, *r_out, "r_out");
-      no_grad(r_out);
       TORCH_CHECK_VALUE(r_out->scalar_type() == res.scalar_type(),
                         "r_out must have residual's dtype");
     } else {
@@ -307,7 +314,6 @@ PyObject* block_norm(PyObject*, PyObject* const* v, Py_ssize_t n_args) {
   if (want_h) {
     if (h_out) {
       same_device(dev, *h_out, "h_out");
-      no_grad(h_out);
     } else {
       h_out = fresh(t, h, int32(v[13], "h_dtype"), dev, v[15]);
     }

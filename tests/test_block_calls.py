@@ -65,3 +65,39 @@ def test_a_binding_of_an_older_build_is_refused(bare):
          "try: dw.dense_matmul(x, x)\n"
          "except ImportError as e: assert 'built for torch another version' in str(e), e\n"
          "else: raise SystemExit('no refusal')\n", bare)
+
+
+def test_forward_mode_derivatives_are_refused():
+    """A tangent would be lost without a word."""
+    import torch.autograd.forward_ad as fw
+
+    import dw_tpu_b200 as dw
+    x, w = torch.zeros((4, 64), dtype=torch.bfloat16), torch.zeros((64, 64), dtype=torch.bfloat16)
+    v, f = torch.ones(64, dtype=torch.bfloat16), torch.zeros((4, 64))
+    with fw.dual_level():
+        def dual(t):
+            return fw.make_dual(t.clone(), torch.ones_like(t))
+        calls = [lambda: dw.dense_matmul(dual(x), w), lambda: dw.dense_matmul(x, dual(w)),
+                 lambda: dw.dense_matmul(x, w, bias=dual(v)),
+                 lambda: dw.dense_matmul(x, w, residual=dual(x)),
+                 lambda: dw.dense_matmul(x, w, out=dual(x)),
+                 lambda: dw.route_grouped_topk(dual(f), 4, 8, 4),
+                 lambda: dw.route_grouped_topk(dual(f.half()), 4, 8, 4),
+                 lambda: dw.route_grouped_topk(f, 4, 8, 4, bias=dual(f[0])),
+                 lambda: dw.pre_norm(dual(x), v), lambda: dw.pre_norm(x, dual(v)),
+                 lambda: dw.pre_norm(x, v, dual(v)), lambda: dw.post_norm(dual(x), x),
+                 lambda: dw.post_norm(x, x, residual_out=dual(x)),
+                 lambda: dw.pre_norm(x, v, out=dual(x)),
+                 lambda: dw.post_norm(x, dual(x)), lambda: dw.post_norm(x, x, gate=dual(v)),
+                 lambda: dw.post_norm(x, x, norm_weight=dual(v)),
+                 lambda: dw.post_norm(x, x, next_weight=v, next_bias=dual(v))]
+        for grad in (True, False):
+            with torch.set_grad_enabled(grad):
+                for call in calls:
+                    with pytest.raises(ValueError, match="inference only"):
+                        call()
+        # No tangent, or none that is recorded: as far as the CUDA check.
+        with pytest.raises(ValueError, match="CUDA"):
+            dw.dense_matmul(x, w)
+        with fw._set_fwd_grad_enabled(False), pytest.raises(ValueError, match="CUDA"):
+            dw.dense_matmul(dual(x), w)
