@@ -32,6 +32,13 @@ constexpr int TILE_W = 128;     // rows of w per tile
 constexpr int THREADS = 256;
 constexpr int A_STAGE = TILE_W * BK * 2;  // 16 KiB
 constexpr int MAX_CLUSTER = 8;
+// An f32 result is the sum of parts of at most this many k steps (2048 k), each an
+// accumulator of its own. The tensor cores cut an accumulator off after every addition,
+// always towards zero: one over 4096 k loses 4.4e-6 of the sum, over 8192 9.1e-6, where
+// f32 additions with rounding lose 0.6e-6 and 1e-6; in parts 2.1e-6 at any k. (A bf16
+// result rounds off 1.7e-3 and takes one accumulator. The few-rows kernel's warps have
+// an eighth of k at most, and lose 0.15e-6 of 8192.)
+constexpr int PART_STEPS = 32;
 
 struct Args {
   const void* bias;      // [n] or NULL
@@ -45,6 +52,7 @@ struct Args {
   int bias_vec, res_vec, out_vec;
   int out_wide;  // 32 bytes of a row are 32-byte aligned
   float limit, res_scale;
+  int part_steps;  // k steps of an accumulator (split kernel; pair kernel with SUMS)
   int* status;
 };
 
@@ -58,7 +66,7 @@ struct Layout {
   static constexpr int OFF_BAR = S * STG;
   static constexpr int OFF_MISC = OFF_BAR + (2 * S + 2) * 8;
   static constexpr int ALLOC = OFF_MISC + 16 + 1024;  // slack for 1 KiB alignment
-  static constexpr int TMEM_COLS = BT < 32 ? 32 : BT;
+  static constexpr int MAX_PARTS = 512 / BT;  // accumulators that fit TMEM
   static_assert(STG % 1024 == 0, "swizzled tiles need 1 KiB alignment");
   static_assert(2 * PARTIAL <= S * STG && ALLOC <= 232448, "shared memory");
 };
@@ -337,6 +345,9 @@ __global__ void __launch_bounds__(THREADS, 1)
   const int kt = (a.k + BK - 1) / BK;
   const int k_lo = (int)((int64_t)kt * rank / split), k_hi = (int)((int64_t)kt * (rank + 1) / split);
   const int steps = k_hi - k_lo;  // at least one
+  const int parts = (steps + a.part_steps - 1) / a.part_steps;
+  int tmem_cols = 32;
+  while (tmem_cols < parts * BT) tmem_cols *= 2;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < S; ++i) {
@@ -351,7 +362,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     tma_prefetch_desc(&tm_x);
   }
   if (warp == 1) {
-    tmem_alloc(tmem_slot, L::TMEM_COLS);
+    tmem_alloc(tmem_slot, tmem_cols);
     tmem_relinquish();
   }
   tc_fence_before();
@@ -390,6 +401,8 @@ __global__ void __launch_bounds__(THREADS, 1)
     const bool issuer = elect_one();
     constexpr uint32_t idesc = idesc_bf16(TILE_W, BT, false, false);
     bool ok = true;
+    uint32_t acc = tmem;  // the part's accumulator
+    int in = 0;           // its steps so far
     for (int i = 0; i < steps; ++i) {
       const int st = i % S;
       ok = __all_sync(0xffffffffu, mbar_wait(&full[st], (i / S) & 1, abort_flag, a.status));
@@ -399,11 +412,15 @@ __global__ void __launch_bounds__(THREADS, 1)
         const uint32_t base = smem_u32(smem + st * L::STG);
 #pragma unroll
         for (int j = 0; j < BK / 16; ++j)
-          umma_bf16(tmem, smem_desc_sw128(base + j * 32, 16, 1024),
-                    smem_desc_sw128(base + A_STAGE + j * 32, 16, 1024), idesc, (i | j) != 0);
+          umma_bf16(acc, smem_desc_sw128(base + j * 32, 16, 1024),
+                    smem_desc_sw128(base + A_STAGE + j * 32, 16, 1024), idesc, (in | j) != 0);
         umma_commit(&empty[st]);
       }
       __syncwarp();
+      if (++in == a.part_steps) {
+        in = 0;
+        acc += BT;
+      }
     }
     if (issuer) umma_commit(done);
     __syncwarp();
@@ -429,8 +446,17 @@ __global__ void __launch_bounds__(THREADS, 1)
         const int t0 = half * COLS + c;
         if (t0 >= rows) break;
         uint32_t r[16];
-        tmem_ld16(tmem + ((uint32_t)(q * 32) << 16) + t0, r);
+        const uint32_t at = tmem + ((uint32_t)(q * 32) << 16) + t0;
+        tmem_ld16(at, r);
         tmem_ld_wait(r);
+        for (int p = 1; p < parts; ++p) {
+          uint32_t more[16];
+          tmem_ld16(at + p * BT, more);
+          tmem_ld_wait(more);
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            r[e] = __float_as_uint(__uint_as_float(r[e]) + __uint_as_float(more[e]));
+        }
 #pragma unroll
         for (int e = 0; e < 16; ++e)
           sts_u32(part + (uint32_t)(((t0 + e) * TILE_W + q * 32 + lane) * 4), r[e]);
@@ -460,7 +486,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     __syncthreads();
   }
   tc_fence_after();
-  if (warp == 1) tmem_dealloc(tmem, L::TMEM_COLS);
+  if (warp == 1) tmem_dealloc(tmem, tmem_cols);
 
   // This CTA's rows: the partials in CTA order, 8 columns a thread.
   if (ok) {
@@ -563,8 +589,10 @@ int resident_clusters(int size) {
 
 template <int BT, int EPI>
 int launch_split(const void* x, int64_t ldx, const void* w, int64_t ldw, int n, int split,
-                 const Args& a, cudaStream_t stream) {
+                 Args a, cudaStream_t stream) {
   using L = Layout<BT>;
+  const int steps = ((a.k + BK - 1) / BK + split - 1) / split;  // of a CTA, or one fewer
+  a.part_steps = !a.out_f32 ? steps : std::max(PART_STEPS, (steps + L::MAX_PARTS - 1) / L::MAX_PARTS);
   constexpr int FEAT = EPI == GLU ? TILE_W / 2 : TILE_W;
   DWM_CHECK_ARG((a.m + (int64_t)BT - 1) / BT <= 65535 &&
                     (a.n_out + (int64_t)FEAT - 1) / FEAT <= 65535,
@@ -650,8 +678,11 @@ __device__ __forceinline__ uint32_t box_at(int r, int c, int f32) {
 }
 
 // VEC: rows of out and of the residual start on 16 bytes; RES: there is one
-// (without VEC it is read where it is added).
-template <int EPI, bool VEC, bool RES>
+// (without VEC it is read where it is added). SUMS: a sum over k is made of parts
+// (PART_STEPS): one accumulator takes them, and the epilogue warps add each to the
+// other one, where they find the whole sum at last. (The UMMAs wait for that once a
+// part: 8192 x 8192 x 2048 f32 takes 209 us, 196 with one accumulator.)
+template <int EPI, bool VEC, bool RES, bool SUMS>
 __global__ void __launch_bounds__(THREADS, 1)
     dense_pair_kernel(const __grid_constant__ CUtensorMap tm_x,
                       const __grid_constant__ CUtensorMap tm_w,
@@ -765,9 +796,46 @@ __global__ void __launch_bounds__(THREADS, 1)
         break;
       }
       tc_fence_after();
-      const uint32_t acc =
+      uint32_t acc =
           tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(slot * TILE + half * (FEAT / 2));
       uint32_t r0[16], r1[16];
+      if (SUMS) {
+        bool whole = true;
+        for (int k0 = 0;;) {
+          for (int c = 0; c < blocks * 16; c += 16)
+#pragma unroll
+            for (int up = 0; up < (EPI == GLU ? 2 : 1); ++up) {
+              const uint32_t at = acc + (uint32_t)(c + up * HALF);
+              tmem_ld16(at, r0);
+              if (k0 > 0) tmem_ld16(at + TILE, r1);
+              tmem_ld_wait(r0);
+              if (k0 > 0) {
+                tmem_ld_wait(r1);
+#pragma unroll
+                for (int j = 0; j < 16; ++j)
+                  r0[j] = __float_as_uint(__uint_as_float(r0[j]) + __uint_as_float(r1[j]));
+              }
+              tmem_st16(at + TILE, r0);
+            }
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_remote(acc_empty_0);
+          ph ^= 1;
+          k0 += PART_STEPS;
+          if (k0 >= kt) break;
+          if (!__all_sync(0xffffffffu, mbar_wait<64>(&acc_full[0], ph, abort_flag, a.status))) {
+            whole = false;
+            break;
+          }
+          tc_fence_after();
+        }
+        if (!whole) {
+          land(steps);
+          break;
+        }
+        acc += TILE;
+      }
       auto fetch = [&](int c) {
         tmem_ld16(acc + c, r0);
         if (EPI == GLU) tmem_ld16(acc + c + HALF, r1);
@@ -904,10 +972,12 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
       }
       if (!res_ok) break;
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive_remote(acc_empty_0 + (uint32_t)(slot * 8));
-      if (++slot == 2) { slot = 0; ph ^= 1; }
+      if (!SUMS) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_remote(acc_empty_0 + (uint32_t)(slot * 8));
+        if (++slot == 2) { slot = 0; ph ^= 1; }
+      }
     }
     if (VEC && lane == 0) bulk_wait_all();  // before this CTA's shared memory goes
   } else if (warp == TMA_WARP) {
@@ -948,33 +1018,42 @@ __global__ void __launch_bounds__(THREADS, 1)
       int st = 0, slot = 0;
       uint32_t ph = 0, acc_ph = 0;
       bool ok = true;
+      const int part = SUMS ? PART_STEPS : kt;  // k steps of an accumulator
       for (int idx = cl; idx < total && ok; idx += ncl) {
-        if (!__all_sync(0xffffffffu, mbar_wait(&acc_empty[slot], acc_ph ^ 1, abort_flag, a.status)))
-          break;
-        tc_fence_after();
-        const uint32_t d = tmem + (uint32_t)(slot * TILE);
-        for (int kk = 0; kk < kt; ++kk) {
-          if (!__all_sync(0xffffffffu, mbar_wait(&full[st], ph, abort_flag, a.status))) {
-            ok = false;
-            break;
-          }
+        for (int k0 = 0; k0 < kt && ok; k0 += part) {
+          ok = __all_sync(0xffffffffu, mbar_wait(&acc_empty[slot], acc_ph ^ 1, abort_flag, a.status));
+          if (!ok) break;
           tc_fence_after();
-          if (issuer) {
-            const uint32_t base = smem_u32(smem + st * STG);
+          const uint32_t d = tmem + (uint32_t)(slot * TILE);
+          const int k1 = min(kt, k0 + part);
+          for (int kk = k0; kk < k1; ++kk) {
+            if (!__all_sync(0xffffffffu, mbar_wait(&full[st], ph, abort_flag, a.status))) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            if (issuer) {
+              const uint32_t base = smem_u32(smem + st * STG);
 #pragma unroll
-            for (int j = 0; j < BK / 16; ++j)
-              umma_pair_bf16(d, smem_desc_sw128(base + j * 32, 16, 1024),
-                             smem_desc_sw128(base + OP_STAGE + j * 32, 16, 1024), idesc,
-                             (kk | j) != 0);
-            umma_commit_pair(&empty[st]);
+              for (int j = 0; j < BK / 16; ++j)
+                umma_pair_bf16(d, smem_desc_sw128(base + j * 32, 16, 1024),
+                               smem_desc_sw128(base + OP_STAGE + j * 32, 16, 1024), idesc,
+                               ((kk - k0) | j) != 0);
+              umma_commit_pair(&empty[st]);
+            }
+            __syncwarp();
+            if (++st == S) { st = 0; ph ^= 1; }
           }
+          if (!ok) break;
+          if (issuer) umma_commit_pair(&acc_full[slot]);
           __syncwarp();
-          if (++st == S) { st = 0; ph ^= 1; }
+          if (SUMS) {
+            acc_ph ^= 1;  // (the other accumulator is the epilogue's)
+          } else if (++slot == 2) {
+            slot = 0;
+            acc_ph ^= 1;
+          }
         }
-        if (!ok) break;
-        if (issuer) umma_commit_pair(&acc_full[slot]);
-        __syncwarp();
-        if (++slot == 2) { slot = 0; acc_ph ^= 1; }
       }
       if (issuer) umma_commit_pair(drain);
       __syncwarp();
@@ -1004,9 +1083,9 @@ __global__ void __launch_bounds__(THREADS, 1)
   cluster_sync();
 }
 
-template <int EPI, bool VEC, bool RES>
-int launch(const void* x, int64_t ldx, const void* w, int64_t ldw, int n, const Args& a,
-           cudaStream_t stream) {
+template <int EPI, bool VEC, bool RES, bool SUMS>
+int launch_as(const void* x, int64_t ldx, const void* w, int64_t ldw, int n, const Args& a,
+              cudaStream_t stream) {
   using L = Layout<RES>;
   constexpr int FEAT = EPI == GLU ? HALF : TILE;
   const int64_t tiles = (int64_t)((a.m + (int64_t)TILE - 1) / TILE) *
@@ -1028,14 +1107,22 @@ int launch(const void* x, int64_t ldx, const void* w, int64_t ldw, int n, const 
   tm_out = tm_res = tm_x;  // (unused without VEC, without RES)
   if (VEC && (rc = box_map(&tm_out, a.out, a.ldo, a.out_f32))) return rc;
   if (RES && (rc = box_map(&tm_res, a.residual, a.ldr, a.res_f32))) return rc;
-  rc = set_smem_limit(reinterpret_cast<const void*>(dense_pair_kernel<EPI, VEC, RES>), L::ALLOC,
+  rc = set_smem_limit(reinterpret_cast<const void*>(dense_pair_kernel<EPI, VEC, RES, SUMS>), L::ALLOC,
                       "dense pair smem attribute");
   if (rc) return rc;
   return check_cuda(
-      overlap_launch(dense_pair_kernel<EPI, VEC, RES>,
+      overlap_launch(dense_pair_kernel<EPI, VEC, RES, SUMS>,
                      dim3(2 * (unsigned)std::min<int64_t>(tiles, resident_clusters(2))),
                      dim3(THREADS), L::ALLOC, 2, stream, tm_x, tm_w, tm_out, tm_res, a),
       "dense_matmul launch");
+}
+
+template <int EPI, bool VEC, bool RES>
+int launch(const void* x, int64_t ldx, const void* w, int64_t ldw, int n, const Args& a,
+           cudaStream_t stream) {
+  return a.out_f32 && (a.k + BK - 1) / BK > PART_STEPS
+             ? launch_as<EPI, VEC, RES, true>(x, ldx, w, ldw, n, a, stream)
+             : launch_as<EPI, VEC, RES, false>(x, ldx, w, ldw, n, a, stream);
 }
 
 }  // namespace pair
@@ -1270,12 +1357,16 @@ int run_epi(const void* x, int64_t ldx, const void* w, int64_t ldw, int n, const
   const float b = (float)bt / 128.0f;
   int split = 1;
   float best = 0.0f;
-  for (int s = 1; s <= MAX_CLUSTER && (s == 1 || kt >= 2 * s); s *= 2) {
+  // (An f32 result's parts have to fit TMEM.)
+  const int least_split = a.out_f32 ? (kt + PART_STEPS * 512 / bt - 1) / (PART_STEPS * 512 / bt) : 1;
+  int first = 1;
+  while (first < std::min(least_split, MAX_CLUSTER)) first *= 2;
+  for (int s = first; s <= MAX_CLUSTER && (s == first || kt >= 2 * s); s *= 2) {
     const float v = waves(tiles, s);
     const float t = v * (std::max(0.22f * (float)((kt + s - 1) / s), 1.05f * hbm / v) + 2.75f +
                          2.5f * b + (s > 1 ? 0.85f + 0.8f * b : 0.0f)) -
                     0.6f;
-    if (s == 1 || t < best) {
+    if (s == first || t < best) {
       best = t;
       split = s;
     }
@@ -1383,6 +1474,7 @@ extern "C" int dwm_dense_matmul(const void* x, int64_t ldx, const void* w, int64
   a.out_wide = addr(out) % 32 == 0 && ldo * oes % 32 == 0;
   a.limit = act_limit;
   a.res_scale = residual_scale;
+  a.part_steps = 0;
   a.status = status_ptr();
   return dense::run(x, ldx, w, ldw, n, a, static_cast<cudaStream_t>(stream));
 }
