@@ -6,9 +6,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib as L
-from .ops import code_of
-
-_NORMS = {"rms": L.NORM_RMS, "layer": L.NORM_LAYER}
+from .ops import NORMS, code_of
 
 
 def pre_norm(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *,
@@ -20,7 +18,7 @@ def pre_norm(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = 
     if weight is None:
         raise ValueError("pre_norm needs a weight")
     return L.bind().block_norm(x, None, None, None, None, 1.0, 1.0, weight, bias, eps,
-                               code_of(_NORMS, kind, "norm kind"), None, out,
+                               code_of(NORMS, kind, "norm kind"), None, out,
                                code_of(L.FLOATS, out_dtype, "out_dtype"), True, None)[1]
 
 
@@ -47,6 +45,6 @@ def post_norm(y: torch.Tensor, residual: torch.Tensor, *,
     if y is None:
         raise ValueError("post_norm needs y")
     return L.bind().block_norm(residual, y, norm_weight, norm_bias, gate, scale, residual_scale,
-                               next_weight, next_bias, eps, code_of(_NORMS, kind, "norm kind"),
+                               next_weight, next_bias, eps, code_of(NORMS, kind, "norm kind"),
                                residual_out, out, code_of(L.FLOATS, out_dtype, "out_dtype"),
                                next_weight is not None, None)

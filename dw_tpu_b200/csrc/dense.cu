@@ -37,7 +37,7 @@ constexpr int MAX_CLUSTER = 8;
 // always towards zero: one over 4096 k loses 4.4e-6 of the sum, over 8192 9.1e-6, where
 // f32 additions with rounding lose 0.6e-6 and 1e-6; in parts 2.1e-6 at any k. (A bf16
 // result rounds off 1.7e-3 and takes one accumulator. The few-rows kernel's warps have
-// an eighth of k at most, and lose 0.15e-6 of 8192.)
+// at most an eighth of k, and lose 0.15e-6 of 8192.)
 constexpr int PART_STEPS = 32;
 
 struct Args {
@@ -52,7 +52,8 @@ struct Args {
   int bias_vec, res_vec, out_vec;
   int out_wide;  // 32 bytes of a row are 32-byte aligned
   float limit, res_scale;
-  int part_steps;  // k steps of an accumulator (split kernel; pair kernel with SUMS)
+  // Split kernel: k steps of an accumulator, and the columns that they all take.
+  int part_steps, tmem_cols;
   int* status;
 };
 
@@ -76,27 +77,22 @@ __device__ __forceinline__ float ld1(const void* p, int64_t i, int f32) {
              : bf16_bits_to_f32(static_cast<const uint16_t*>(p)[i]);
 }
 
-// N (8 or 16) neighbouring elements, 16-byte aligned.
-template <int N>
-__device__ __forceinline__ void load_n(const void* p, int64_t i, int f32, float (&v)[N]) {
+// 8 neighbouring elements, 16-byte aligned.
+__device__ __forceinline__ void load_8(const void* p, int64_t i, int f32, float (&v)[8]) {
   if (f32) {
     const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
 #pragma unroll
-    for (int j = 0; j < N / 4; ++j) {
+    for (int j = 0; j < 2; ++j) {
       const float4 x = q[j];
       v[4 * j] = x.x; v[4 * j + 1] = x.y; v[4 * j + 2] = x.z; v[4 * j + 3] = x.w;
     }
   } else {
-    const uint4* q = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + i);
+    const uint4 x = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + i);
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-    for (int j = 0; j < N / 8; ++j) {
-      const uint4 x = q[j];
-      const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        v[8 * j + 2 * e] = __uint_as_float(w[e] << 16);
-        v[8 * j + 2 * e + 1] = __uint_as_float(w[e] & 0xFFFF0000u);
-      }
+    for (int e = 0; e < 4; ++e) {
+      v[2 * e] = __uint_as_float(w[e] << 16);
+      v[2 * e + 1] = __uint_as_float(w[e] & 0xFFFF0000u);
     }
   }
 }
@@ -108,37 +104,24 @@ __device__ __forceinline__ void stg_256(void* p, const uint32_t (&w)[8]) {
                : "memory");
 }
 
-// N values to `p` (bf16 or f32), 16-byte aligned; wide: 32-byte aligned.
-template <int N>
-__device__ __forceinline__ void store_n(void* p, int64_t i, int f32, bool wide,
-                                        const float (&v)[N]) {
-  uint32_t w[N];
-  int words;
-  uint8_t* at;
+// 8 values to `p` (bf16 or f32), 16-byte aligned; wide: 32-byte aligned.
+__device__ __forceinline__ void store_8(void* p, int64_t i, int f32, bool wide,
+                                        const float (&v)[8]) {
   if (f32) {
+    float* at = static_cast<float*>(p) + i;
+    uint32_t w[8];
 #pragma unroll
-    for (int q = 0; q < N; ++q) w[q] = __float_as_uint(v[q]);
-    words = N;
-    at = static_cast<uint8_t*>(p) + i * 4;
-  } else {
-#pragma unroll
-    for (int q = 0; q < N / 2; ++q) w[q] = f32x2_to_bf16x2(v[2 * q], v[2 * q + 1]);
-    words = N / 2;
-    at = static_cast<uint8_t*>(p) + i * 2;
-  }
-#pragma unroll
-  for (int j = 0; j < N; j += 8) {
-    if (j >= words) break;
-    if (wide && j + 8 <= words) {
-      const uint32_t x[8] = {w[j], w[(j + 1) % N], w[(j + 2) % N], w[(j + 3) % N],
-                             w[(j + 4) % N], w[(j + 5) % N], w[(j + 6) % N], w[(j + 7) % N]};
-      stg_256(at + j * 4, x);
+    for (int q = 0; q < 8; ++q) w[q] = __float_as_uint(v[q]);
+    if (wide) {
+      stg_256(at, w);
     } else {
-      *reinterpret_cast<uint4*>(at + j * 4) = make_uint4(w[j], w[j + 1], w[j + 2], w[j + 3]);
-      if (j + 8 <= words)
-        *reinterpret_cast<uint4*>(at + j * 4 + 16) =
-            make_uint4(w[(j + 4) % N], w[(j + 5) % N], w[(j + 6) % N], w[(j + 7) % N]);
+      *reinterpret_cast<uint4*>(at) = make_uint4(w[0], w[1], w[2], w[3]);
+      *reinterpret_cast<uint4*>(at + 4) = make_uint4(w[4], w[5], w[6], w[7]);
     }
+  } else {
+    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + i) =
+        make_uint4(f32x2_to_bf16x2(v[0], v[1]), f32x2_to_bf16x2(v[2], v[3]),
+                   f32x2_to_bf16x2(v[4], v[5]), f32x2_to_bf16x2(v[6], v[7]));
   }
 }
 
@@ -196,58 +179,52 @@ __device__ __forceinline__ void activate(const Args& a, float (&z)[N], float (&u
   }
 }
 
-// Outputs [col, col + N) of row `row`, N = 8 or 16, from the products z (and,
-// with SwiGLU, the up products u): bias, activation, residual, one rounding.
-// Rows of out start on 16 bytes (Args::out_vec).
-template <int EPI, int N>
-__device__ __forceinline__ void bias_and_act(const Args& a, int col, float (&z)[N],
-                                             float (&u)[N]) {
-  const bool whole = col + N <= a.n_out;
+// Outputs [col, col + 8) of row `row` from the products z (and, with SwiGLU, the up
+// products u): bias, activation, residual, one rounding. Rows of out start on 16 bytes
+// (Args::out_vec).
+template <int EPI>
+__device__ __forceinline__ void epilogue(const Args& a, int64_t row, int col, float (&z)[8],
+                                         float (&u)[8]) {
+  const bool whole = col + 8 <= a.n_out;
   if (a.bias) {
-    float b[N];
+    float b[8];
     auto bias = [&](int off) {
       if (whole && a.bias_vec) {
-        load_n(a.bias, off + col, a.bias_f32, b);
+        load_8(a.bias, off + col, a.bias_f32, b);
       } else {
 #pragma unroll
-        for (int q = 0; q < N; ++q) b[q] = ld1(a.bias, off + min(col + q, a.n_out - 1), a.bias_f32);
+        for (int q = 0; q < 8; ++q) b[q] = ld1(a.bias, off + min(col + q, a.n_out - 1), a.bias_f32);
       }
     };
     bias(0);
 #pragma unroll
-    for (int q = 0; q < N; ++q) z[q] += b[q];
+    for (int q = 0; q < 8; ++q) z[q] += b[q];
     if (EPI == GLU) {
       bias(a.n_out);
 #pragma unroll
-      for (int q = 0; q < N; ++q) u[q] += b[q];
+      for (int q = 0; q < 8; ++q) u[q] += b[q];
     }
   }
   activate<EPI>(a, z, u);
-}
-template <int EPI, int N>
-__device__ __forceinline__ void epilogue(const Args& a, int64_t row, int col, float (&z)[N],
-                                         float (&u)[N]) {
-  const bool whole = col + N <= a.n_out;
-  bias_and_act<EPI>(a, col, z, u);
   if (a.residual) {
     const int64_t at = row * a.ldr + col;
     if (whole && a.res_vec) {
-      float r[N];
-      load_n(a.residual, at, a.res_f32, r);
+      float r[8];
+      load_8(a.residual, at, a.res_f32, r);
 #pragma unroll
-      for (int q = 0; q < N; ++q) z[q] = fmaf(a.res_scale, r[q], z[q]);
+      for (int q = 0; q < 8; ++q) z[q] = fmaf(a.res_scale, r[q], z[q]);
     } else {
 #pragma unroll
-      for (int q = 0; q < N; ++q)
+      for (int q = 0; q < 8; ++q)
         if (col + q < a.n_out) z[q] = fmaf(a.res_scale, ld1(a.residual, at + q, a.res_f32), z[q]);
     }
   }
   const int64_t at = row * a.ldo + col;
   if (whole) {
-    store_n(a.out, at, a.out_f32, a.out_wide != 0, z);
+    store_8(a.out, at, a.out_f32, a.out_wide != 0, z);
   } else {
 #pragma unroll
-    for (int q = 0; q < N; ++q)
+    for (int q = 0; q < 8; ++q)
       if (col + q < a.n_out) {
         if (a.out_f32)
           static_cast<float*>(a.out)[at + q] = z[q];
@@ -345,9 +322,6 @@ __global__ void __launch_bounds__(THREADS, 1)
   const int kt = (a.k + BK - 1) / BK;
   const int k_lo = (int)((int64_t)kt * rank / split), k_hi = (int)((int64_t)kt * (rank + 1) / split);
   const int steps = k_hi - k_lo;  // at least one
-  const int parts = (steps + a.part_steps - 1) / a.part_steps;
-  int tmem_cols = 32;
-  while (tmem_cols < parts * BT) tmem_cols *= 2;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < S; ++i) {
@@ -362,7 +336,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     tma_prefetch_desc(&tm_x);
   }
   if (warp == 1) {
-    tmem_alloc(tmem_slot, tmem_cols);
+    tmem_alloc(tmem_slot, a.tmem_cols);
     tmem_relinquish();
   }
   tc_fence_before();
@@ -446,12 +420,13 @@ __global__ void __launch_bounds__(THREADS, 1)
         const int t0 = half * COLS + c;
         if (t0 >= rows) break;
         uint32_t r[16];
-        const uint32_t at = tmem + ((uint32_t)(q * 32) << 16) + t0;
+        uint32_t at = tmem + ((uint32_t)(q * 32) << 16) + t0;
         tmem_ld16(at, r);
         tmem_ld_wait(r);
-        for (int p = 1; p < parts; ++p) {
+        for (int i = a.part_steps; i < steps; i += a.part_steps) {
           uint32_t more[16];
-          tmem_ld16(at + p * BT, more);
+          at += BT;
+          tmem_ld16(at, more);
           tmem_ld_wait(more);
 #pragma unroll
           for (int e = 0; e < 16; ++e)
@@ -486,7 +461,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     __syncthreads();
   }
   tc_fence_after();
-  if (warp == 1) tmem_dealloc(tmem, tmem_cols);
+  if (warp == 1) tmem_dealloc(tmem, a.tmem_cols);
 
   // This CTA's rows: the partials in CTA order, 8 columns a thread.
   if (ok) {
@@ -592,7 +567,10 @@ int launch_split(const void* x, int64_t ldx, const void* w, int64_t ldw, int n, 
                  Args a, cudaStream_t stream) {
   using L = Layout<BT>;
   const int steps = ((a.k + BK - 1) / BK + split - 1) / split;  // of a CTA, or one fewer
-  a.part_steps = !a.out_f32 ? steps : std::max(PART_STEPS, (steps + L::MAX_PARTS - 1) / L::MAX_PARTS);
+  a.part_steps =
+      a.out_f32 ? std::max(PART_STEPS, (steps + L::MAX_PARTS - 1) / L::MAX_PARTS) : steps;
+  const int parts = (steps + a.part_steps - 1) / a.part_steps;
+  for (a.tmem_cols = 32; a.tmem_cols < parts * BT;) a.tmem_cols *= 2;
   constexpr int FEAT = EPI == GLU ? TILE_W / 2 : TILE_W;
   DWM_CHECK_ARG((a.m + (int64_t)BT - 1) / BT <= 65535 &&
                     (a.n_out + (int64_t)FEAT - 1) / FEAT <= 65535,
@@ -1357,10 +1335,9 @@ int run_epi(const void* x, int64_t ldx, const void* w, int64_t ldw, int n, const
   const float b = (float)bt / 128.0f;
   int split = 1;
   float best = 0.0f;
-  // (An f32 result's parts have to fit TMEM.)
-  const int least_split = a.out_f32 ? (kt + PART_STEPS * 512 / bt - 1) / (PART_STEPS * 512 / bt) : 1;
+  // (An f32 result's parts have to fit a CTA's TMEM.)
   int first = 1;
-  while (first < std::min(least_split, MAX_CLUSTER)) first *= 2;
+  while (a.out_f32 && first < MAX_CLUSTER && kt > first * PART_STEPS * (512 / bt)) first *= 2;
   for (int s = first; s <= MAX_CLUSTER && (s == first || kt >= 2 * s); s *= 2) {
     const float v = waves(tiles, s);
     const float t = v * (std::max(0.22f * (float)((kt + s - 1) / s), 1.05f * hbm / v) + 2.75f +
@@ -1474,7 +1451,7 @@ extern "C" int dwm_dense_matmul(const void* x, int64_t ldx, const void* w, int64
   a.out_wide = addr(out) % 32 == 0 && ldo * oes % 32 == 0;
   a.limit = act_limit;
   a.res_scale = residual_scale;
-  a.part_steps = 0;
+  a.part_steps = a.tmem_cols = 0;
   a.status = status_ptr();
   return dense::run(x, ldx, w, ldw, n, a, static_cast<cudaStream_t>(stream));
 }

@@ -412,7 +412,7 @@ def e8m0_decode_out(codes, out, stream=None):
 # ----------------------------------------------------------------------------
 
 _GROUP_SCORES = {"max": L.GROUP_MAX, "top2": L.GROUP_TOP2}
-_NORMS = {"rms": L.NORM_RMS, "layer": L.NORM_LAYER}
+NORMS = {"rms": L.NORM_RMS, "layer": L.NORM_LAYER}
 
 
 def code_of(table, key, what):
@@ -421,6 +421,14 @@ def code_of(table, key, what):
         return table[key]
     except (KeyError, TypeError):
         raise ValueError(f"unknown {what} {key!r} (one of {list(table)})") from None
+
+
+def _route_grouped(logits, top_k, num_groups, topk_groups, scoring_fn, group_score, renormalize,
+                   routed_scale, bias, num_valid_tokens, *outputs):
+    return L.bind().route_grouped_topk(
+        logits, top_k, num_groups, topk_groups, code_of(_SCORING, scoring_fn, "scoring_fn"),
+        code_of(_GROUP_SCORES, group_score, "group_score"), 1 if renormalize else 0, routed_scale,
+        bias, -1 if num_valid_tokens is None else max(0, num_valid_tokens), *outputs)
 
 
 def route_grouped_topk_out(logits, top_k, num_groups, topk_groups, ids_out, w32_out=None,
@@ -432,21 +440,16 @@ def route_grouped_topk_out(logits, top_k, num_groups, topk_groups, ids_out, w32_
     w16_out bf16 of the same shape. Logits rows may be strided."""
     if ids_out is None:
         raise ValueError("ids_out is required")
-    L.bind().route_grouped_topk(
-        logits, top_k, num_groups, topk_groups, code_of(_SCORING, scoring_fn, "scoring_fn"),
-        code_of(_GROUP_SCORES, group_score, "group_score"), int(bool(renormalize)), routed_scale,
-        bias, -1 if num_valid_tokens is None else max(0, num_valid_tokens), L.F32, ids_out,
-        w32_out, w16_out, stream)
+    _route_grouped(logits, top_k, num_groups, topk_groups, scoring_fn, group_score, renormalize,
+                   routed_scale, bias, num_valid_tokens, L.F32, ids_out, w32_out, w16_out, stream)
 
 
 def route_grouped_topk_new(logits, top_k, num_groups, topk_groups, dtype_code, scoring_fn,
                            group_score, renormalize, routed_scale, bias, num_valid_tokens):
     """The same into new tensors: (weights, bf16 or f32 by their code, and ids)."""
-    return L.bind().route_grouped_topk(
-        logits, top_k, num_groups, topk_groups, code_of(_SCORING, scoring_fn, "scoring_fn"),
-        code_of(_GROUP_SCORES, group_score, "group_score"), 1 if renormalize else 0, routed_scale,
-        bias, -1 if num_valid_tokens is None else max(0, num_valid_tokens), dtype_code, None,
-        None, None, None)
+    return _route_grouped(logits, top_k, num_groups, topk_groups, scoring_fn, group_score,
+                          renormalize, routed_scale, bias, num_valid_tokens, dtype_code, None,
+                          None, None, None)
 
 
 def dense_matmul_out(x, w, out, *, bias=None, act=L.ACT_NONE, act_limit=0.0, residual=None,
@@ -471,7 +474,7 @@ def block_norm_out(residual, h_out=None, *, weight=None, bias=None, y=None, r_ou
     tensor (h_out of ``h_dtype``). Returns (r_out, h_out)."""
     return L.bind().block_norm(
         residual, y, norm_weight, norm_bias, gate, scale, residual_scale, weight, bias, eps,
-        code_of(_NORMS, kind, "norm kind"), r_out, h_out, code_of(L.FLOATS, h_dtype, "out_dtype"),
+        code_of(NORMS, kind, "norm kind"), r_out, h_out, code_of(L.FLOATS, h_dtype, "out_dtype"),
         weight is not None, stream)
 
 

@@ -277,11 +277,12 @@ int dwm_combine_shared(const void* x, int x_dtype, int64_t x_rows, const int32_t
  *   out = residual_scale * residual + act(x w^T + bias)
  * x bf16 [m, k] and w bf16 [n, k] (rows ldx and ldw elements apart; every row
  * starts on 16 bytes: k, ldx and ldw are multiples of 8), products accumulated
- * in f32 (for an f32 out in parts of at most 2048 k up to k = 16384, which keeps what
- * the tensor cores cut off at 2e-6 of a sum), bias [n] (bf16 or f32, may be NULL), act one of DWM_ACT_* (SwiGLU on
- * the [gate | up] halves of w's rows: n_out = n / 2, else n), residual
- * [m, n_out] (bf16 or f32, rows ldr apart, may be NULL), out [m, n_out] (bf16
- * or f32, rows ldo apart), everything after the products in f32, rounded once.
+ * in f32 (for an f32 out in parts of at most 2048 k up to k = 16384, which keeps
+ * what the tensor cores cut off at 2e-6 of a sum), bias [n] (bf16 or f32, may be
+ * NULL), act one of DWM_ACT_* (SwiGLU on the [gate | up] halves of w's rows:
+ * n_out = n / 2, else n), residual [m, n_out] (bf16 or f32, rows ldr apart, may
+ * be NULL), out [m, n_out] (bf16 or f32, rows ldo apart), everything after the
+ * products in f32, rounded once.
  * out may be the residual itself; it must not overlap anything else. m, n and
  * the strides of residual and out are free (rows that start on 16 bytes are
  * stored faster). The result of a call depends on its shapes and values alone
