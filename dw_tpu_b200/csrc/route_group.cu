@@ -704,13 +704,18 @@ int launch(const Args& a, cudaStream_t s) {
                     "route_grouped_topk launch");
 }
 
+// Places for a lane's run: the next multiple of 4. Places that stay empty cost as much
+// as the others: 32768 tokens of 160 experts in 8 groups with a bias take 25.0 us in
+// 20 places, 29.7 in 24 and 34.7 in 32; of 96 experts 20.0 in 12 and 23.9 in 16.
 template <int LD, int LPT_LOG>
 int by_run(const Args& a, cudaStream_t s) {
   if (a.run <= 4) return launch<LD, 4, LPT_LOG>(a, s);
   if (a.run <= 8) return launch<LD, 8, LPT_LOG>(a, s);
+  if (a.run <= 12) return launch<LD, 12, LPT_LOG>(a, s);
   if (a.run <= 16) return launch<LD, 16, LPT_LOG>(a, s);
   if (a.run <= 20) return launch<LD, 20, LPT_LOG>(a, s);
   if (a.run <= 24) return launch<LD, 24, LPT_LOG>(a, s);
+  if (a.run <= 28) return launch<LD, 28, LPT_LOG>(a, s);
   if (a.run <= 32) return launch<LD, 32, LPT_LOG>(a, s);
   if constexpr (LPT_LOG == 5) return launch<LD, 64, LPT_LOG>(a, s);
   return set_error(DWM_ERR_UNSUPPORTED, "run=%d", a.run);  // (more lanes have fewer)

@@ -368,3 +368,17 @@ def test_64_bit_logits_padding_strides_and_types(dw):
         n.argsort(1, descending=True)[:, :4].tolist()
     h = torch.randn((20, 64), generator=g).half().cuda()
     _check(dw, h, 4, 8, 2)
+
+
+@pytest.mark.parametrize("per", list(range(1, 41)) + [63, 64, 100, 128])
+def test_groups_of_every_size(dw, per):
+    """Every length of a lane's run, by itself in a lane or over several."""
+    g = torch.Generator().manual_seed(per)
+    for t in (9, 2001):
+        x = torch.randn((t, 8 * per), generator=g) * 1.5
+        x[::3] = _near_groups(per, len(x[::3]), 8 * per, 8)
+        b = (torch.randn(8 * per, generator=g) * 0.1).cuda()
+        for dtype in (F32, BF):
+            y = x.to(dtype).cuda()
+            _check(dw, y, min(6, 3 * per), 8, 3, "softmax", "max")
+            _check(dw, y, min(6, 3 * per), 8, 3, "sigmoid", "top2", b)
