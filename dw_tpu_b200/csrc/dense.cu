@@ -15,10 +15,10 @@
 // With SwiGLU a tile is 64 gate rows and the 64 up rows of the same features,
 // which meet in the partial tile.
 //
-// Bound: the stream of w and, at 64 k a step, of the tile's x from L2 (24 KB a
-// step of 0.22 us at 64 rows: near the 64 bytes a clock that an SM gets from L2);
-// one CTA per SM keeps ~190 KB of copies in flight. 64 x 4096 x 4096 with SwiGLU
-// takes 10.4 us (3.3 TB/s), 64 x 4096 x 32768 48 (5.6 TB/s).
+// Bound: a fixed part of some 5 us (set-up, the first copies, the exchange of the
+// partials, the epilogue, which nothing overlaps), then the stream of w at the rate of
+// the HBM: 64 x 4096 x 4096 with SwiGLU takes 10.5 us (its bytes 5.2), twice the k 5 us
+// more, 64 x 4096 x 32768 48 (5.6 TB/s). One CTA per SM keeps ~190 KB of copies in flight.
 #include <algorithm>
 #include <atomic>
 
@@ -1304,8 +1304,8 @@ int launch(const void* x, int64_t ldx, const void* w, int64_t ldw, const Plan& p
 }  // namespace few
 
 // The kernel, and how k is split, by what they take, in us. Fitted to times of
-// every kernel and split at 170 shapes, k = 64 .. 8192, n = 16 .. 8192, m = 16 ..
-// 2048, one launch after another; HBM: w and x at 6.5 TB/s:
+// every kernel and split at 169 shapes, k = 64 .. 8192, n = 16 .. 8192, m = 16 ..
+// 2048, bf16 out without bias and residual, one launch after another; HBM: w and x at 6.5 TB/s:
 //   few, tiles of 16 x 16   1.15 + max(1.45 * HBM, waves * 0.042 * k steps of a CTA
 //                                      + CTAs an SM * (0.46 + 0.024 * k steps))
 //        tiles of 32 x 32   1.15 + max(2 * HBM, waves * 0.09 * k steps

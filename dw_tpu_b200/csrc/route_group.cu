@@ -11,14 +11,15 @@
 // A token takes 8, 16 or 32 lanes of a warp: each lane holds a run of at most 64
 // experts of one group in registers, so that the scan for the largest is the
 // same few instructions for the experts of 4, 2 or 1 tokens. The lanes work in
-// f32 and note how far apart the values are where a choice was made. Where two
-// are closer than the f32 error (a few tokens in a hundred for random logits),
-// the groups or the picks in question are compared in 64 bits; a token that
-// this does not settle, or one of whose weights f32 does not hold, is done again
-// in 64 bits by the whole warp (8-12 us, which one token of 1024 would make the
-// time of all). Bound: instruction issue; a
-// single token takes 3.9 us of dependent instructions, 32771 tokens of 160
-// experts 20 us where their bytes take 3.4 (in 64 bits throughout: 83).
+// f32 and note how far apart the values are where a choice was made: the picks
+// among themselves, the last pick and all that is left, the groups at the border.
+// Where two are closer than packing and f32 tell apart (a few tokens in a hundred
+// for random logits), they are compared value by value, and if that leaves a
+// doubt in 64 bits; a token that this does not settle, or one of whose weights
+// f32 does not hold, is done again in 64 bits by the whole warp (8-12 us, which
+// one token of 1024 would make the time of all). Bound: instruction issue; a
+// single token takes 3.4 us of dependent instructions, 32771 tokens of 160
+// experts 20.4 us where their bytes take 3.4 (in 64 bits, as f64 logits: 108).
 #include <algorithm>
 #include <type_traits>
 
@@ -796,9 +797,9 @@ extern "C" int dwm_route_grouped_topk(const void* logits, int logits_dtype, int6
   // Lanes: a power of two of groups, each of as many lanes as leave at most 32
   // experts a lane (64 where the warp has no more lanes); 8 a token at least, and
   // up to twelve tokens an SM the whole warp, for its shorter runs and its one
-  // instruction for a maximum (256 experts with a bias: one token 4.1 us against
-  // 6.0 with 8 lanes, 1024 tokens 5.1 and 6.8; 32768 tokens 45.8 and 41.5, of 160
-  // experts 49 and 24).
+  // instruction for a maximum (256 experts: one token 3.4 us against 4.9 with 8
+  // lanes, 1776 tokens 5.5 and 6.9, 2500 tokens 7.9 and 7.4, 32768 tokens 51.7 and
+  // 25.6; of 160 experts 49.9 and 18.8).
   const int lanes_log = t <= 12 * (int64_t)num_sms() ? 5 : 3;
   int groups_log = 0;
   while ((1 << groups_log) < num_groups) ++groups_log;
