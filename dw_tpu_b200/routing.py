@@ -43,8 +43,8 @@ def route_grouped_topk(gating_output: torch.Tensor, top_k: int, num_groups: int,
     The experts are ``num_groups`` (at most 32) groups of consecutive ones; the
     ``topk_groups`` best groups stay open and the ``top_k`` best experts are
     chosen in them, best first, ties to the lower index. An expert's choice
-    value is its score plus ``bias`` (the balance bias: selection only), a
-    group's the best choice in it (``group_score="max"``) or the sum of its two
+    value is its score plus ``bias`` (the balance bias, taken in f32: selection only;
+    without one the experts are in their logits' order), a group's the best choice in it (``group_score="max"``) or the sum of its two
     best ("top2"). The weights are the scores, divided by their sum if
     ``renormalize``, times ``routed_scale``. Selection is that of 64-bit scores
     whatever the logits' dtype (f64 logits take several times as long). Inference

@@ -101,3 +101,16 @@ def test_forward_mode_derivatives_are_refused():
             dw.dense_matmul(x, w)
         with fw._set_fwd_grad_enabled(False), pytest.raises(ValueError, match="CUDA"):
             dw.dense_matmul(dual(x), w)
+
+
+@pytest.mark.parametrize("kw,message", [
+    (dict(logits=(1 << 20) + 4), "misaligned"), (dict(dt=4), "dtype"), (dict(ld=63), "shorter"),
+    (dict(ids=(1 << 20) + 4 * 64 * 8 - 4), "overlaps"), (dict(t=-1), "bad shape"),
+])
+def test_refusals_of_64_bit_logits(kw, message):
+    from dw_tpu_b200 import _lib
+    a = dict(logits=1 << 20, dt=_lib.F64, ld=64, t=4, e=64, k=4, groups=8, keep=4, scoring=1, gs=1,
+             renorm=1, scale=1.0, bias=None, nv=-1, ids=2 << 20, w32=None, w16=None, stream=None)
+    a.update(kw)
+    assert _lib.load().dwm_route_grouped_topk(*a.values()) == -1
+    assert message in _lib.last_error()
