@@ -43,12 +43,13 @@ def route_grouped_topk(gating_output: torch.Tensor, top_k: int, num_groups: int,
     The experts are ``num_groups`` (at most 32) groups of consecutive ones; the
     ``topk_groups`` best groups stay open and the ``top_k`` best experts are
     chosen in them, best first, ties to the lower index. An expert's choice
-    value is its score plus ``bias`` (the balance bias, taken in f32: selection only;
-    without one the experts are in their logits' order), a group's the best choice in it (``group_score="max"``) or the sum of its two
-    best ("top2"). The weights are the scores, divided by their sum if
+    value is its score plus ``bias`` (the balance bias, taken in f32: selection
+    only; without one the experts are in their logits' order), a group's the
+    best choice in it (``group_score="max"``) or the sum of its two best
+    ("top2"). The weights are the scores, divided by their sum if
     ``renormalize``, times ``routed_scale``. Selection is that of 64-bit scores
-    whatever the logits' dtype (f64 logits take several times as long). Inference
-    only: no gradient."""
+    whatever the logits' dtype (f64 logits take several times as long).
+    Inference only: no gradient."""
     logits = gating_output
     if logits.dtype not in L.FLOATS and logits.dtype is not torch.float64:
         # f32 holds the 16- and 8-bit floats whole, f64 the integers.
