@@ -72,3 +72,33 @@ def test_every_value_of_a_long_k(m, k, n):
     assert torch.equal(off, got)
     assert torch.equal(dw.dense_matmul(x, w, bias=b, residual=got, out=got).double(),
                        2 * z + 2 * b + 0.5 * r)
+
+
+def test_two_streams_and_a_graph():
+    """Calls of every kernel with sums in parts, on two streams at once and replayed."""
+    import dw_tpu_b200 as dw
+    data = [_operands(m, k, n, seed=i) for i, (m, k, n) in
+            enumerate([(1024, 4096, 4096), (64, 8192, 16384), (129, 8192, 4096), (16, 12288, 4096)])]
+    alone = [dw.dense_matmul(x, w, out_dtype=F32) for x, w in data]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = []
+    for turn in range(10):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                x, w = data[(turn + 2 * i) % 4]
+                got.append(((turn + 2 * i) % 4, dw.dense_matmul(x, w, out_dtype=F32)))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, alone[i]) for i, y in got)
+    outs = [torch.empty_like(y) for y in alone]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for (x, w), out in zip(data, outs):
+            dw.dense_matmul(x, w, out=out)
+    for _ in range(3):
+        for out in outs:
+            out.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(y, z) for y, z in zip(outs, alone))

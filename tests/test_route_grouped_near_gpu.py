@@ -36,11 +36,12 @@ def _scores(x, scoring):
 
 def _ref(x, k, groups, keep, renorm, scoring, group_score, scale, bias):
     """(weights, ids, undecided rows) in 64 bits: values descending, ties to the
-    lower index, without a bias by the logits. Undecided: two groups at the border,
-    of different pairs of experts, whose sums lie within 2^-44 of the row's largest
-    |score| + |bias|. A score is off by a few steps of 2^-53 of itself, under softmax
-    by those of a sum of 1024 (some 2^-47), here and in the kernel; the difference of
-    two sums of two such values, twice, by less than 2^-44."""
+    lower index, without a bias by the logits. Undecided: groups of unlike pairs of
+    experts on both sides of the border, whose sums lie within 2^-44 of the row's
+    largest |score| + |bias|, or (with a bias) two unlike experts in a row that do. A
+    score is off by a few steps of 2^-53 of itself, under softmax by those of a sum of
+    1024 (some 2^-47), here and in the kernel; the difference of two sums of two such
+    values, twice, by less than 2^-44."""
     x = x.double().cpu()
     t, e = x.shape
     per = e // groups
@@ -56,19 +57,24 @@ def _ref(x, k, groups, keep, renorm, scoring, group_score, scale, bias):
         v = (s + b if bias is not None else s).reshape(t, groups, per).gather(2, at).sum(2)
     by = v.sort(dim=1, descending=True, stable=True)[1]
     undecided = torch.zeros(t, dtype=torch.bool)
+    slack = 2.0 ** -44 * (s + b.abs()).amax(1, keepdim=True)
     if keep < groups and group_score == "top2":
-        rows = torch.arange(t)
-        inside, outside = by[:, keep - 1], by[:, keep]
-        size = (s + b.abs()).amax(1)
-        near = v[rows, inside] - v[rows, outside] <= 2.0 ** -44 * size
-        of = b.expand(t, e).reshape(t, groups, per).gather(2, at)
-        same = ((pairs[rows, inside] == pairs[rows, outside]) &
-                (of[rows, inside] == of[rows, outside])).all(1)
-        undecided = near & ~same
+        in_order = v.gather(1, by)
+        near = (v - in_order[:, keep - 1:keep]).abs() <= slack
+        like = torch.cat([pairs, b.expand(t, e).reshape(t, groups, per).gather(2, at)], 2)
+        most = torch.where(near[:, :, None], like, -math.inf).amax(1)
+        least = torch.where(near[:, :, None], like, math.inf).amin(1)
+        outside = in_order[:, keep - 1] - in_order[:, keep] <= slack[:, 0]
+        undecided = outside & ~(most == least).all(1)
     open_ = torch.zeros((t, groups), dtype=torch.bool).scatter_(1, by[:, :keep], True)
     order = c.sort(dim=1, descending=True, stable=True)[1]
     is_open = open_.repeat_interleave(per, 1).gather(1, order)
-    ids = order.gather(1, (~is_open).to(torch.int8).sort(dim=1, stable=True)[1])[:, :k]
+    ids = order.gather(1, (~is_open).to(torch.int8).sort(dim=1, stable=True)[1])[:, :k + 1]
+    if bias is not None and k < keep * per:
+        picked, logit, of = c.gather(1, ids), x.gather(1, ids), b[ids]
+        unlike = (logit[:, 1:] != logit[:, :-1]) | (of[:, 1:] != of[:, :-1])
+        undecided |= ((picked[:, :-1] - picked[:, 1:] <= slack) & unlike).any(1)
+    ids = ids[:, :k]
     w = s.gather(1, ids)
     if renorm:
         total = w.sum(1, keepdim=True)
