@@ -999,7 +999,8 @@ __global__ void __launch_bounds__(THREADS, 1)
       const int part = SUMS ? PART_STEPS : kt;  // k steps of an accumulator
       for (int idx = cl; idx < total && ok; idx += ncl) {
         for (int k0 = 0; k0 < kt && ok; k0 += part) {
-          ok = __all_sync(0xffffffffu, mbar_wait(&acc_empty[slot], acc_ph ^ 1, abort_flag, a.status));
+          ok = __all_sync(0xffffffffu,
+                          mbar_wait(&acc_empty[slot], acc_ph ^ 1, abort_flag, a.status));
           if (!ok) break;
           tc_fence_after();
           const uint32_t d = tmem + (uint32_t)(slot * TILE);
@@ -1085,11 +1086,11 @@ int launch_as(const void* x, int64_t ldx, const void* w, int64_t ldw, int n, con
   tm_out = tm_res = tm_x;  // (unused without VEC, without RES)
   if (VEC && (rc = box_map(&tm_out, a.out, a.ldo, a.out_f32))) return rc;
   if (RES && (rc = box_map(&tm_res, a.residual, a.ldr, a.res_f32))) return rc;
-  rc = set_smem_limit(reinterpret_cast<const void*>(dense_pair_kernel<EPI, VEC, RES, SUMS>), L::ALLOC,
-                      "dense pair smem attribute");
+  auto fn = dense_pair_kernel<EPI, VEC, RES, SUMS>;
+  rc = set_smem_limit(reinterpret_cast<const void*>(fn), L::ALLOC, "dense pair smem attribute");
   if (rc) return rc;
   return check_cuda(
-      overlap_launch(dense_pair_kernel<EPI, VEC, RES, SUMS>,
+      overlap_launch(fn,
                      dim3(2 * (unsigned)std::min<int64_t>(tiles, resident_clusters(2))),
                      dim3(THREADS), L::ALLOC, 2, stream, tm_x, tm_w, tm_out, tm_res, a),
       "dense_matmul launch");
